@@ -592,6 +592,69 @@ int mis_comm_world(void);      /* ranks of the live communicator, 0 if none */
 int mis_allreduce_bucket(float* buf, long long n, void* stream);
 int mis_comm_finalize(void);
 
+/* ---- token operators: the channel-mixing half of a transformer stage (norm -> gated feed-forward -> projection onto the residual stream) on a level's pixels / voxels ----
+ * A token is one row of `width` consecutive values; rows lie `ld` elements apart (ld >= width, any alignment of the element type; 16-byte aligned rows are faster).  dtype is that
+ * of the activations AND the weights; biases, norm parameters and their gradients are f32, and so is what a forward pass keeps for its backward pass (mean, rstd, z, g, u).
+ * Rows: any number from 0 (a forward call then does nothing, a backward call writes zero parameter gradients).  Outputs must not overlap inputs.
+ * Workspaces belong to the call until the stream has passed it.  Sums have a fixed order: equal calls give equal bits. */
+
+/* y = (x - mean) * rstd * gamma + beta over each row's D values, rstd = 1 / sqrt(var + eps); gamma / beta NULL: 1 / 0; mean / rstd ([M] f32) NULL: not kept */
+int mis_layernorm_fwd(int dtype, const void* x, long long ldx, long long M, int D, float eps, const float* gamma, const float* beta, void* y, long long ldy, float* mean, float* rstd,
+                      void* stream);
+size_t mis_layernorm_bwd_workspace_bytes(int dtype, long long M, int D);
+/* dx, dgamma, dbeta (each may be NULL: not wanted) from dy and what the forward pass kept; parameter gradients are written, not accumulated */
+int mis_layernorm_bwd(int dtype, const void* dy, long long lddy, const void* x, long long ldx, long long M, int D, const float* gamma, const float* mean, const float* rstd,
+                      void* dx, long long lddx, float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* activations of the two products */
+#define MIS_ACT_NONE 0
+#define MIS_ACT_RELU 1
+#define MIS_ACT_GELU 2       /* z Phi(z) */
+#define MIS_ACT_GELU_TANH 3  /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define MIS_ACT_SILU 4       /* z sigmoid(z) */
+#define MIS_ACT_SIGMOID 5
+
+/* y = act(x w^T + bias) + res; w [N][K] (nn.Linear's layout) */
+typedef struct MisLinearDesc {
+    int dtype, act;
+    long long M;             /* rows */
+    int N, K;                /* width of y, width of x */
+    const void* x; long long ldx;
+    const void* w; long long ldw;
+    const float* bias;       /* [N] or NULL */
+    const void* res; long long ldres;      /* or NULL */
+    void* y; long long ldy;
+    float* z; long long ldz;               /* x w^T + bias, [M][N] f32: written by the forward pass when not NULL, read by the backward pass when act != MIS_ACT_NONE */
+    const void* dy; long long lddy;        /* backward pass: in; the gradient of res is dy itself */
+    void* dx; long long lddx;              /* out, each NULL: not wanted */
+    void* dw; long long lddw;
+    float* dbias;
+    void* workspace; size_t workspace_bytes;
+} MisLinearDesc;
+int mis_linear_fwd(const MisLinearDesc* d, void* stream);
+size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d);
+int mis_linear_bwd(const MisLinearDesc* d, void* stream);
+
+/* h = act(x wg^T + bg) * (x wu^T + bu): both projections, the activation and the product in one pass; wg, wu [F][K] */
+typedef struct MisGatedDesc {
+    int dtype, act;
+    long long M;
+    int F, K;                /* width of h, width of x */
+    const void* x; long long ldx;
+    const void* wg; const void* wu; long long ldw;
+    const float* bg; const float* bu;      /* [F] or NULL */
+    void* h; long long ldh;
+    float* g; float* u; long long ldz;     /* the two pre-activations [M][F] f32: written by the forward pass when not NULL, read by the backward pass */
+    const void* dh; long long lddh;
+    void* dx; long long lddx;
+    void* dwg; void* dwu; long long lddw;  /* together or neither */
+    float* dbg; float* dbu;
+    void* workspace; size_t workspace_bytes;
+} MisGatedDesc;
+int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream);
+size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d);
+int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,330 @@
+// C entries of the token operators' matrix products (include/misamd.h: mis_linear_*, mis_gated_ffn_*) and the element-wise part of their backward passes.
+//
+//   linear:  z = x W^T + b, y = act(z) + res          dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum_rows dz
+//   gated:   g = x Wg^T + bg, u = x Wu^T + bu,        dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, biases: row sums of dg, du
+//            h = act(g) u
+// z, g, u are kept in f32 for the backward pass: the bias gradients are f32 sums of dz, and a z rounded to bf16 would put 2^-9 into every one of their terms.  dz (dg | du) is rounded to
+// the operand type once, for the matrix instructions; the bias sums are taken before that rounding, per block of rows, and the blocks' partial rows are added in a fixed order.
+#include "tok_gemm.hpp"
+
+namespace {
+constexpr int TO_COLS = 128;          // columns of a block (16 threads x 8)
+// rows of a block: 64, more when that would leave over 512 partial rows for the second pass
+inline long long to_rows(long long M) {
+    long long r = 64;
+    while ((M + r - 1) / r > 512) r *= 2;
+    return r;
+}
+inline long long to_nblk(long long M) { return (M + to_rows(M) - 1) / to_rows(M); }
+}   // namespace
+
+// dz = dy act'(z) (MODE 0: linear), (dg | du) (MODE 1: gated), nothing but the column sums of dy (MODE 2).  A thread: 8 columns, every 16th row of its block.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, long long lddy, const float* __restrict__ z, const float* __restrict__ z2, long long ldz, int act,
+                                                     long long M, long long N, T* __restrict__ dz, long long lddz, float* __restrict__ part, float* __restrict__ part2,
+                                                     long long rows, int nrb) {
+    constexpr bool PRECISE = sizeof(T) == 4;
+    __shared__ float red[2][16][TO_COLS];
+    const int cg = threadIdx.x & 15, rl = threadIdx.x >> 4;
+    const long long rb = blockIdx.x % nrb, n = (long long)(blockIdx.x / nrb) * TO_COLS + cg * 8;
+    const int nv = N - n >= 8 ? 8 : (N > n ? (int)(N - n) : 0);
+    float s[8], s2[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = s2[i] = 0.f;
+    const long long m1 = (rb + 1) * rows < M ? (rb + 1) * rows : M;
+    if (nv > 0)
+        for (long long m = rb * rows + rl; m < m1; m += 16) {
+            float d[8];
+            tok_ldn<T>(dy + m * lddy + n, d, nv);
+            if constexpr (MODE == 0) {
+                float v[8], e[8];
+                tok_ldn<float>(z + m * ldz + n, v, nv);
+                tok_act8<PRECISE, true>(act, v, e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] *= e[i];
+                if (dz != nullptr) tok_stn<T>(dz + m * lddz + n, d, nv);
+            } else if constexpr (MODE == 1) {
+                float g[8], e[8], u[8], du[8];
+                tok_ldn<float>(z + m * ldz + n, g, nv);
+                tok_ldn<float>(z2 + m * ldz + n, u, nv);
+                tok_act8<PRECISE, true>(act, g, e);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    du[i] = d[i] * g[i];
+                    d[i] = d[i] * u[i] * e[i];
+                    s2[i] += du[i];
+                }
+                tok_stn<T>(dz + m * lddz + n, d, nv);
+                tok_stn<T>(dz + m * lddz + N + n, du, nv);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += d[i];
+        }
+    if (part == nullptr && part2 == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        red[0][rl][cg * 8 + i] = s[i];
+        if constexpr (MODE == 1) red[1][rl][cg * 8 + i] = s2[i];
+    }
+    __syncthreads();
+    const int w = threadIdx.x >> 7, c = threadIdx.x & 127;          // first 128 threads: s, the others: s2
+    const long long col = (long long)(blockIdx.x / nrb) * TO_COLS + c;
+    float* const out = w == 0 ? part : part2;
+    if ((w == 0 || MODE == 1) && out != nullptr && col < N) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t += red[w][r][c];
+        out[rb * N + col] = t;
+    }
+}
+
+// out[n] = sum over nrow rows of part[row][n], in row order per lane group, then over the 4 groups
+__global__ __launch_bounds__(256) void tok_colsum_kernel(const float* __restrict__ part, long long nrow, long long N, float* __restrict__ out) {
+    __shared__ float red[4][64];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const long long n = (long long)blockIdx.x * 64 + c;
+    float s = 0.f;
+    if (n < N)
+        for (long long r = g; r < nrow; r += 4) s += part[r * N + n];
+    red[g][c] = s;
+    __syncthreads();
+    if (g == 0 && n < N) out[n] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+
+namespace {
+template <int MODE>
+int to_dz(int dtype, const void* dy, long long lddy, const float* z, const float* z2, long long ldz, int act, long long M, long long N, void* dz, long long lddz, float* part,
+          float* part2, hipStream_t stream) {
+    const long long rows = to_rows(M), nrb = to_nblk(M), ncb = (N + TO_COLS - 1) / TO_COLS;
+    MIS_REQUIRE(nrb * ncb < (1ll << 31), MIS_EUNSUPPORTED, "token gradient: the grid is too large");
+    const dim3 grid((unsigned)(nrb * ncb));
+    if (dtype == MIS_BF16)
+        hipLaunchKernelGGL((tok_dz_kernel<__bf16, MODE>), grid, dim3(256), 0, stream, (const __bf16*)dy, lddy, z, z2, ldz, act, M, N, (__bf16*)dz, lddz, part, part2, rows, (int)nrb);
+    else
+        hipLaunchKernelGGL((tok_dz_kernel<float, MODE>), grid, dim3(256), 0, stream, (const float*)dy, lddy, z, z2, ldz, act, M, N, (float*)dz, lddz, part, part2, rows, (int)nrb);
+    MIS_LAUNCH_CHECK("token gradient");
+    return MIS_OK;
+}
+int to_colsum(const float* part, long long nrow, long long N, float* out, hipStream_t stream) {
+    hipLaunchKernelGGL(tok_colsum_kernel, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, stream, part, nrow, N, out);
+    MIS_LAUNCH_CHECK("token column sum");
+    return MIS_OK;
+}
+// the dz buffer's row pitch: whole 16-byte chunks, so that the products read it aligned whatever N is
+inline long long to_pitch(int dtype, long long n) {
+    const long long e = dtype == MIS_BF16 ? 8 : 4;
+    return (n + e - 1) / e * e;
+}
+inline size_t es_of(int dtype) { return dtype == MIS_BF16 ? 2 : 4; }
+
+constexpr long long TO_MAX = 1ll << 40;          // elements of one tensor: keeps every byte offset and workspace size far inside 64 bits
+
+int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
+    MIS_REQUIRE(dtype == MIS_F32 || dtype == MIS_BF16, MIS_EINVAL, "%s: dtype must be MIS_F32 or MIS_BF16", who);
+    MIS_REQUIRE(tok_act_ok(act), MIS_EINVAL, "%s: unknown activation %d", who, act);
+    MIS_REQUIRE(M >= 0 && N >= 1 && K >= 1, MIS_EINVAL, "%s: needs rows >= 0 and widths >= 1 (got %lld, %d, %d)", who, M, N, K);
+    MIS_REQUIRE(M < TO_MAX / N && M < TO_MAX / K, MIS_EUNSUPPORTED, "%s: %lld rows of %d / %d values are too many", who, M, N, K);
+    return MIS_OK;
+}
+#define TO_LD(who, ld, n, what) MIS_REQUIRE((ld) >= (n) && (ld) < TO_MAX, MIS_EINVAL, "%s: the row stride of " what " (%lld) is below its width", who, (long long)(ld))
+// (the grid of the largest product of a call; the launchers check it too, but only after earlier launches of the call)
+#define TO_PTR(who, p, what) MIS_REQUIRE((p) != nullptr, MIS_EINVAL, "%s: " what " is null", who)
+
+struct LinWs {
+    size_t dz, part, total;
+};
+LinWs lin_ws(const MisLinearDesc* d) {
+    LinWs w{};
+    size_t at = 0;
+    const bool act = d->act != MIS_ACT_NONE;
+    w.dz = at;
+    if (act && (d->dx != nullptr || d->dw != nullptr)) at += tok_align((size_t)d->M * to_pitch(d->dtype, d->N) * es_of(d->dtype));
+    w.part = at;
+    if (d->dbias != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->N * 4);
+    w.total = at;
+    return w;
+}
+struct GatWs {
+    size_t dz, pg, pu, total;
+};
+GatWs gat_ws(const MisGatedDesc* d) {
+    GatWs w{};
+    size_t at = 0;
+    w.dz = at;
+    at += tok_align((size_t)d->M * to_pitch(d->dtype, 2 * (long long)d->F) * es_of(d->dtype));
+    w.pg = at;
+    if (d->dbg != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
+    w.pu = at;
+    if (d->dbu != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
+    w.total = at;
+    return w;
+}
+// an empty batch has zero gradients
+__global__ void tok_zero_kernel(char* p, long long pitch, long long rows, long long bytes) {
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * bytes; i += (long long)gridDim.x * blockDim.x) p[(i / bytes) * pitch + i % bytes] = 0;
+}
+int to_zero(void* p, long long ld, long long rows, long long cols, size_t es, hipStream_t s) {
+    const long long n = rows * cols * (long long)es;
+    hipLaunchKernelGGL(tok_zero_kernel, dim3((unsigned)(n < (1 << 20) ? (n + 255) / 256 : 4096)), dim3(256), 0, s, (char*)p, ld * (long long)es, rows, cols * (long long)es);
+    MIS_LAUNCH_CHECK("token zero");
+    return MIS_OK;
+}
+#define TO_TRY(call)                       \
+    do {                                   \
+        if (const int rc__ = (call)) return rc__; \
+    } while (0)
+}   // namespace
+
+extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
+    const hipStream_t stream = (hipStream_t)stream_;
+    const char* who = "mis_linear_fwd";
+    TO_PTR(who, d, "the descriptor");
+    TO_TRY(check_dims(who, d->dtype, d->act, d->M, d->N, d->K));
+    if (d->M == 0) return MIS_OK;
+    TO_PTR(who, d->x, "x"); TO_PTR(who, d->w, "w"); TO_PTR(who, d->y, "y");
+    TO_LD(who, d->ldx, d->K, "x"); TO_LD(who, d->ldw, d->K, "w"); TO_LD(who, d->ldy, d->N, "y");
+    if (d->res != nullptr) TO_LD(who, d->ldres, d->N, "res");
+    if (d->z != nullptr) TO_LD(who, d->ldz, d->N, "z");
+    TgArgs a{};
+    a.a = TgOperand{d->x, d->x, d->ldx, TO_MAX};
+    a.b = TgOperand{d->w, d->w, d->ldw, TO_MAX};
+    a.M = d->M; a.N = d->N; a.K = d->K;
+    a.act = d->act; a.bias = d->bias; a.res = d->res; a.ldres = d->ldres;
+    a.y = a.y2 = d->y; a.ldy = d->ldy; a.msplit = TO_MAX;
+    a.z = d->z; a.ldz = d->ldz;
+    return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, stream);
+}
+
+extern "C" size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d) {
+    if (d == nullptr || check_dims("mis_linear_bwd", d->dtype, d->act, d->M, d->N, d->K) != MIS_OK) return 0;
+    return lin_ws(d).total;
+}
+
+extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
+    const hipStream_t stream = (hipStream_t)stream_;
+    const char* who = "mis_linear_bwd";
+    TO_PTR(who, d, "the descriptor");
+    TO_TRY(check_dims(who, d->dtype, d->act, d->M, d->N, d->K));
+    const size_t es = es_of(d->dtype);
+    if (d->dw != nullptr) TO_LD(who, d->lddw, d->K, "dw");
+    if (d->M == 0) {
+        if (d->dw != nullptr) TO_TRY(to_zero(d->dw, d->lddw, d->N, d->K, es, stream));
+        if (d->dbias != nullptr) TO_TRY(to_zero(d->dbias, d->N, 1, d->N, 4, stream));
+        return MIS_OK;
+    }
+    const bool act = d->act != MIS_ACT_NONE, prod = d->dx != nullptr || d->dw != nullptr;
+    TO_PTR(who, d->dy, "dy");
+    TO_LD(who, d->lddy, d->N, "dy");
+    if (act) { TO_PTR(who, d->z, "z (the forward pass keeps it)"); TO_LD(who, d->ldz, d->N, "z"); }
+    if (d->dx != nullptr) { TO_PTR(who, d->w, "w"); TO_LD(who, d->ldw, d->K, "w"); TO_LD(who, d->lddx, d->K, "dx"); }
+    if (d->dw != nullptr) { TO_PTR(who, d->x, "x"); TO_LD(who, d->ldx, d->K, "x"); }
+    const LinWs w = lin_ws(d);
+    MIS_REQUIRE(w.total == 0 || (d->workspace != nullptr && d->workspace_bytes >= w.total), MIS_EINVAL, "%s: the workspace has %zu bytes, %zu are needed", who, d->workspace_bytes, w.total);
+    char* const ws = (char*)d->workspace;
+    const void* dz = d->dy;
+    long long lddz = d->lddy;
+    float* const part = d->dbias != nullptr ? (float*)(ws + w.part) : nullptr;
+    if (act && (prod || part != nullptr)) {
+        lddz = to_pitch(d->dtype, d->N);
+        TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->z, nullptr, d->ldz, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, lddz, part, nullptr, stream));
+        dz = ws + w.dz;
+    } else if (part != nullptr) {
+        TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, nullptr, 0, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
+    }
+    if (part != nullptr) TO_TRY(to_colsum(part, to_nblk(d->M), d->N, d->dbias, stream));
+    if (d->dx != nullptr) {
+        TgArgs a{};
+        a.a = TgOperand{dz, dz, lddz, TO_MAX};
+        a.b = TgOperand{d->w, d->w, d->ldw, TO_MAX};
+        a.M = d->M; a.N = d->K; a.K = d->N;
+        a.y = a.y2 = d->dx; a.ldy = d->lddx; a.msplit = TO_MAX;
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_LINEAR, a, stream));
+    }
+    if (d->dw != nullptr) {
+        TgArgs a{};
+        a.a = TgOperand{dz, dz, lddz, TO_MAX};
+        a.b = TgOperand{d->x, d->x, d->ldx, TO_MAX};
+        a.M = d->N; a.N = d->K; a.K = d->M;
+        a.y = a.y2 = d->dw; a.ldy = d->lddw; a.msplit = TO_MAX;
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_LINEAR, a, stream));
+    }
+    return MIS_OK;
+}
+
+extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
+    const hipStream_t stream = (hipStream_t)stream_;
+    const char* who = "mis_gated_ffn_fwd";
+    TO_PTR(who, d, "the descriptor");
+    TO_TRY(check_dims(who, d->dtype, d->act, d->M, d->F, d->K));
+    if (d->M == 0) return MIS_OK;
+    TO_PTR(who, d->x, "x"); TO_PTR(who, d->wg, "wg"); TO_PTR(who, d->wu, "wu"); TO_PTR(who, d->h, "h");
+    TO_LD(who, d->ldx, d->K, "x"); TO_LD(who, d->ldw, d->K, "wg / wu"); TO_LD(who, d->ldh, d->F, "h");
+    MIS_REQUIRE((d->g == nullptr) == (d->u == nullptr), MIS_EINVAL, "%s: g and u are kept together", who);
+    if (d->g != nullptr) TO_LD(who, d->ldz, d->F, "g / u");
+    TgArgs a{};
+    a.a = TgOperand{d->x, d->x, d->ldx, TO_MAX};
+    a.b = TgOperand{d->wg, d->wu, d->ldw, TO_MAX};
+    a.M = d->M; a.N = d->F; a.K = d->K;
+    a.act = d->act; a.bias = d->bg; a.bias2 = d->bu;
+    a.y = a.y2 = d->h; a.ldy = d->ldh; a.msplit = TO_MAX;
+    a.z = d->g; a.z2 = d->u; a.ldz = d->ldz;
+    return tg_launch(d->dtype, 0, 0, TG_GATED, a, stream);
+}
+
+extern "C" size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d) {
+    if (d == nullptr || check_dims("mis_gated_ffn_bwd", d->dtype, d->act, d->M, d->F, d->K) != MIS_OK) return 0;
+    return gat_ws(d).total;
+}
+
+extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
+    const hipStream_t stream = (hipStream_t)stream_;
+    const char* who = "mis_gated_ffn_bwd";
+    TO_PTR(who, d, "the descriptor");
+    TO_TRY(check_dims(who, d->dtype, d->act, d->M, d->F, d->K));
+    const size_t es = es_of(d->dtype);
+    MIS_REQUIRE((d->dwg == nullptr) == (d->dwu == nullptr), MIS_EINVAL, "%s: dwg and dwu come together", who);
+    if (d->dwg != nullptr) TO_LD(who, d->lddw, d->K, "dwg / dwu");
+    if (d->M == 0) {
+        if (d->dwg != nullptr) {
+            TO_TRY(to_zero(d->dwg, d->lddw, d->F, d->K, es, stream));
+            TO_TRY(to_zero(d->dwu, d->lddw, d->F, d->K, es, stream));
+        }
+        if (d->dbg != nullptr) TO_TRY(to_zero(d->dbg, d->F, 1, d->F, 4, stream));
+        if (d->dbu != nullptr) TO_TRY(to_zero(d->dbu, d->F, 1, d->F, 4, stream));
+        return MIS_OK;
+    }
+    TO_PTR(who, d->dh, "dh"); TO_PTR(who, d->g, "g (the forward pass keeps it)"); TO_PTR(who, d->u, "u (the forward pass keeps it)");
+    TO_LD(who, d->lddh, d->F, "dh"); TO_LD(who, d->ldz, d->F, "g / u");
+    if (d->dx != nullptr) {
+        TO_PTR(who, d->wg, "wg"); TO_PTR(who, d->wu, "wu");
+        TO_LD(who, d->ldw, d->K, "wg / wu"); TO_LD(who, d->lddx, d->K, "dx");
+    }
+    if (d->dwg != nullptr) { TO_PTR(who, d->x, "x"); TO_LD(who, d->ldx, d->K, "x"); }
+    const GatWs w = gat_ws(d);
+    MIS_REQUIRE(d->workspace != nullptr && d->workspace_bytes >= w.total, MIS_EINVAL, "%s: the workspace has %zu bytes, %zu are needed", who, d->workspace_bytes, w.total);
+    char* const ws = (char*)d->workspace;
+    const long long F = d->F, lddz = to_pitch(d->dtype, 2 * F);
+    float* const pg = d->dbg != nullptr ? (float*)(ws + w.pg) : nullptr;
+    float* const pu = d->dbu != nullptr ? (float*)(ws + w.pu) : nullptr;
+    void* const dz = ws + w.dz;          // [M][dg (F) | du (F)]
+    TO_TRY(to_dz<1>(d->dtype, d->dh, d->lddh, d->g, d->u, d->ldz, d->act, d->M, F, dz, lddz, pg, pu, stream));
+    if (pg != nullptr) TO_TRY(to_colsum(pg, to_nblk(d->M), F, d->dbg, stream));
+    if (pu != nullptr) TO_TRY(to_colsum(pu, to_nblk(d->M), F, d->dbu, stream));
+    if (d->dx != nullptr) {
+        TgArgs a{};
+        a.a = TgOperand{dz, dz, lddz, TO_MAX};
+        a.b = TgOperand{d->wg, d->wu, d->ldw, F};
+        a.M = d->M; a.N = d->K; a.K = 2 * F;
+        a.y = a.y2 = d->dx; a.ldy = d->lddx; a.msplit = TO_MAX;
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_LINEAR, a, stream));
+    }
+    if (d->dwg != nullptr) {
+        TgArgs a{};
+        a.a = TgOperand{dz, dz, lddz, TO_MAX};
+        a.b = TgOperand{d->x, d->x, d->ldx, TO_MAX};
+        a.M = 2 * F; a.N = d->K; a.K = d->M;
+        a.y = d->dwg; a.y2 = d->dwu; a.ldy = d->lddw; a.msplit = F;
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_LINEAR, a, stream));
+    }
+    return MIS_OK;
+}

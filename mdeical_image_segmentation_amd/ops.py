@@ -1021,3 +1021,179 @@ def gather3d_bwd(dy, dx, ranges):
         raise MisError("gather3d_bwd: slices / ranges do not match")
     check(lib.mis_gather3d_bwd(dtype_code(dy.dtype), dy.ptr, dy.ld, dx.ptr, dx.ld, dx.N, dx.D, dx.H, dx.W, dy.D, dy.H, dy.W, dx.C, ranges[0].data_ptr(),
                                ranges[1].data_ptr(), ranges[2].data_ptr(), stream_ptr()), "mis_gather3d_bwd")
+
+
+# ---- token operators (csrc/layernorm.hip, tok_gemm.hip, token_ops.hip): rows of a 2-D tensor; `tokens` holds the differentiable functions over them ----
+ACT_CODES_TOKEN = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+
+def token_act(name):
+    try:
+        return ACT_CODES_TOKEN[name]
+    except (KeyError, TypeError):
+        raise MisError(f"activation must be one of {sorted(k for k in ACT_CODES_TOKEN if k)} or None, got {name!r}") from None
+
+
+class _TokenCall:
+    """argument checks of one call: every tensor on one GPU, the rows of a matrix `ld` elements apart with unit stride inside, vectors contiguous"""
+
+    def __init__(self, who, ref):
+        if not isinstance(ref, torch.Tensor) or ref.device.type != "cuda":
+            raise MisError(f"{who}: runs on MI355X only: got {ref.device if isinstance(ref, torch.Tensor) else type(ref)} (no CPU fallback)")
+        self.who, self.device, self.dtype = who, ref.device, ref.dtype
+        self.code = dtype_code(ref.dtype)
+
+    def mat(self, t, name, rows, cols, dtype=None):
+        """(pointer, row stride) of a [rows][cols] matrix"""
+        dtype = self.dtype if dtype is None else dtype
+        if t.device != self.device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+            raise MisError(f"{self.who}: {name} must be a ({rows}, {cols}) {dtype} tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        s0, s1 = t.stride()
+        if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
+            raise MisError(f"{self.who}: {name} must have unit stride inside its rows and rows that do not overlap, got strides {(s0, s1)}")
+        return t.data_ptr(), (s0 if rows > 1 else cols)
+
+    def vec(self, t, name, n):
+        """pointer of a contiguous f32 vector, None for None"""
+        if t is None:
+            return None
+        if t.device != self.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+            raise MisError(f"{self.who}: {name} must be a contiguous ({n},) float32 tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    def run(self, fn, *args):
+        if self.device.index == torch.cuda.current_device():
+            check(fn(*args, stream_ptr()), self.who)
+        else:
+            with torch.cuda.device(self.device):
+                check(fn(*args, stream_ptr()), self.who)
+
+    def scratch(self, nbytes):
+        """a call's own workspace, from the caching allocator: two streams, two captured graphs never share one"""
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+
+
+def layernorm_fwd(x, y, gamma=None, beta=None, mean=None, rstd=None, eps=1e-5):
+    """y = (x - mean) * rstd * gamma + beta over the rows of x (M, D); mean, rstd (M,) f32 are written when given (mis_layernorm_fwd)"""
+    c = _TokenCall("layernorm_fwd", x)
+    if x.dim() != 2:
+        raise MisError(f"layernorm_fwd: x must be a matrix of rows, got {tuple(x.shape)}")
+    M, D = x.shape
+    (px, ldx), (py, ldy) = c.mat(x, "x", M, D), c.mat(y, "y", M, D)
+    c.run(load().mis_layernorm_fwd, c.code, px, ldx, M, D, float(eps), c.vec(gamma, "gamma", D), c.vec(beta, "beta", D), py, ldy, c.vec(mean, "mean", M), c.vec(rstd, "rstd", M))
+
+
+def layernorm_bwd(dy, x, mean, rstd, gamma=None, dx=None, dgamma=None, dbeta=None):
+    """the wanted ones of dx (M, D), dgamma, dbeta (D,) f32 from dy and the forward pass's x, mean, rstd (mis_layernorm_bwd); written, not accumulated"""
+    c = _TokenCall("layernorm_bwd", x)
+    if x.dim() != 2:
+        raise MisError(f"layernorm_bwd: x must be a matrix of rows, got {tuple(x.shape)}")
+    M, D = x.shape
+    (px, ldx), (pd, ldd) = c.mat(x, "x", M, D), c.mat(dy, "dy", M, D)
+    pdx, lddx = (None, D) if dx is None else c.mat(dx, "dx", M, D)
+    lib = load()
+    ws = c.scratch(lib.mis_layernorm_bwd_workspace_bytes(c.code, M, D) if dgamma is not None or dbeta is not None else 0)
+    c.run(lib.mis_layernorm_bwd, c.code, pd, ldd, px, ldx, M, D, c.vec(gamma, "gamma", D), c.vec(mean, "mean", M), c.vec(rstd, "rstd", M), pdx, lddx,
+          c.vec(dgamma, "dgamma", D), c.vec(dbeta, "dbeta", D), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+
+
+def _linear_desc(c, x, w, act):
+    if x.dim() != 2 or w.dim() != 2:
+        raise MisError(f"{c.who}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
+    d = _lib.LinearDesc()
+    d.dtype, d.act = c.code, token_act(act)
+    d.M, d.K, d.N = x.shape[0], x.shape[1], w.shape[0]
+    d.x, d.ldx = c.mat(x, "x", d.M, d.K)
+    d.w, d.ldw = c.mat(w, "w", d.N, d.K)
+    return d
+
+
+def linear_fwd(x, w, y, bias=None, act=None, res=None, z=None):
+    """y = act(x w^T + bias) + res: x (M, K), w (N, K), y (M, N), bias (N,) f32, res like y; z (M, N) f32 receives x w^T + bias for linear_bwd (mis_linear_fwd)"""
+    c = _TokenCall("linear_fwd", x)
+    d = _linear_desc(c, x, w, act)
+    d.bias = c.vec(bias, "bias", d.N)
+    d.y, d.ldy = c.mat(y, "y", d.M, d.N)
+    if res is not None:
+        d.res, d.ldres = c.mat(res, "res", d.M, d.N)
+    if z is not None:
+        d.z, d.ldz = c.mat(z, "z", d.M, d.N, torch.float32)
+    c.run(load().mis_linear_fwd, C.byref(d))
+
+
+def linear_bwd(dy, x, w, act=None, z=None, dx=None, dw=None, dbias=None):
+    """the wanted ones of dx (M, K), dw (N, K), dbias (N,) f32 from dy (M, N) and, with an activation, the forward pass's z (mis_linear_bwd); written, not accumulated"""
+    c = _TokenCall("linear_bwd", x)
+    d = _linear_desc(c, x, w, act)
+    d.dy, d.lddy = c.mat(dy, "dy", d.M, d.N)
+    if d.act and z is None:
+        raise MisError("linear_bwd: with an activation the forward pass has to keep z")
+    if z is not None:
+        d.z, d.ldz = c.mat(z, "z", d.M, d.N, torch.float32)
+    if dx is not None:
+        d.dx, d.lddx = c.mat(dx, "dx", d.M, d.K)
+    if dw is not None:
+        d.dw, d.lddw = c.mat(dw, "dw", d.N, d.K)
+    d.dbias = c.vec(dbias, "dbias", d.N)
+    lib = load()
+    ws = c.scratch(lib.mis_linear_bwd_workspace_bytes(C.byref(d)))
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+    c.run(lib.mis_linear_bwd, C.byref(d))
+
+
+def _gated_desc(c, x, wg, wu, act):
+    if x.dim() != 2 or wg.dim() != 2:
+        raise MisError(f"{c.who}: x, wg and wu must be matrices, got {tuple(x.shape)}, {tuple(wg.shape)}, {tuple(wu.shape)}")
+    d = _lib.GatedDesc()
+    d.dtype, d.act = c.code, token_act(act)
+    d.M, d.K, d.F = x.shape[0], x.shape[1], wg.shape[0]
+    d.x, d.ldx = c.mat(x, "x", d.M, d.K)
+    d.wg, d.ldw = c.mat(wg, "wg", d.F, d.K)
+    d.wu, ldu = c.mat(wu, "wu", d.F, d.K)
+    if ldu != d.ldw:
+        raise MisError(f"{c.who}: wg and wu must have the same row stride, got {d.ldw} and {ldu}")
+    return d
+
+
+def gated_ffn_fwd(x, wg, wu, h, bg=None, bu=None, act="silu", g=None, u=None):
+    """h = act(x wg^T + bg) * (x wu^T + bu): x (M, K), wg / wu (F, K), h (M, F), bg / bu (F,) f32; g, u (M, F) f32 receive the two pre-activations for gated_ffn_bwd
+    (mis_gated_ffn_fwd)"""
+    c = _TokenCall("gated_ffn_fwd", x)
+    d = _gated_desc(c, x, wg, wu, act)
+    d.bg, d.bu = c.vec(bg, "bg", d.F), c.vec(bu, "bu", d.F)
+    d.h, d.ldh = c.mat(h, "h", d.M, d.F)
+    if (g is None) != (u is None):
+        raise MisError("gated_ffn_fwd: g and u are kept together")
+    if g is not None:
+        d.g, d.ldz = c.mat(g, "g", d.M, d.F, torch.float32)
+        d.u, ldu = c.mat(u, "u", d.M, d.F, torch.float32)
+        if ldu != d.ldz:
+            raise MisError("gated_ffn_fwd: g and u must have the same row stride")
+    c.run(load().mis_gated_ffn_fwd, C.byref(d))
+
+
+def gated_ffn_bwd(dh, x, wg, wu, g, u, act="silu", dx=None, dwg=None, dwu=None, dbg=None, dbu=None):
+    """the wanted ones of dx (M, K), dwg / dwu (F, K; together), dbg, dbu (F,) f32 from dh (M, F) and the forward pass's g, u (mis_gated_ffn_bwd); written, not accumulated"""
+    c = _TokenCall("gated_ffn_bwd", x)
+    d = _gated_desc(c, x, wg, wu, act)
+    d.dh, d.lddh = c.mat(dh, "dh", d.M, d.F)
+    d.g, d.ldz = c.mat(g, "g", d.M, d.F, torch.float32)
+    d.u, ldu = c.mat(u, "u", d.M, d.F, torch.float32)
+    if ldu != d.ldz:
+        raise MisError("gated_ffn_bwd: g and u must have the same row stride")
+    if dx is not None:
+        d.dx, d.lddx = c.mat(dx, "dx", d.M, d.K)
+    if (dwg is None) != (dwu is None):
+        raise MisError("gated_ffn_bwd: dwg and dwu come together")
+    if dwg is not None:
+        d.dwg, d.lddw = c.mat(dwg, "dwg", d.F, d.K)
+        d.dwu, ldd = c.mat(dwu, "dwu", d.F, d.K)
+        if ldd != d.lddw:
+            raise MisError("gated_ffn_bwd: dwg and dwu must have the same row stride")
+    d.dbg, d.dbu = c.vec(dbg, "dbg", d.F), c.vec(dbu, "dbu", d.F)
+    lib = load()
+    ws = c.scratch(lib.mis_gated_ffn_bwd_workspace_bytes(C.byref(d)))
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+    c.run(lib.mis_gated_ffn_bwd, C.byref(d))

@@ -1,0 +1,128 @@
+"""Token operators without a GPU: what the Python and the C entries refuse, and the oracle against torch's own differentiation in 64 bits."""
+import ctypes as C
+
+import pytest
+import torch
+
+from mdeical_image_segmentation_amd import _lib, ops, tokens
+from mdeical_image_segmentation_amd._lib import MisError
+from oracle import tokens_oracle as O
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.randn(4, 8), torch.randn(6, 8)
+    for call in (lambda: tokens.layer_norm(x), lambda: tokens.linear(x, w), lambda: tokens.gated_ffn(x, w, w), lambda: ops.layernorm_fwd(x, x), lambda: ops.linear_fwd(x, w, x)):
+        with pytest.raises(MisError, match="MI355X"):
+            call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda x, w: tokens.linear(x, w[:, :7]), lambda x, w: tokens.linear(x, w[0]), lambda x, w: tokens.linear(x, w, residual=x), lambda x, w: tokens.gated_ffn(x[..., :0], w, w),
+    lambda x, w: tokens.linear(torch.tensor(1.0), w), lambda x, w: ops.token_act("swish"), lambda x, w: ops.token_act(["gelu"])])
+def test_wrong_shapes_and_names_are_refused(call):
+    with pytest.raises(MisError):
+        call(torch.randn(4, 8), torch.randn(6, 8))
+
+
+def _lin(**kw):
+    d = _lib.LinearDesc()
+    d.dtype, d.M, d.N, d.K = _lib.MIS_F32, 4, 6, 8
+    d.ldx = d.ldw = d.lddx = d.lddw = 8
+    d.ldy = d.lddy = d.ldz = d.ldres = 6
+    d.x = d.w = d.y = d.dy = d.z = d.dx = 4096          # never reached: each call below is refused before a launch
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _gat(**kw):
+    d = _lib.GatedDesc()
+    d.dtype, d.act, d.M, d.F, d.K = _lib.MIS_BF16, 4, 4, 6, 8
+    d.ldx = d.ldw = d.lddx = d.lddw = 8
+    d.ldh = d.lddh = d.ldz = 6
+    d.x = d.wg = d.wu = d.h = d.dh = d.g = d.u = d.dx = 4096
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw, word", [({"dtype": 2}, b"dtype"), ({"act": 6}, b"activation"), ({"act": -1}, b"activation"), ({"M": -1}, b"rows"), ({"N": 0}, b"width"), ({"K": 0}, b"width"),
+                                      ({"x": None}, b"null"), ({"w": None}, b"null"), ({"y": None}, b"null"), ({"ldx": 7}, b"stride"), ({"ldw": 7}, b"stride"), ({"ldy": 5}, b"stride"),
+                                      ({"ldz": 5}, b"stride"), ({"res": 4096, "ldres": 5}, b"stride"), ({"M": 1 << 60}, b"too many")])
+def test_linear_fwd_refuses(kw, word):
+    lib = _lib.load()
+    assert lib.mis_linear_fwd(C.byref(_lin(**kw)), None) < 0
+    assert word in lib.mis_last_error()
+
+
+@pytest.mark.parametrize("kw, word", [({"dtype": 9}, b"dtype"), ({"dy": None}, b"null"), ({"lddy": 5}, b"stride"), ({"lddx": 7}, b"stride"), ({"dw": 4096, "lddw": 7}, b"stride"),
+                                      ({"dw": 4096, "x": None}, b"null"), ({"act": 2, "z": None}, b"keeps"), ({"act": 2}, b"workspace"), ({"dbias": 4096}, b"workspace"),
+                                      ({"act": 2, "workspace": 4096, "workspace_bytes": 64}, b"workspace")])
+def test_linear_bwd_refuses(kw, word):
+    lib = _lib.load()
+    assert lib.mis_linear_bwd(C.byref(_lin(**kw)), None) < 0
+    assert word in lib.mis_last_error()
+
+
+@pytest.mark.parametrize("kw, word", [({"dtype": 2}, b"dtype"), ({"act": 9}, b"activation"), ({"F": 0}, b"width"), ({"wu": None}, b"null"), ({"h": None}, b"null"), ({"ldh": 5}, b"stride"),
+                                      ({"u": None}, b"together"), ({"ldz": 5}, b"stride")])
+def test_gated_fwd_refuses(kw, word):
+    lib = _lib.load()
+    assert lib.mis_gated_ffn_fwd(C.byref(_gat(**kw)), None) < 0
+    assert word in lib.mis_last_error()
+
+
+@pytest.mark.parametrize("kw, word", [({"dh": None}, b"null"), ({"g": None}, b"keeps"), ({"u": None}, b"keeps"), ({"dwg": 4096}, b"together"), ({"lddh": 5}, b"stride"), ({}, b"workspace")])
+def test_gated_bwd_refuses(kw, word):
+    lib = _lib.load()
+    assert lib.mis_gated_ffn_bwd(C.byref(_gat(**kw)), None) < 0
+    assert word in lib.mis_last_error()
+
+
+def test_layernorm_refuses():
+    lib = _lib.load()
+    p = 4096
+    assert lib.mis_layernorm_fwd(5, p, 8, 4, 8, 1e-5, None, None, p, 8, None, None, None) < 0 and b"dtype" in lib.mis_last_error()
+    assert lib.mis_layernorm_fwd(0, p, 8, 4, 0, 1e-5, None, None, p, 8, None, None, None) < 0 and b"width" in lib.mis_last_error()
+    assert lib.mis_layernorm_fwd(0, p, 7, 4, 8, 1e-5, None, None, p, 8, None, None, None) < 0 and b"stride" in lib.mis_last_error()
+    assert lib.mis_layernorm_fwd(0, None, 8, 4, 8, 1e-5, None, None, p, 8, None, None, None) < 0 and b"null" in lib.mis_last_error()
+    assert lib.mis_layernorm_fwd(0, p, 8, 1 << 40, 8, 1e-5, None, None, p, 8, None, None, None) < 0 and b"grid" in lib.mis_last_error()
+    assert lib.mis_layernorm_fwd(0, p, 1 << 23, 4, 1 << 23, 1e-5, None, None, p, 1 << 23, None, None, None) < 0 and b"2^22" in lib.mis_last_error()
+    assert lib.mis_layernorm_bwd(0, p, 8, p, 8, 4, 8, None, p, None, p, 8, p, p, p, 1 << 20, None) < 0 and b"null" in lib.mis_last_error()
+    assert lib.mis_layernorm_bwd(0, p, 8, p, 8, 4, 8, None, p, p, p, 8, p, p, p, 16, None) < 0 and b"workspace" in lib.mis_last_error()
+
+
+def test_null_descriptors_are_refused():
+    lib = _lib.load()
+    for f in (lib.mis_linear_fwd, lib.mis_linear_bwd, lib.mis_gated_ffn_fwd, lib.mis_gated_ffn_bwd):
+        assert f(None, None) < 0 and b"null" in lib.mis_last_error()
+    assert lib.mis_linear_bwd_workspace_bytes(None) == 0 and lib.mis_gated_ffn_bwd_workspace_bytes(None) == 0
+
+
+def test_empty_batches_are_no_error():
+    lib = _lib.load()
+    assert lib.mis_linear_fwd(C.byref(_lin(M=0)), None) == 0
+    assert lib.mis_gated_ffn_fwd(C.byref(_gat(M=0)), None) == 0
+    assert lib.mis_layernorm_fwd(0, None, 8, 0, 8, 1e-5, None, None, None, 8, None, None, None) == 0
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
+def test_oracle_gradients_are_torchs(name):
+    g = torch.Generator().manual_seed(5)
+    x, w, v, b, c, r, dy = (torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((7, 5), (6, 5), (6, 5), (6,), (6,), (7, 6), (7, 6)))
+    f = {"none": lambda t: t, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "gelu_tanh": lambda t: torch.nn.functional.gelu(t, approximate="tanh"),
+         "silu": torch.nn.functional.silu, "sigmoid": torch.sigmoid}[name]
+    y = f(x @ w.t() + b) + r
+    o = O.linear(x, w, b, name, r, dy)
+    for got, want in zip((y, *torch.autograd.grad(y, (x, w, b), dy.detach())), (o["y"], o["dx"], o["dw"], o["db"])):
+        torch.testing.assert_close(want[0], got.detach(), rtol=1e-12, atol=1e-12)
+    y = f(x @ w.t() + b) * (x @ v.t() + c)
+    o = O.gated(x, w, v, b, c, name, dy)
+    for got, want in zip((y, *torch.autograd.grad(y, (x, w, v, b, c), dy.detach())), (o["y"], o["dx"], o["dwg"], o["dwu"], o["dbg"], o["dbu"])):
+        torch.testing.assert_close(want[0], got.detach(), rtol=1e-12, atol=1e-12)
+    gam, bet = w[:, 0].detach().clone().requires_grad_(), b
+    dz = torch.randn(7, 6, generator=g, dtype=torch.float64)
+    y = torch.nn.functional.layer_norm(r, (6,), gam, bet, 1e-5)
+    o = O.layer_norm(r, gam, bet, 1e-5, dz)
+    for got, want in zip((y, *torch.autograd.grad(y, (r, gam, bet), dz)), (o["y"], o["dx"], o["dw"], o["db"])):
+        torch.testing.assert_close(want[0], got.detach(), rtol=1e-12, atol=1e-12)
