@@ -1,0 +1,59 @@
+// Epilogues of the token products: a lane holds runs of 8 consecutive columns of one row.
+#pragma once
+#include "tok_gemm.hpp"
+
+// y = act(v + bias) + res, v (+ bias) kept in z
+template <typename T> struct TgLinearRow {
+    const TgArgs& a;
+    long long n;            // first column of the run
+    int nv;                 // columns of it inside the matrix
+    void* y;
+    float bias[8];
+    __device__ __forceinline__ TgLinearRow(const TgArgs& a_, void* y_, long long n_) : a(a_), n(n_), nv(a_.N - n_ >= 8 ? 8 : (int)(a_.N - n_)), y(y_) {
+        if (a.bias != nullptr && nv > 0) tok_ldn<float>(a.bias + n, bias, nv);
+    }
+    __device__ __forceinline__ void operator()(long long m, float (&v)[8]) const {
+        if (a.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += bias[j];
+        }
+        if (a.z != nullptr) tok_stn<float>(a.z + m * a.ldz + n, v, nv);
+        tok_act8<sizeof(T) == 4, false>(a.act, v, nullptr);
+        if (a.res != nullptr) {
+            float r[8];
+            tok_ldn<T>(reinterpret_cast<const T*>(a.res) + m * a.ldres + n, r, nv);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += r[j];
+        }
+        tok_stn<T>(reinterpret_cast<T*>(y) + m * a.ldy + n, v, nv);
+    }
+};
+// h = act(g + bg) (u + bu), the two sums kept in z, z2
+template <typename T> struct TgGatedRow {
+    const TgArgs& a;
+    long long n;
+    int nv;
+    float bg[8], bu[8];
+    __device__ __forceinline__ TgGatedRow(const TgArgs& a_, long long n_) : a(a_), n(n_), nv(a_.N - n_ >= 8 ? 8 : (int)(a_.N - n_)) {
+        if (a.bias != nullptr && nv > 0) tok_ldn<float>(a.bias + n, bg, nv);
+        if (a.bias2 != nullptr && nv > 0) tok_ldn<float>(a.bias2 + n, bu, nv);
+    }
+    __device__ __forceinline__ void operator()(long long m, float (&g)[8], float (&u)[8]) const {
+        if (a.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] += bg[j];
+        }
+        if (a.bias2 != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] += bu[j];
+        }
+        if (a.z != nullptr) {
+            tok_stn<float>(a.z + m * a.ldz + n, g, nv);
+            tok_stn<float>(a.z2 + m * a.ldz + n, u, nv);
+        }
+        tok_act8<sizeof(T) == 4, false>(a.act, g, nullptr);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= u[j];
+        tok_stn<T>(reinterpret_cast<T*>(a.y) + m * a.ldy + n, g, nv);
+    }
+};

@@ -3,27 +3,35 @@
 #pragma once
 #include "tok_common.hpp"
 
+// A product may run over two ranges of k (dx = dg Wg + du Wu: range 0 on p, range 1 on p2, K long each) or be two products of one shape (dWg = dg^T x, dWu = du^T x: batch 1 reads a.p2 and
+// writes y2).  The gated forward product takes the rows of the "up" projection from b.p2.
 struct TgOperand {
     const void* p;          // element (i, k): p[i * ld + k] (k contiguous) or p[k * ld + i]
-    const void* p2;         // second tensor of a pair: the columns of the "up" projection (EPI gated), or the k >= split of (gate | up) weights
+    const void* p2;
     long long ld;
-    long long split;
 };
-enum { TG_LINEAR = 0, TG_GATED = 1 };
+enum { TG_LINEAR = 0, TG_GATED = 1, TG_STORE = 2, TG_SLAB = 3 };          // epilogues: forward products; a rounded store (gradients); an f32 slab of one part of k (internal)
 struct TgArgs {
     TgOperand a, b;
     long long M, N, K;      // gated: N = columns of h; the products have 2 N
+    int ranges, batches;    // 1 or 2
     int act;
     const float* bias;      // [N] or null
     const float* bias2;     // gated: of the up projection
     const void* res;        // linear: added after the activation, or null
     long long ldres;
-    void* y;                // [M][N]; rows m >= msplit go to y2
+    void* y;                // [M][N]
     void* y2;
-    long long ldy, msplit;
+    long long ldy;
     float* z;               // pre-activation(s) kept for the backward pass, [M][N] f32, or null
     float* z2;
     long long ldz;
 };
-// dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_*.  Enqueues on `stream`.
-int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, hipStream_t stream);
+// dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_LINEAR, TG_GATED or TG_STORE.  Enqueues on `stream`.  A TG_STORE product may be cut along
+// k: its parts go to `slab` (tg_slab_bytes) and are added in their order.
+int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream);
+size_t tg_slab_bytes(int dtype, long long M, long long N, long long K, int ranges, int batches);
+
+// tok_gemm_pp.hip; tok_gemm.hip
+int tg_pp_launch(int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, int splits, hipStream_t stream);
+int tg_slab_sum(int dtype, const TgArgs& a, const float* slab, int splits, hipStream_t stream);

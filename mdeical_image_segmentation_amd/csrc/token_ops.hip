@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
                     s2[i] += du[i];
                 }
                 tok_stn<T>(dz + m * lddz + n, d, nv);
-                tok_stn<T>(dz + m * lddz + N + n, du, nv);
+                tok_stn<T>(dz + m * lddz + (lddz >> 1) + n, du, nv);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] += d[i];
@@ -130,8 +130,9 @@ int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
 // (the grid of the largest product of a call; the launchers check it too, but only after earlier launches of the call)
 #define TO_PTR(who, p, what) MIS_REQUIRE((p) != nullptr, MIS_EINVAL, "%s: " what " is null", who)
 
+size_t most(size_t a, size_t b) { return a > b ? a : b; }
 struct LinWs {
-    size_t dz, part, total;
+    size_t dz, part, slab, total;
 };
 LinWs lin_ws(const MisLinearDesc* d) {
     LinWs w{};
@@ -141,21 +142,25 @@ LinWs lin_ws(const MisLinearDesc* d) {
     if (act && (d->dx != nullptr || d->dw != nullptr)) at += tok_align((size_t)d->M * to_pitch(d->dtype, d->N) * es_of(d->dtype));
     w.part = at;
     if (d->dbias != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->N * 4);
+    w.slab = at;            // one product after the other
+    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, d->M, d->K, d->N, 1, 1) : 0, d->dw != nullptr ? tg_slab_bytes(d->dtype, d->N, d->K, d->M, 1, 1) : 0);
     w.total = at;
     return w;
 }
 struct GatWs {
-    size_t dz, pg, pu, total;
+    size_t dz, pg, pu, slab, total;
 };
 GatWs gat_ws(const MisGatedDesc* d) {
     GatWs w{};
     size_t at = 0;
     w.dz = at;
-    at += tok_align((size_t)d->M * to_pitch(d->dtype, 2 * (long long)d->F) * es_of(d->dtype));
+    at += tok_align((size_t)d->M * 2 * to_pitch(d->dtype, d->F) * es_of(d->dtype));
     w.pg = at;
     if (d->dbg != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
     w.pu = at;
     if (d->dbu != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
+    w.slab = at;
+    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, d->M, d->K, d->F, 2, 1) : 0, d->dwg != nullptr ? tg_slab_bytes(d->dtype, d->F, d->K, d->M, 1, 2) : 0);
     w.total = at;
     return w;
 }
@@ -186,13 +191,14 @@ extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
     if (d->res != nullptr) TO_LD(who, d->ldres, d->N, "res");
     if (d->z != nullptr) TO_LD(who, d->ldz, d->N, "z");
     TgArgs a{};
-    a.a = TgOperand{d->x, d->x, d->ldx, TO_MAX};
-    a.b = TgOperand{d->w, d->w, d->ldw, TO_MAX};
+    a.ranges = a.batches = 1;
+    a.a = TgOperand{d->x, d->x, d->ldx};
+    a.b = TgOperand{d->w, d->w, d->ldw};
     a.M = d->M; a.N = d->N; a.K = d->K;
     a.act = d->act; a.bias = d->bias; a.res = d->res; a.ldres = d->ldres;
-    a.y = a.y2 = d->y; a.ldy = d->ldy; a.msplit = TO_MAX;
+    a.y = a.y2 = d->y; a.ldy = d->ldy;
     a.z = d->z; a.ldz = d->ldz;
-    return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, stream);
+    return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, nullptr, stream);
 }
 
 extern "C" size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d) {
@@ -234,19 +240,21 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     if (part != nullptr) TO_TRY(to_colsum(part, to_nblk(d->M), d->N, d->dbias, stream));
     if (d->dx != nullptr) {
         TgArgs a{};
-        a.a = TgOperand{dz, dz, lddz, TO_MAX};
-        a.b = TgOperand{d->w, d->w, d->ldw, TO_MAX};
+        a.ranges = a.batches = 1;
+        a.a = TgOperand{dz, dz, lddz};
+        a.b = TgOperand{d->w, d->w, d->ldw};
         a.M = d->M; a.N = d->K; a.K = d->N;
-        a.y = a.y2 = d->dx; a.ldy = d->lddx; a.msplit = TO_MAX;
-        TO_TRY(tg_launch(d->dtype, 0, 1, TG_LINEAR, a, stream));
+        a.y = a.y2 = d->dx; a.ldy = d->lddx;
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
     }
     if (d->dw != nullptr) {
         TgArgs a{};
-        a.a = TgOperand{dz, dz, lddz, TO_MAX};
-        a.b = TgOperand{d->x, d->x, d->ldx, TO_MAX};
+        a.ranges = a.batches = 1;
+        a.a = TgOperand{dz, dz, lddz};
+        a.b = TgOperand{d->x, d->x, d->ldx};
         a.M = d->N; a.N = d->K; a.K = d->M;
-        a.y = a.y2 = d->dw; a.ldy = d->lddw; a.msplit = TO_MAX;
-        TO_TRY(tg_launch(d->dtype, 1, 1, TG_LINEAR, a, stream));
+        a.y = a.y2 = d->dw; a.ldy = d->lddw;
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
     }
     return MIS_OK;
 }
@@ -262,13 +270,14 @@ extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
     MIS_REQUIRE((d->g == nullptr) == (d->u == nullptr), MIS_EINVAL, "%s: g and u are kept together", who);
     if (d->g != nullptr) TO_LD(who, d->ldz, d->F, "g / u");
     TgArgs a{};
-    a.a = TgOperand{d->x, d->x, d->ldx, TO_MAX};
-    a.b = TgOperand{d->wg, d->wu, d->ldw, TO_MAX};
+    a.ranges = a.batches = 1;
+    a.a = TgOperand{d->x, d->x, d->ldx};
+    a.b = TgOperand{d->wg, d->wu, d->ldw};
     a.M = d->M; a.N = d->F; a.K = d->K;
     a.act = d->act; a.bias = d->bg; a.bias2 = d->bu;
-    a.y = a.y2 = d->h; a.ldy = d->ldh; a.msplit = TO_MAX;
+    a.y = a.y2 = d->h; a.ldy = d->ldh;
     a.z = d->g; a.z2 = d->u; a.ldz = d->ldz;
-    return tg_launch(d->dtype, 0, 0, TG_GATED, a, stream);
+    return tg_launch(d->dtype, 0, 0, TG_GATED, a, nullptr, stream);
 }
 
 extern "C" size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d) {
@@ -303,28 +312,32 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     const GatWs w = gat_ws(d);
     MIS_REQUIRE(d->workspace != nullptr && d->workspace_bytes >= w.total, MIS_EINVAL, "%s: the workspace has %zu bytes, %zu are needed", who, d->workspace_bytes, w.total);
     char* const ws = (char*)d->workspace;
-    const long long F = d->F, lddz = to_pitch(d->dtype, 2 * F);
+    const long long F = d->F, pitch = to_pitch(d->dtype, F), lddz = 2 * pitch;
     float* const pg = d->dbg != nullptr ? (float*)(ws + w.pg) : nullptr;
     float* const pu = d->dbu != nullptr ? (float*)(ws + w.pu) : nullptr;
-    void* const dz = ws + w.dz;          // [M][dg (F) | du (F)]
+    void* const dz = ws + w.dz;          // [M][dg (F, padded to pitch) | du]
+    void* const du = ws + w.dz + pitch * es;
     TO_TRY(to_dz<1>(d->dtype, d->dh, d->lddh, d->g, d->u, d->ldz, d->act, d->M, F, dz, lddz, pg, pu, stream));
     if (pg != nullptr) TO_TRY(to_colsum(pg, to_nblk(d->M), F, d->dbg, stream));
     if (pu != nullptr) TO_TRY(to_colsum(pu, to_nblk(d->M), F, d->dbu, stream));
     if (d->dx != nullptr) {
         TgArgs a{};
-        a.a = TgOperand{dz, dz, lddz, TO_MAX};
-        a.b = TgOperand{d->wg, d->wu, d->ldw, F};
-        a.M = d->M; a.N = d->K; a.K = 2 * F;
-        a.y = a.y2 = d->dx; a.ldy = d->lddx; a.msplit = TO_MAX;
-        TO_TRY(tg_launch(d->dtype, 0, 1, TG_LINEAR, a, stream));
+        a.ranges = a.batches = 1;
+        a.a = TgOperand{dz, du, lddz};
+        a.b = TgOperand{d->wg, d->wu, d->ldw};
+        a.M = d->M; a.N = d->K; a.K = F;
+        a.ranges = 2;
+        a.y = a.y2 = d->dx; a.ldy = d->lddx;
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
     }
     if (d->dwg != nullptr) {
         TgArgs a{};
-        a.a = TgOperand{dz, dz, lddz, TO_MAX};
-        a.b = TgOperand{d->x, d->x, d->ldx, TO_MAX};
-        a.M = 2 * F; a.N = d->K; a.K = d->M;
-        a.y = d->dwg; a.y2 = d->dwu; a.ldy = d->lddw; a.msplit = F;
-        TO_TRY(tg_launch(d->dtype, 1, 1, TG_LINEAR, a, stream));
+        a.ranges = a.batches = 1;
+        a.a = TgOperand{dz, du, lddz};
+        a.b = TgOperand{d->x, d->x, d->ldx};
+        a.M = F; a.N = d->K; a.K = d->M;
+        a.y = d->dwg; a.y2 = d->dwu; a.ldy = d->lddw; a.batches = 2;
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
     }
     return MIS_OK;
 }
