@@ -3,13 +3,14 @@
 // 8 waves, 2 (m) x 4 (n), a wave owns 128 x 64 of C as 8 x 4 MFMA tiles of 16 x 16 (128 accumulator registers).  A step is 64 k: two segments of 12 fragments (24 KiB of LDS reads per
 // wave and step for 64 MFMAs) - the two waves of a SIMD are one barrier apart, so that one is always inside its 32 MFMAs (512 cycles) while the other fetches fragments:
 //
-//      slot        0            1         2         3            4
-//      group 0     R0 issue     M0        R1        M1 wait      R0' ...          R = fragment reads, M = 32 MFMAs, every slot ends with a barrier of all 8 waves
-//      group 1     M1" issue    R0        M0        R1 wait      M1 issue
+//      slot        0            1            2            3               4
+//      group 0     R0 B(s+1)    M0           R1 A(s+2)    M1 wait         R0' ...      R = fragment reads, M = 32 MFMAs, every slot ends with a barrier of all 8 waves
+//      group 1     M1"          R0 B(s+1)    M0           R1 A(s+2) wait  M1 ...
 //
-// Both operands arrive by LDS-DMA, 64 KiB a step, double-buffered (128 of 160 KiB); a step's 8 instructions per wave are issued in slot 0 of the step before - the buffer's last readers
-// passed the barrier in front of it - and retired by vmcnt(0) in slot 3, which leaves them about 2000 cycles.  The step sequence is flat over a block's tiles (grid = number of CUs), so a
-// tile's first step is in flight while the tile before is finished and stored.
+// Both operands arrive by LDS-DMA, 64 KiB a step, four instructions of 1 KiB per wave in each of its R segments: the CU's load path takes about 25 cycles for one, and a wave that
+// issues into the full path stalls (two of them inside an M segment made it 800 cycles long).  B is double-buffered and fetched one step ahead, A has three buffers and is fetched two
+// steps ahead (all 160 KiB of LDS); a buffer's last readers passed the barrier in front of the slot that refills it, and slot 3 retires step s + 1 by a counted wait that leaves the
+// four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
 // LDS images and swizzles are those of tok_gemm.hip with 256 rows: [row][128 B] for a k-contiguous operand, [k][512 B] for the other kind, read with the transposing ds_read_b64_tr_b16.
 // The fragment reads and their wait are one asm statement: hipcc would put a vmcnt(0), i.e. a wait for the prefetch, in front of a plain LDS read while an LDS-DMA is in flight.
 #include <stdlib.h>
@@ -20,7 +21,8 @@
 
 namespace {
 constexpr int PG_OP = 32768;              // bytes of one operand's 64-k step
-constexpr int PG_STAGE = 2 * PG_OP;
+constexpr int PG_B0 = 3 * PG_OP;          // LDS: three A buffers, two B buffers
+constexpr int PG_LDS = 5 * PG_OP;
 
 struct PgPlan {
     int tm, tn;             // tiles of a product
@@ -85,35 +87,36 @@ __device__ __forceinline__ void pg_read_mm(u32x4 (&A)[8], u32x4 (&B)[4], uint32_
     for (int p = 0; p < 8; ++p) A[p] = pg_join(a[2 * p], a[2 * p + 1]);
 }
 
-// One operand's source of the step to be issued: where its 32 KiB come from
-template <bool MN> struct PgSrc {
-    const char* base;       // tile origin of the current range (wave-uniform)
-    unsigned v0;            // this lane's byte offset in the wave's first instruction
-    unsigned jstep;         // ... and between its instructions (64 rows / 16 k further)
-    long long kstep;        // bytes per 64 k
-    int c8;                 // k-contiguous: first k of this lane's chunk; else its k row in the wave's first instruction
-    int ragged;             // tile rows (columns) present, 256 or fewer
-    int r0;                 // k-contiguous: this lane's row in the wave's first instruction; else the first column of its chunk
+// Where this lane's 16 bytes of an operand's DMA instructions lie, relative to the step's first element
+struct PgLane {
+    unsigned v0;            // byte offset in the wave's first instruction
+    unsigned jstep;         // ... and between its four instructions: 64 rows (gated B: 32 columns) or 16 k further
+    int row;                // k contiguous: row of the first instruction; else first column of the chunk
+    int k;                  // k contiguous: first k of the chunk; else k row of the first instruction
+};
+// one operand's 64-k step (wave-uniform)
+struct PgStep {
+    const char* base;
+    int left;               // k present, 64 or fewer
+    int rows;               // tile rows (columns) present
+    int whole;              // all of both
 };
 
-template <bool MN>
-__device__ __forceinline__ void pg_issue(const PgSrc<MN>& s, long long kstart, long long K, char* dst, int wave) {
-    // valid lanes are inside the operand by construction; a lane that has to read zeros carries an offset past num_records
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(s.base + (kstart >> 6) * s.kstep), 0, 0x7fffffff, 0x00020000);
-    const int left = K - kstart < 64 ? (int)(K - kstart) : 64;
-    if (left == 64 && s.ragged == 256) {
+// The wave's four instructions of a step.  Valid lanes are inside the operand by construction; a lane that has to read zeros carries an offset past num_records.
+template <bool MN, int RSTEP> __device__ __forceinline__ void pg_issue(const PgLane& l, const PgStep& s, char* dst, int wave) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(s.base), 0, 0x7fffffff, 0x00020000);
+    if (s.whole) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pp_dma16s(r, (int)s.v0, (int)(j * s.jstep), dst + (wave + 8 * j) * 1024);
+        for (int j = 0; j < 4; ++j) pp_dma16s(r, (int)l.v0, (int)(j * l.jstep), dst + (wave + 8 * j) * 1024);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool ok = MN ? (s.c8 + 16 * j < left && s.r0 < s.ragged) : (s.c8 < left && s.r0 + 64 * j < s.ragged);
-            pp_dma16s(r, ok ? (int)s.v0 : PP_OOB, (int)(j * s.jstep), dst + (wave + 8 * j) * 1024);
+            const bool ok = MN ? (l.k + 16 * j < s.left && l.row < s.rows) : (l.k < s.left && l.row + RSTEP * j < s.rows);
+            pp_dma16s(r, ok ? (int)l.v0 : PP_OOB, (int)(j * l.jstep), dst + (wave + 8 * j) * 1024);
         }
     }
 }
 }   // namespace
-
 
 template <bool AMN, bool BMN, int EPI>
 __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgPlan pl) {
@@ -134,48 +137,37 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
     uint32_t fA, fB;
     if constexpr (!AMN) fA = wm * 16384 + li * 128 + ((lg ^ (li >> 1)) << 4);
     else fA = (8 * lg + (li >> 2)) * 512 + ((wm * 8 + ((li >> 2) | ((lg & 1) << 2))) << 5) + 8 * (li & 3);
-    if constexpr (!BMN) fB = PG_OP + wn * 8192 + (8 * (li >> 2) + (li & 3)) * 128 + ((lg ^ (((li >> 1) & 1) | ((li >> 2) << 1))) << 4);
-    else fB = PG_OP + (8 * lg + (li >> 2)) * 512 + (((wn * 4 + ((li & 3) >> 1)) ^ ((li >> 2) << 1)) << 5) + 16 * (li & 1);
+    if constexpr (!BMN) fB = PG_B0 + wn * 8192 + (8 * (li >> 2) + (li & 3)) * 128 + ((lg ^ (((li >> 1) & 1) | ((li >> 2) << 1))) << 4);
+    else fB = PG_B0 + (8 * lg + (li >> 2)) * 512 + (((wn * 4 + ((li & 3) >> 1)) ^ ((li >> 2) << 1)) << 5) + 16 * (li & 1);
 
     // ---- DMA source offsets of this lane ----
-    PgSrc<AMN> sa;
-    PgSrc<BMN> sb;
+    PgLane la, lb;
+    constexpr int BROWS = EPI == TG_GATED ? 32 : 64;          // B rows (columns of C) an instruction index adds
     if constexpr (!AMN) {
         const int r = 8 * wave + (lane >> 3);                 // (+ 64 j)
-        sa.c8 = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
-        sa.r0 = r;
-        sa.v0 = (unsigned)(r * a.a.ld + sa.c8) * 2;
-        sa.jstep = (unsigned)(128 * a.a.ld);
-        sa.kstep = 128;
+        la.row = r;
+        la.k = ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+        la.v0 = (unsigned)(r * a.a.ld + la.k) * 2;
+        la.jstep = (unsigned)(128 * a.a.ld);
     } else {
         const int k = 2 * wave + (lane >> 5);                 // (+ 16 j)
-        const int c32 = ((lane & 31) >> 1) ^ ((k & 3) | (((k >> 3) & 1) << 2));
-        sa.c8 = k;
-        sa.r0 = c32 * 16 + (lane & 1) * 8;
-        sa.v0 = (unsigned)(k * a.a.ld + sa.r0) * 2;
-        sa.jstep = (unsigned)(32 * a.a.ld);
-        sa.kstep = 128 * a.a.ld;
+        la.k = k;
+        la.row = (((lane & 31) >> 1) ^ ((k & 3) | (((k >> 3) & 1) << 2))) * 16 + (lane & 1) * 8;
+        la.v0 = (unsigned)(k * a.a.ld + la.row) * 2;
+        la.jstep = (unsigned)(32 * a.a.ld);
     }
     if constexpr (!BMN) {
-        int r = 8 * wave + (lane >> 3);
-        sb.c8 = ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))) * 8;
-        if constexpr (EPI == TG_GATED) {                       // rows 64 j + r of the tile: r < 32 column 32 j + r of gate, else of up
-            r &= 31;
-            sb.jstep = (unsigned)(64 * a.b.ld);
-        } else {
-            sb.jstep = (unsigned)(128 * a.b.ld);
-        }
-        sb.r0 = r;
-        sb.v0 = (unsigned)(r * a.b.ld + sb.c8) * 2;
-        sb.kstep = 128;
+        const int r = 8 * wave + (lane >> 3);
+        lb.row = EPI == TG_GATED ? (r & 31) : r;              // gated: rows 64 j + r of the tile hold column 32 j + (r & 31), of gate for r < 32 (waves 0..3), else of up
+        lb.k = ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))) * 8;
+        lb.v0 = (unsigned)(lb.row * a.b.ld + lb.k) * 2;
+        lb.jstep = (unsigned)(2 * BROWS * a.b.ld);
     } else {
         const int k = 2 * wave + (lane >> 5);
-        const int c32 = ((lane & 31) >> 1) ^ ((k & 3) << 1);
-        sb.c8 = k;
-        sb.r0 = c32 * 16 + (lane & 1) * 8;
-        sb.v0 = (unsigned)(k * a.b.ld + sb.r0) * 2;
-        sb.jstep = (unsigned)(32 * a.b.ld);
-        sb.kstep = 128 * a.b.ld;
+        lb.k = k;
+        lb.row = (((lane & 31) >> 1) ^ ((k & 3) << 1)) * 16 + (lane & 1) * 8;
+        lb.v0 = (unsigned)(k * a.b.ld + lb.row) * 2;
+        lb.jstep = (unsigned)(32 * a.b.ld);
     }
 
     // items: batch-major, then k part, then tile; tiles in bands of 4 tile rows, column by column inside a band (32 neighbours of an XCD share 4 row panels and 8 column panels in its L2)
@@ -194,58 +186,58 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
         return nsteps_all - s0 < pl.sps ? nsteps_all - s0 : pl.sps;
     };
 
-    // ---- load cursor ----
-    int lit = first, lstep = 0, lrem = 0, lbt = 0;
-    long long lm0 = 0, ln0 = 0;
-    auto rebase = [&](int range) {                            // tile origin in the operands of this range
+    // ---- load cursor: `na` is the step whose A is issued next, `nb` the one whose B is (the step before, once the pipeline runs) ----
+    int lit = first, lrange = 0, lrem = 0, krem = 0;          // item, range, steps of the item from the cursor's on, k of the range from the cursor's on
+    PgStep na, nb, nb1;                                       // nb1: B of na's step
+    bool va = true, vb = true;                                // whether na / nb is a step of this block
+    const long long step_a = AMN ? 128 * a.a.ld : 128, step_b = BMN ? 128 * a.b.ld : 128;
+    auto flags = [&]() __attribute__((always_inline)) {
+        na.left = nb1.left = krem < 64 ? krem : 64;
+        na.whole = na.left == 64 && na.rows == 256;
+        nb1.whole = nb1.left == 64 && nb1.rows == BN;
+    };
+    // (tile, k part) of item lit at step `at` of its product -> na, nb1
+    auto place = [&](long long m0, long long n0, int bt, int at) {
+        lrange = at >= pl.spr ? 1 : 0;
+        const int ks = at - lrange * pl.spr;
         // (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
-        const char* const pa = (const char*)a.a.p + (long long)(AMN ? lbt : range) * ((const char*)a.a.p2 - (const char*)a.a.p);
-        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : range) * ((const char*)a.b.p2 - (const char*)a.b.p);
-        sa.base = pa + (AMN ? lm0 : lm0 * a.a.ld) * 2;
-        sb.base = pb + (BMN ? ln0 : ln0 * a.b.ld) * 2;
+        const char* const pa = (const char*)a.a.p + (long long)(AMN ? bt : lrange) * ((const char*)a.a.p2 - (const char*)a.a.p);
+        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : lrange) * ((const char*)a.b.p2 - (const char*)a.b.p);
+        na.base = pa + (AMN ? m0 : m0 * a.a.ld) * 2 + ks * step_a;
+        nb1.base = pb + (BMN ? n0 : n0 * a.b.ld) * 2 + ks * step_b;
+        krem = (int)a.K - ks * 64;
+        na.rows = a.M - m0 < 256 ? (int)(a.M - m0) : 256;
+        nb1.rows = a.N - n0 < BN ? (int)(a.N - n0) : BN;
+        flags();
     };
     auto load_tile = [&]() {
-        int sp;
-        tile_of(lit, lbt, sp, lm0, ln0);
-        lstep = sp * pl.sps;
+        int bt, sp;
+        long long m0, n0;
+        tile_of(lit, bt, sp, m0, n0);
         lrem = steps_of(sp);
-        sa.ragged = a.M - lm0 < 256 ? (int)(a.M - lm0) : 256;
-        if constexpr (EPI == TG_GATED) {
-            // per instruction 32 columns: r0 + 64 j < ragged has to mean r0 + 32 j < columns present
-            sb.ragged = a.N - ln0 < 128 ? (int)(a.N - ln0) : 256;
-        } else {
-            sb.ragged = a.N - ln0 < 256 ? (int)(a.N - ln0) : 256;
-        }
-        rebase(lstep >= pl.spr ? 1 : 0);
+        place(m0, n0, bt, sp * pl.sps);
     };
-    load_tile();
-    bool lmore = true;
-    auto issue = [&](char* stage) {                           // the cursor's step -> stage; then the cursor moves on
-        const int range = lstep >= pl.spr ? 1 : 0;
-        const long long k = (long long)(lstep - range * pl.spr) * 64;
-        pg_issue<AMN>(sa, k, a.K, stage, wave);
-        if constexpr (EPI == TG_GATED) {
-            if (sb.ragged < 256) {
-                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(sb.base + (k >> 6) * sb.kstep), 0, 0x7fffffff, 0x00020000);
-                const int left = a.K - k < 64 ? (int)(a.K - k) : 64;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    pp_dma16s(r, sb.c8 < left && sb.r0 + 32 * j < sb.ragged ? (int)sb.v0 : PP_OOB, (int)(j * sb.jstep), stage + PG_OP + (wave + 8 * j) * 1024);
-            } else {
-                pg_issue<BMN>(sb, k, a.K, stage + PG_OP, wave);
-            }
-        } else {
-            pg_issue<BMN>(sb, k, a.K, stage + PG_OP, wave);
-        }
-        ++lstep;
+    auto advance = [&]() __attribute__((always_inline)) {     // A of the cursor's step is issued: its B is next, and A of the step behind it
+        nb = nb1;
+        vb = va;
+        if (!va) return;
+        na.base += step_a;
+        nb1.base += step_b;
+        krem -= 64;
         if (--lrem == 0) {
             lit += gridDim.x;
-            lmore = lit < pl.items;
-            if (lmore) load_tile();
-        } else if (lstep == pl.spr) {
-            rebase(1);
+            va = lit < pl.items;
+            if (va) load_tile();
+        } else if (krem <= 0) {                               // the second range of the same tile
+            int bt, sp;
+            long long m0, n0;
+            tile_of(lit, bt, sp, m0, n0);
+            place(m0, n0, bt, pl.spr);
+        } else {
+            flags();
         }
     };
+    load_tile();
 
     f32x4 acc[4][8];
 #pragma unroll
@@ -253,15 +245,19 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
 #pragma unroll
         for (int p = 0; p < 8; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    issue(smem);
+    int sA = 0, sB = 0;                                       // buffers of the current step
+    auto a_buf = [&](int ahead) { return smem + (sA + ahead >= 3 ? sA + ahead - 3 : sA + ahead) * PG_OP; };
+    auto b_buf = [&](int ahead) { return smem + PG_B0 + ((sB + ahead) & 1) * PG_OP; };
+    auto issue_a = [&](char* dst) __attribute__((always_inline)) { pg_issue<AMN, 64>(la, na, dst, wave); };
+    auto issue_b = [&](char* dst) __attribute__((always_inline)) { pg_issue<BMN, BROWS>(lb, nb, dst, wave); };
+    issue_a(smem);
+    advance();
+    issue_b(smem + PG_B0);
+    if (va) issue_a(a_buf(1));                                // A of step 1
+    advance();                                                // nb: B of step 1, na: A of step 2
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    int st = 0;                                               // stage of the current step
-    if (grp == 1) {
-        if (lmore) issue(smem + PG_STAGE);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();                         // the stagger
-    }
+    if (grp == 1) __builtin_amdgcn_s_barrier();               // the stagger
     __builtin_amdgcn_sched_barrier(0);
 
     int cit = first, crem, bt, sp;
@@ -271,15 +267,15 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
 
     u32x4 fa[8], fb[4];
     auto read = [&](int kk) {
-        const uint32_t s = (uint32_t)(uintptr_t)smem + st * PG_STAGE;
         // k-contiguous: the second half of the step is 64 bytes further in the row, i.e. chunk position ^ 4; else 32 k rows further
-        const uint32_t xa = AMN ? fA + kk * 16384 : fA ^ (kk * 64), xb = BMN ? fB + kk * 16384 : fB ^ (kk * 64);
-        if constexpr (!AMN && !BMN) pg_read_kk(fa, fb, s + xa, s + xb);
-        else if constexpr (!AMN) pg_read_km(fa, fb, s + xa, s + xb);
-        else pg_read_mm(fa, fb, s + xa, s + xb);
+        const uint32_t xa = (uint32_t)(uintptr_t)smem + sA * PG_OP + (AMN ? fA + kk * 16384 : fA ^ (kk * 64));
+        const uint32_t xb = (uint32_t)(uintptr_t)smem + sB * PG_OP + (BMN ? fB + kk * 16384 : fB ^ (kk * 64));
+        if constexpr (!AMN && !BMN) pg_read_kk(fa, fb, xa, xb);
+        else if constexpr (!AMN) pg_read_km(fa, fb, xa, xb);
+        else pg_read_mm(fa, fb, xa, xb);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto mma = [&]() {
+    auto mma = [&]() __attribute__((always_inline)) {
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int f = 0; f < 4; ++f)
@@ -288,37 +284,40 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto barrier = [&]() {
+    auto barrier = [&]() __attribute__((always_inline)) {
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
+    };
+    // step s + 1 is complete once at most the four A(s + 2) just issued are in flight
+    auto retire = [&](bool inflight) __attribute__((always_inline)) {
+        if (inflight) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
 
 #pragma unroll 1
     while (true) {
         // ---- segment 0 ----
-        if (grp == 0) {
-            if (lmore) issue(smem + (st ^ 1) * PG_STAGE);
-            else __builtin_amdgcn_s_sleep(1);                 // keep a distance between the barrier that published this stage and its first read
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        if (vb) issue_b(b_buf(1));
+        else __builtin_amdgcn_s_sleep(1);                     // keep a distance between the barrier that published this step and its first read
+        __builtin_amdgcn_sched_barrier(0);
         read(0);
         barrier();
         mma();
         barrier();
         // ---- segment 1 ----
+        const bool inflight = va;
+        if (va) issue_a(a_buf(2));
+        __builtin_amdgcn_sched_barrier(0);
         read(1);
-        if (grp == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        advance();
+        if (grp == 1) retire(inflight);
         barrier();
-        if (grp == 1) {
-            // the stage just read by both groups is free: the step after the next one goes there
-            if (lmore) issue(smem + st * PG_STAGE);
-            __builtin_amdgcn_sched_barrier(0);
-        }
         mma();
-        if (grp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (grp == 0) retire(inflight);
         barrier();
-        st ^= 1;
+        sA = sA == 2 ? 0 : sA + 1;
+        sB ^= 1;
         if (--crem == 0) {
             // ---- this wave's part of the tile is complete ----
             if constexpr (EPI == TG_GATED) {
@@ -390,9 +389,9 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const PgP
 namespace {
 template <bool AMN, bool BMN, int EPI> int pg_go(const TgArgs& a, const PgPlan& pl, hipStream_t stream) {
     static std::atomic<unsigned long long> attr_done{0};
-    if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tg_pp_kernel<AMN, BMN, EPI>), 2 * PG_STAGE, "token product")) return rc;
+    if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tg_pp_kernel<AMN, BMN, EPI>), PG_LDS, "token product")) return rc;
     const int cus = mis_persist_cus();
-    hipLaunchKernelGGL((tg_pp_kernel<AMN, BMN, EPI>), dim3((unsigned)(pl.items < cus ? pl.items : cus)), dim3(512), 2 * PG_STAGE, stream, a, pl);
+    hipLaunchKernelGGL((tg_pp_kernel<AMN, BMN, EPI>), dim3((unsigned)(pl.items < cus ? pl.items : cus)), dim3(512), PG_LDS, stream, a, pl);
     MIS_LAUNCH_CHECK("token product (256 x 256)");
     return MIS_OK;
 }

@@ -9,9 +9,10 @@ template <typename T> struct TgLinearRow {
     int nv;                 // columns of it inside the matrix
     void* y;
     float bias[8];
-    __device__ __forceinline__ TgLinearRow(const TgArgs& a_, void* y_, long long n_) : a(a_), n(n_), nv(a_.N - n_ >= 8 ? 8 : (int)(a_.N - n_)), y(y_) {
-        if (a.bias != nullptr && nv > 0) tok_ldn<float>(a.bias + n, bias, nv);
+    __device__ __forceinline__ TgLinearRow(const TgArgs& a_, void* y_, long long n_, bool full) : a(a_), n(n_), nv(a_.N - n_ >= 8 ? 8 : (int)(a_.N - n_)), y(y_) {
+        if (full && a.bias != nullptr && nv > 0) tok_ldn<float>(a.bias + n, bias, nv);
     }
+    __device__ __forceinline__ void store(long long m, const float (&v)[8]) const { tok_stn<T>(reinterpret_cast<T*>(y) + m * a.ldy + n, v, nv); }
     __device__ __forceinline__ void operator()(long long m, float (&v)[8]) const {
         if (a.bias != nullptr) {
 #pragma unroll
@@ -25,7 +26,7 @@ template <typename T> struct TgLinearRow {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += r[j];
         }
-        tok_stn<T>(reinterpret_cast<T*>(y) + m * a.ldy + n, v, nv);
+        store(m, v);
     }
 };
 // h = act(g + bg) (u + bu), the two sums kept in z, z2

@@ -31,7 +31,3 @@ struct TgArgs {
 // k: its parts go to `slab` (tg_slab_bytes) and are added in their order.
 int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream);
 size_t tg_slab_bytes(int dtype, long long M, long long N, long long K, int ranges, int batches);
-
-// tok_gemm_pp.hip; tok_gemm.hip
-int tg_pp_launch(int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, int splits, hipStream_t stream);
-int tg_slab_sum(int dtype, const TgArgs& a, const float* slab, int splits, hipStream_t stream);

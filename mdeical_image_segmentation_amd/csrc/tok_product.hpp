@@ -1,0 +1,349 @@
+// The kernel of the token products, any shape / stride / alignment: C[m][n] = sum_k A(m, k) B(n, k) (tok_gemm.hpp), included by one .hip per (type, tile).
+//
+// A block of 4 waves (2 x 2) owns a 128 x 128 piece of C (two blocks per CU), a wave F x F MFMA tiles of 16 x 16, F = 4.
+//
+// A step is 128 bytes of k per row (64 bf16 / 32 f32), in two halves.  The pipeline of a wave, all of it plain code whose waits the compiler counts:
+//      half 0   MFMAs of half 0 | fragments of half 1 <- LDS | step s + 1: registers -> other LDS buffer | step s + 2: global -> registers
+//      barrier
+//      half 1   MFMAs of half 1 | fragments of half 0 of step s + 1 <- other LDS buffer
+// One barrier a step: a buffer is overwritten a step after its last reads, which were waited for in front of the barrier between.  The steps are flat over a block's tiles (the grid is what
+// the chip holds at once), so the next tile's first steps are on their way while a finished tile is stored.
+//
+// B(n) feeds the MFMA's row side, A(m) its column side: a lane then holds runs of 8 consecutive n of one m, and bias, residual and stores are 16 bytes wide.
+//   LDS image, k contiguous:   [row][128 B], 16-byte chunks at position c ^ key(row): a fragment read touches each bank once
+//   LDS image, own index cont.: [k][TILE elements]; bf16 fragments by the transposing read (16 lanes: 4 k x 4 runs of 4), f32 ones by plain 16-byte reads, which give one k of four
+//                              MFMA tiles (tile v then holds the indices 4 r + v)
+// Sums are f32 (MFMA accumulators); k order inside a step is the same for both operands, which is all the sum needs.
+#pragma once
+#include "tok_epilogue.hpp"
+#include "tok_product_plan.hpp"
+
+namespace {
+typedef __attribute__((address_space(3))) s16x4 tp_lds_s16x4;
+constexpr int TP_OOB = (int)0xFFFFFF00u;          // past every buffer below: reads as zero
+
+// swizzle keys.  Rows of a fragment: A side 16 f + li, B side 32 (f >> 1) + 8 (li >> 2) + 4 (f & 1) + (li & 3)
+template <bool B> __device__ __forceinline__ int tp_key(int row) {
+    return B ? (((row >> 1) & 1) | (((row >> 3) & 3) << 1)) : ((row >> 1) & 7);
+}
+// 32-byte position of a [k][i] bf16 row.  A side: a group of 16 lanes reads 32 bytes of 4 rows; B side: 8 of every 16 bytes of a 64-byte run of 4 rows
+template <bool B> __device__ __forceinline__ int tp_pos32(int c32, int k) {
+    return B ? (c32 ^ ((k & 3) << 1)) : (c32 ^ ((k & 3) | (((k >> 3) & 1) << 2)));
+}
+// one 16-byte chunk of which n elements exist, at any element address
+template <typename T> __device__ __forceinline__ u32x4 tp_chunk(const T* p, long long n) {
+    constexpr int EPC = Tr<T>::EPC;
+    if (n >= EPC) return tok_ld16<T>(p);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n > 0) {
+        float f[EPC];
+#pragma unroll
+        for (int i = 0; i < EPC; ++i) f[i] = i < n ? ld_elem<T>(p + i) : 0.f;
+        v = pack_chunk<T>(f);
+    }
+    return v;
+}
+
+// one operand's step: origin of the tile at its first k, k and rows (own indices) present from there on (wave-uniform)
+struct TpStep {
+    const char* base;
+    const char* base2;      // gated B: the up rows
+    long long left, rows;
+};
+
+// Staging of one operand: F chunks of 16 bytes per thread.  k contiguous: chunk c = t & 7 of the rows (t >> 3) + 32 j; own index contiguous: chunk t % CPR of the k rows t / CPR + j KR.
+template <typename T, bool MN, bool B, int EPI, bool AL, int F> struct TpStage {
+    static constexpr int ES = sizeof(T), EPC = Tr<T>::EPC, TILE = 32 * F, CPR = TILE / EPC, KR = 256 / CPR;
+    static constexpr bool PAIR = B && EPI == TG_GATED;
+    int c, r;               // chunk, first row / k row
+    unsigned voff;          // byte offset of chunk 0 (AL)
+    long long ld;
+    u32x4 v[F];
+    __device__ __forceinline__ TpStage(long long ld_) : ld(ld_) {
+        const int t = threadIdx.x;
+        c = MN ? t % CPR : t & 7;
+        r = MN ? t / CPR : t >> 3;
+        voff = (unsigned)(r * ld * ES) + c * 16;
+    }
+    // chunk j of the step; one that does not exist reads as zeros
+    __device__ __forceinline__ void load(const TpStep& s, int j) {
+        if constexpr (AL) {
+            // (chunks are whole here: a lane is in or out)
+            const __amdgpu_buffer_rsrc_t q = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(PAIR && (j & 1) ? s.base2 : s.base), 0, 0x7fffffff, 0x00020000);
+            const bool ok = MN ? (r + j * KR < s.left && c * EPC < s.rows) : (c * EPC < s.left && r + rowstep(j) < s.rows);
+            v[j] = __builtin_amdgcn_raw_buffer_load_b128(q, ok ? (int)voff : TP_OOB, (int)(rowstep(j) * ld * ES), 0);
+        } else {
+            const T* p = reinterpret_cast<const T*>(PAIR && (j & 1) ? s.base2 : s.base) + (long long)(r + rowstep(j)) * ld + c * EPC;
+            if constexpr (MN) v[j] = tp_chunk<T>(p, r + j * KR < s.left ? s.rows - c * EPC : 0);
+            else v[j] = tp_chunk<T>(p, r + rowstep(j) < s.rows ? s.left - c * EPC : 0);
+        }
+    }
+    static constexpr int TILE_K = Tr<T>::CK;
+    // rows (k rows) that chunk j lies behind chunk 0; gated B: rows 64 b + q of the tile are column 32 b + (q & 31), of gate for q < 32, else of up
+    static constexpr int rowstep(int j) { return MN ? j * KR : (PAIR ? (j >> 1) * 32 : j * 32); }
+    __device__ __forceinline__ void put(char* lds, int j) const {
+        int off;
+        if constexpr (!MN) {
+            off = (r + 32 * j) * 128 + ((c ^ tp_key<B>(r)) << 4);          // (key(r + 32 j) = key(r))
+        } else if constexpr (ES == 2) {
+            const int k = r + j * KR;
+            off = k * (TILE * 2) + (tp_pos32<B>(c >> 1, k) << 5) + ((c & 1) << 4);
+        } else {
+            off = (r + j * KR) * (TILE * 4) + c * 16;
+        }
+        lds_write_b128(lds, off, v[j]);
+    }
+};
+
+// fragment f of a wave's 16 F rows (own indices) for half kk of a step; f32 with its own index contiguous: 16-byte reads give four fragments at once (asked for with f = 0)
+template <typename T, bool MN, bool B, int F> __device__ __forceinline__ void tp_frag(u32x4 (&v)[F], const char* lds, int w, int kk, int f) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    constexpr int TILE = 32 * F;
+    if constexpr (!MN) {
+        const int row = w * 16 * F + (B ? 32 * (f >> 1) + 8 * (li >> 2) + 4 * (f & 1) + (li & 3) : 16 * f + li);
+        v[f] = lds_read_b128(lds, row * 128 + (((kk * 4 + lg) ^ tp_key<B>(row)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+        const int i = w * 16 * F + (B ? 32 * (f >> 1) + 8 * (li & 3) + 4 * (f & 1) : 16 * f + 4 * (li & 3));
+        s16x4 h[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int k = kk * 32 + 8 * lg + 4 * s + (li >> 2);
+            const uint32_t at = (uint32_t)(uintptr_t)lds + k * (TILE * 2) + (tp_pos32<B>(i >> 4, k) << 5) + ((i & 15) << 1);
+            h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tp_lds_s16x4*>(at));
+        }
+        const u32x2 lo = __builtin_bit_cast(u32x2, h[0]), hi = __builtin_bit_cast(u32x2, h[1]);
+        v[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+        static_assert(F == 4, "f32: 64 own indices per wave");
+        if (f != 0) return;
+        u32x4 t[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) t[s] = lds_read_b128(lds, (kk * 16 + 4 * lg + s) * (TILE * 4) + (w * 64 + 4 * li) * 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = u32x4{t[0][q], t[1][q], t[2][q], t[3][q]};
+    }
+}
+
+// B side index of value j (0..7) of run h of a lane: base(h) + j, held by tile f, accumulator q
+template <typename T, bool BMN> struct TpRun {
+    static constexpr bool R4 = BMN && sizeof(T) == 4;
+    static __device__ __forceinline__ int base(int h, int lg) { return R4 ? 16 * lg + 8 * h : 32 * h + 8 * lg; }
+    static constexpr int f(int h, int j) { return R4 ? (j & 3) : 2 * h + (j >> 2); }
+    static constexpr int q(int h, int j) { return R4 ? 2 * h + (j >> 2) : (j & 3); }
+};
+}   // namespace
+
+template <typename T, bool AMN, bool BMN, int EPI, bool AL, int F>
+__global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, const TpPlan pl) {
+    constexpr int CK = Tr<T>::CK, ES = sizeof(T), TILE = 32 * F, BN = EPI == TG_GATED ? TILE / 2 : TILE, OP = TILE * 128;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];          // 2 x [A | B]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    const int li = lane & 15, lg = lane >> 4;
+    const int first = xcd_remap(blockIdx.x, gridDim.x);
+    if (first >= pl.items) return;                            // block-uniform
+    const int tiles = pl.tm * pl.tn, all_steps = a.ranges * pl.spr;
+
+    // items: batch-major, then k part, then tile; tiles in bands of 4 tile rows, column by column inside a band (the neighbours that run on an XCD share row and column panels in its L2)
+    auto tile_of = [&](int it, int& bt, int& sp, long long& m0, long long& n0) {
+        const int bs = it / tiles, t = it - bs * tiles;
+        bt = bs / pl.splits;
+        sp = bs - bt * pl.splits;
+        const int band = t / (4 * pl.tn), in = t - band * 4 * pl.tn;
+        const int h = pl.tm - band * 4 < 4 ? pl.tm - band * 4 : 4;
+        const int c = in / h;
+        m0 = (long long)(band * 4 + in - c * h) * TILE;
+        n0 = (long long)c * BN;
+    };
+    auto steps_of = [&](int sp) { return all_steps - sp * pl.sps < pl.sps ? all_steps - sp * pl.sps : pl.sps; };
+
+    // ---- load cursor: the step that goes into the staging registers next ----
+    TpStage<T, AMN, false, EPI, AL, F> ga(a.a.ld);
+    TpStage<T, BMN, true, EPI, AL, F> gb(a.b.ld);
+    TpStep na, nb;
+    int lit = first, lrem = 0;
+    const long long step_a = AMN ? CK * ES * a.a.ld : CK * ES, step_b = BMN ? CK * ES * a.b.ld : CK * ES;
+    auto place = [&](long long m0, long long n0, int bt, int at) {
+        const int range = at >= pl.spr ? 1 : 0, ks = at - range * pl.spr;
+        // (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
+        const long long da = (const char*)a.a.p2 - (const char*)a.a.p, db = (const char*)a.b.p2 - (const char*)a.b.p;
+        na.base = (const char*)a.a.p + (AMN ? bt : range) * da + (AMN ? m0 : m0 * a.a.ld) * ES + ks * step_a;
+        nb.base = (const char*)a.b.p + (EPI == TG_GATED ? 0 : range) * db + (BMN ? n0 : n0 * a.b.ld) * ES + ks * step_b;
+        nb.base2 = nb.base + db;
+        na.left = nb.left = a.K - (long long)ks * CK;
+        na.rows = a.M - m0;
+        nb.rows = a.N - n0;
+    };
+    auto load_tile = [&]() {
+        int bt, sp;
+        long long m0, n0;
+        tile_of(lit, bt, sp, m0, n0);
+        lrem = steps_of(sp);
+        place(m0, n0, bt, sp * pl.sps);
+    };
+    auto advance = [&]() {                                    // behind the last step: rows 0, everything reads as zeros
+        na.base += step_a;
+        nb.base += step_b;
+        nb.base2 += step_b;
+        na.left -= CK;
+        nb.left -= CK;
+        if (--lrem == 0) {
+            lit += gridDim.x;
+            if (lit < pl.items) load_tile();
+            else na.rows = nb.rows = 0;
+        } else if (na.left <= 0) {                            // the second range of the same tile
+            int bt, sp;
+            long long m0, n0;
+            tile_of(lit, bt, sp, m0, n0);
+            place(m0, n0, bt, pl.spr);
+        }
+    };
+
+    f32x4 acc[F][F];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int p = 0; p < F; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto barrier = [&]() __attribute__((always_inline)) {     // this wave's LDS traffic is done, then everyone's is; loads from global memory stay in flight
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load_tile();
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+        ga.load(na, j);
+        gb.load(nb, j);
+    }
+    advance();
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+        ga.put(smem, j);
+        gb.put(smem + OP, j);
+        ga.load(na, j);
+        gb.load(nb, j);
+    }
+    advance();
+    barrier();
+    u32x4 a0[F], b0[F], a1[F], b1[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        tp_frag<T, AMN, false, F>(a0, smem, wm, 0, f);
+        tp_frag<T, BMN, true, F>(b0, smem + OP, wn, 0, f);
+    }
+
+    int cit = first, crem, bt, sp, buf = 0;
+    long long m0, n0;
+    tile_of(cit, bt, sp, m0, n0);
+    crem = steps_of(sp);
+    while (true) {
+        char* const cur = smem + buf * 2 * OP;
+        char* const nxt = smem + (buf ^ 1) * 2 * OP;
+        // (sched_barrier: the scheduler interleaves inside a row of MFMAs but does not pull a whole step's loads together, which would not fit the registers)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            if (2 * f < F) {
+#pragma unroll
+                for (int g = 2 * f; g < 2 * f + 2; ++g) {
+                    tp_frag<T, AMN, false, F>(a1, cur, wm, 1, g);
+                    tp_frag<T, BMN, true, F>(b1, cur + OP, wn, 1, g);
+                }
+            }
+            ga.put(nxt, f);
+            gb.put(nxt + OP, f);
+            ga.load(na, f);
+            gb.load(nb, f);
+#pragma unroll
+            for (int p = 0; p < F; ++p) mma_b128<T>(acc[f][p], b0[f], a0[p]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
+        barrier();
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            if (2 * f < F) {
+#pragma unroll
+                for (int g = 2 * f; g < 2 * f + 2; ++g) {
+                    tp_frag<T, AMN, false, F>(a0, nxt, wm, 0, g);
+                    tp_frag<T, BMN, true, F>(b0, nxt + OP, wn, 0, g);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < F; ++p) mma_b128<T>(acc[f][p], b1[f], a1[p]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        buf ^= 1;
+        if (--crem > 0) continue;
+
+        // ---- the tile is complete ----
+        using Run = TpRun<T, BMN>;
+        if constexpr (EPI == TG_GATED) {
+            static_assert(!Run::R4, "gated: k-contiguous weights only");
+#pragma unroll
+            for (int b = 0; b < F / 4; ++b) {                  // MFMA tiles 4 b, 4 b + 1 hold 8 gate columns of a lane, 4 b + 2, 4 b + 3 the same columns of up
+                const TgGatedRow<T> row(a, n0 + wn * 8 * F + 32 * b + 8 * lg);
+                if (row.nv > 0) {
+#pragma unroll
+                    for (int p = 0; p < F; ++p) {
+                        const long long m = m0 + wm * 16 * F + 16 * p + li;
+                        float g[8], u[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            g[j] = acc[4 * b + (j >> 2)][p][j & 3];
+                            u[j] = acc[4 * b + 2 + (j >> 2)][p][j & 3];
+                        }
+                        if (m < a.M) row(m, g, u);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < F / 2; ++h) {
+                const long long n = n0 + wn * 16 * F + Run::base(h, lg);
+                const TgLinearRow<T> row(a, bt == 0 ? a.y : a.y2, n, EPI == TG_LINEAR);
+                float* const sl = pl.slab + (long long)(bt * pl.splits + sp) * a.M * a.N + n;
+                if (row.nv > 0) {
+#pragma unroll
+                    for (int p = 0; p < F; ++p) {
+                        const long long m = m0 + wm * 16 * F + ((AMN && ES == 4) ? 4 * li + p : 16 * p + li);
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = acc[Run::f(h, j)][p][Run::q(h, j)];
+                        if (m < a.M) {
+                            if constexpr (EPI == TG_LINEAR) row(m, v);
+                            else if constexpr (EPI == TG_STORE) row.store(m, v);
+                            else tok_stn<float>(sl + m * a.N, v, row.nv);
+                        }
+                    }
+                }
+            }
+        }
+        cit += gridDim.x;
+        if (cit >= pl.items) return;
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+            for (int p = 0; p < F; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+        tile_of(cit, bt, sp, m0, n0);
+        crem = steps_of(sp);
+    }
+}
+
+namespace {
+template <typename T, bool AMN, bool BMN, int EPI, bool AL, int F> int tp_go(const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
+    constexpr size_t LDS = 2 * 2 * 32 * F * 128;
+    static std::atomic<unsigned long long> attr_done{0};
+    if (LDS > 65536)
+        if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tok_product_kernel<T, AMN, BMN, EPI, AL, F>), LDS, "token product")) return rc;
+    constexpr int hold = 512;                                 // blocks that the chip holds at once
+    hipLaunchKernelGGL((tok_product_kernel<T, AMN, BMN, EPI, AL, F>), dim3((unsigned)(pl.items < hold ? pl.items : hold)), dim3(256), LDS, stream, a, pl);
+    MIS_LAUNCH_CHECK("token product");
+    return MIS_OK;
+}
+template <typename T, int F, bool AL> int tp_pick(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
+    if (epi == TG_GATED) return tp_go<T, false, false, TG_GATED, AL, F>(a, pl, stream);
+    if (epi == TG_LINEAR) return tp_go<T, false, false, TG_LINEAR, AL, F>(a, pl, stream);
+    if (pl.splits == 1) return a_mn ? tp_go<T, true, true, TG_STORE, AL, F>(a, pl, stream) : tp_go<T, false, true, TG_STORE, AL, F>(a, pl, stream);
+    return a_mn ? tp_go<T, true, true, TG_SLAB, AL, F>(a, pl, stream) : tp_go<T, false, true, TG_SLAB, AL, F>(a, pl, stream);
+}
+}   // namespace

@@ -1,0 +1,18 @@
+// How a token product is cut, and the launchers of tok_product_*.hip
+#pragma once
+#include "tok_gemm.hpp"
+
+struct TpPlan {
+    int tm, tn;             // tiles of a product
+    int splits;             // parts of the k steps (TG_SLAB, else 1)
+    int spr;                // steps of one range
+    int sps;                // steps of one part
+    int items;              // batches * splits * tm * tn
+    float* slab;            // TG_SLAB: [batch][part][M][N] f32
+};
+
+int tok_product_bf16_256(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
+int tok_product_bf16_128(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
+int tok_product_bf16_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
+int tok_product_f32_128(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
+int tok_product_f32_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
