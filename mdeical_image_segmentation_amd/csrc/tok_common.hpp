@@ -56,8 +56,19 @@ template <bool PRECISE, bool D> __device__ __forceinline__ void tok_act8(int act
         case MIS_ACT_GELU:
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float x = z[i], c = 0.5f * (1.f + erff(x * 0.70710678118654752f));
-                if constexpr (D) d[i] = c + x * (0.3989422804014327f * (PRECISE ? expf(-0.5f * x * x) : __expf(-0.5f * x * x)));
+                const float x = z[i];
+                float c, e;
+                if constexpr (PRECISE) {
+                    e = D ? expf(-0.5f * x * x) : 0.f;
+                    c = 0.5f * (1.f + erff(x * 0.70710678118654752f));
+                } else {
+                    // Abramowitz & Stegun 7.1.26: erfc(|x| / sqrt 2) = poly(t) exp(-x^2 / 2), |error| <= 1.5e-7 - a third of erff's instructions, and the exponential is the derivative's
+                    e = __expf(-0.5f * x * x);
+                    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(x));
+                    const float q = 0.5f * e * (t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))));
+                    c = x < 0.f ? q : 1.f - q;
+                }
+                if constexpr (D) d[i] = c + x * (0.3989422804014327f * e);
                 z[i] = x * c;
             }
             break;
@@ -99,3 +110,5 @@ template <bool PRECISE, bool D> __device__ __forceinline__ void tok_act8(int act
 
 static inline size_t tok_align(size_t n) { return (n + 255) & ~(size_t)255; }
 static inline bool tok_act_ok(int act) { return act >= MIS_ACT_NONE && act <= MIS_ACT_SIGMOID; }
+// out0[n] = sum over the nrow rows of p0[row][n], out1 the same of p1 (either out may be null), in a fixed order; nrow = 0: zeros (token_ops.hip)
+int tok_column_sums(const float* p0, const float* p1, long long nrow, long long N, float* out0, float* out1, hipStream_t stream);

@@ -84,6 +84,7 @@ size_t tg_slab_bytes(int dtype, long long M, long long N, long long K, int range
 
 int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream) {
     const bool al = tg_aligned(dtype, a, a_mn, b_mn);
+    if (epi != TG_STORE && a.M <= 64 && mis_sw(SW_TOK_TILE) == 0) return tok_product_skinny(dtype, epi, a, al, stream);
     const TgCut c = tg_cut(dtype, al, epi == TG_STORE, a.M, a.N, a.K, a.ranges, a.batches, epi == TG_GATED);
     const long long T = c.big ? 256 : 128, BN = epi == TG_GATED ? T / 2 : T, ck = dtype == MIS_BF16 ? 64 : 32;
     const long long tm = (a.M + T - 1) / T, tn = (a.N + BN - 1) / BN, spr = (a.K + ck - 1) / ck;

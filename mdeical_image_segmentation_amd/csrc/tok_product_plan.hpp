@@ -16,3 +16,5 @@ int tok_product_bf16_128(int a_mn, int b_mn, int epi, const TgArgs& a, const TpP
 int tok_product_bf16_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
 int tok_product_f32_128(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
 int tok_product_f32_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
+// forward products of at most 64 rows (tok_skinny.hip)
+int tok_product_skinny(int dtype, int epi, const TgArgs& a, bool aligned, hipStream_t stream);
