@@ -6,160 +6,274 @@
 
 x is (..., width) with any number of leading dimensions, float32 or bfloat16; weights are (out, width) as in nn.Linear, in x's type; biases and norm parameters are float32.  Each
 function is differentiable once (forward and backward are HIP kernels of libmisamd; torch is the allocator and the tape) and keeps what its backward pass needs only when a gradient is
-wanted.  Work is enqueued on torch's current stream of x's device.  Under stream capture take gradients with torch.autograd.grad, or call the ops.*_bwd functions.
-There is no CPU path: a tensor that is not on the GPU raises."""
+wanted.  Work is enqueued on torch's current stream of x's device; workspaces come from the caching allocator call by call, so streams and captured graphs share none.  Under stream
+capture take gradients with torch.autograd.grad, or call the ops.*_bwd functions.  There is no CPU path: a tensor that is not on the GPU raises.
+
+The same kernels without the tape, on caller-owned buffers with any row strides: ops.layernorm_fwd / _bwd, ops.linear_fwd / _bwd, ops.gated_ffn_fwd / _bwd.  (A small call is bound by the
+host: the functions here fill the C descriptors directly, with the checks inline.)"""
+import ctypes as C
+
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
-from ._lib import MisError
+from ._lib import MIS_BF16, MIS_F32, GatedDesc, LinearDesc, MisError, check, load
+from .ops import token_act
+
+_F32, _BF16 = torch.float32, torch.bfloat16
 
 
-def _rows(t, width, name):
-    """(..., width) -> (rows, width) with unit stride inside a row: a view where the strides allow one, else a copy"""
-    if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.shape[-1] != width or width < 1:
-        raise MisError(f"{name} must be a (..., {width}) tensor, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)}")
-    if t.dim() != 2:
-        t = t.reshape(t.numel() // width, width)
-    return _unit(t)
+def _refuse(who, what):
+    raise MisError(f"{who}: {what}")
+
+
+def _say(t):
+    return f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
 
 
 def _unit(t):
+    """a matrix with unit stride inside its rows and rows that do not overlap: itself, or a copy"""
     s0, s1 = t.stride()
     return t if (s1 == 1 or t.shape[1] == 1) and (s0 >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
-def _weight(w, name):
+def _rows(who, t, width, name="x"):
+    """(..., width) -> (rows, width): a view where the strides allow one, else a copy"""
+    if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.shape[-1] != width or width < 1:
+        _refuse(who, f"{name} must be a (..., {width}) tensor, got {_say(t)}")
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // width, width)
+    return t if t.is_contiguous() else _unit(t)
+
+
+def _tokens(who, x, width):
+    """x as rows, and the library's code of its type"""
+    x2 = _rows(who, x, width)
+    if not x2.is_cuda:
+        _refuse(who, f"runs on MI355X only: got {_say(x)} (no CPU fallback)")
+    dt = x2.dtype
+    if dt is not _BF16 and dt is not _F32:
+        _refuse(who, f"x must be float32 or bfloat16, got {_say(x)}")
+    return x2, MIS_BF16 if dt is _BF16 else MIS_F32
+
+
+def _weight(who, w, name, x=None):
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
-        raise MisError(f"{name} must be an (out, in) matrix, got {tuple(w.shape) if isinstance(w, torch.Tensor) else type(w)}")
-    return _unit(w)
+        _refuse(who, f"{name} must be an (out, in) matrix, got {_say(w)}")
+    return w if w.is_contiguous() else _unit(w)
 
 
-def _pair(a, b):
-    """two matrices with one row stride"""
-    return (a, b) if a.shape[0] <= 1 or a.stride(0) == b.stride(0) else (a.contiguous(), b.contiguous())
+def _like(who, t, name, x):
+    if t.dtype is not x.dtype or t.device != x.device:
+        _refuse(who, f"{name} must be {x.dtype} on {x.device} like x, got {_say(t)}")
 
 
-def _grads(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _vec(who, v, name, n, x):
+    """pointer of a float32 vector of n, None for None"""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor) or v.dtype is not _F32 or v.dim() != 1 or v.shape[0] != n or v.device != x.device or not v.is_contiguous():
+        _refuse(who, f"{name} must be a contiguous ({n},) float32 tensor on {x.device}, got {_say(v)}")
+    return v.data_ptr()
 
 
-def _empty(like, *shape, dtype=None):
-    return torch.empty(shape, dtype=like.dtype if dtype is None else dtype, device=like.device)
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(who, fn, x, *args):
+    dev = x.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, who)
+
+
+def _scratch(nbytes, x):
+    return torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+
+
+def _once(backward):
+    """differentiable once: the plain function, unless a graph of the backward pass itself is asked for (then torch's wrapper, whose outputs refuse a second differentiation)"""
+    wrapped = once_differentiable(backward)
+
+    def run(ctx, dy):
+        return wrapped(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+
+    return staticmethod(run)
 
 
 # ---- layer norm ----------------------------------------------------------------------------------------------------------------------------
+def _norm_fwd(x, weight, bias, eps, keep):
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        _refuse("layer_norm", f"x must be a (..., width) tensor, got {_say(x)}")
+    D = x.shape[-1]
+    x2, code = _tokens("layer_norm", x, D)
+    M = x2.shape[0]
+    pw, pb = _vec("layer_norm", weight, "weight", D, x2), _vec("layer_norm", bias, "bias", D, x2)
+    y = torch.empty((M, D), dtype=x2.dtype, device=x2.device)
+    st = torch.empty((2, M), dtype=_F32, device=x2.device) if keep else None
+    ps = st.data_ptr() if keep else None
+    _call("layer_norm", load().mis_layernorm_fwd, x2, code, x2.data_ptr(), _ld(x2), M, D, eps, pw, pb, y.data_ptr(), D, ps, ps + 4 * M if keep else None)
+    return x2, y if x.dim() == 2 else y.view(x.shape), st
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2 = _rows(x, x.shape[-1], "layer_norm: x")
-        M, D = x2.shape
-        y, mean, rstd = _empty(x2, M, D), _empty(x2, M, dtype=torch.float32), _empty(x2, M, dtype=torch.float32)
-        ops.layernorm_fwd(x2, y, weight, bias, mean, rstd, eps)
-        ctx.save_for_backward(x2, weight, mean, rstd)
+        x2, y, st = _norm_fwd(x, weight, bias, eps, True)
+        ctx.save_for_backward(x2, weight, st)
         ctx.shape = x.shape
-        return y.view(x.shape)
+        return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, st = ctx.saved_tensors
         M, D = x.shape
-        need = ctx.needs_input_grad
-        dx = _empty(x, M, D) if need[0] else None
-        dw = _empty(x, D, dtype=torch.float32) if need[1] else None
-        db = _empty(x, D, dtype=torch.float32) if need[2] else None
-        ops.layernorm_bwd(_rows(dy, D, "dy"), x, mean, rstd, weight, dx, dw, db)
-        return None if dx is None else dx.view(ctx.shape), dw, db, None
+        code = MIS_BF16 if x.dtype is _BF16 else MIS_F32
+        nx, nw, nb, _ = ctx.needs_input_grad
+        dy = _rows("layer_norm (backward)", dy, D, "dy")
+        dx = torch.empty((M, D), dtype=x.dtype, device=x.device) if nx else None
+        dw = torch.empty((D,), dtype=_F32, device=x.device) if nw else None
+        db = torch.empty((D,), dtype=_F32, device=x.device) if nb else None
+        lib = load()
+        n = lib.mis_layernorm_bwd_workspace_bytes(code, M, D) if nw or nb else 0
+        ws, ps = _scratch(n, x), st.data_ptr()
+        _call("layer_norm (backward)", lib.mis_layernorm_bwd, x, code, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), M, D, _ptr(weight), ps, ps + 4 * M, _ptr(dx), D, _ptr(dw), _ptr(db),
+              _ptr(ws), n)
+        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension; weight, bias (width,) float32 or None"""
-    if _grads(x, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    x2 = _rows(x, x.shape[-1], "layer_norm: x")
-    y = _empty(x2, *x2.shape)
-    ops.layernorm_fwd(x2, y, weight, bias, None, None, eps)
-    return y.view(x.shape)
+    return _norm_fwd(x, weight, bias, float(eps), False)[1]
 
 
 # ---- matrix product with bias, activation and residual ------------------------------------------------------------------------------------------
-def _linear_fwd(x, weight, bias, activation, residual, keep):
-    w = _weight(weight, "linear: weight")
-    x2 = _rows(x, w.shape[1], "linear: x")
-    M, N = x2.shape[0], w.shape[0]
-    shape = x.shape[:-1] + (N,)
-    if residual is not None and residual.shape != shape:
-        raise MisError(f"linear: residual must have the result's shape {tuple(shape)}, got {tuple(residual.shape)}")
-    y = _empty(x2, M, N)
-    z = _empty(x2, M, N, dtype=torch.float32) if keep and ops.token_act(activation) else None
-    ops.linear_fwd(x2, w, y, bias, activation, None if residual is None else _rows(residual, N, "linear: residual"), z)
-    return x2, w, y.view(shape), z
+def _linear_fwd(x, weight, bias, act, residual, keep):
+    w = _weight("linear", weight, "weight")
+    N, K = w.shape
+    x2, code = _tokens("linear", x, K)
+    _like("linear", w, "weight", x2)
+    M = x2.shape[0]
+    shape = (M, N) if x.dim() == 2 else x.shape[:-1] + (N,)
+    pr = ldr = None
+    if residual is not None:
+        if residual.shape != shape:
+            _refuse("linear", f"residual must have the result's shape {tuple(shape)}, got {_say(residual)}")
+        r2 = _rows("linear", residual, N, "residual")
+        _like("linear", r2, "residual", x2)
+        pr, ldr = r2.data_ptr(), _ld(r2)
+    pb = _vec("linear", bias, "bias", N, x2)
+    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
+    z = torch.empty((M, N), dtype=_F32, device=x2.device) if keep and act else None
+    d = LinearDesc(code, act, M, N, K, x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), pb, pr, ldr or 0, y.data_ptr(), N, _ptr(z), N)
+    _call("linear", load().mis_linear_fwd, x2, C.byref(d))
+    return x2, w, y if x.dim() == 2 else y.view(shape), z
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, activation, residual):
-        x2, w, y, z = _linear_fwd(x, weight, bias, activation, residual, True)
+    def forward(ctx, x, weight, bias, act, residual):
+        x2, w, y, z = _linear_fwd(x, weight, bias, act, residual, True)
         ctx.save_for_backward(x2, w, z)
-        ctx.activation, ctx.shape = activation, x.shape
+        ctx.act, ctx.shape = act, x.shape
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
+        nx, nw, nb, _, nr = ctx.needs_input_grad
+        dres = dy if nr else None
+        if not (nx or nw or nb):
+            return None, None, None, None, dres
         x, w, z = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = _empty(x, *x.shape) if need[0] else None
-        dw = _empty(w, *w.shape) if need[1] else None
-        db = _empty(x, w.shape[0], dtype=torch.float32) if need[2] else None
-        if need[0] or need[1] or need[2]:
-            ops.linear_bwd(_rows(dy, w.shape[0], "dy"), x, w, ctx.activation, z, dx, dw, db)
-        return None if dx is None else dx.view(ctx.shape), dw, db, None, dy if need[4] else None
+        M, K = x.shape
+        N = w.shape[0]
+        d2 = _rows("linear (backward)", dy, N, "dy")
+        dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if nx else None
+        dw = torch.empty((N, K), dtype=x.dtype, device=x.device) if nw else None
+        db = torch.empty((N,), dtype=_F32, device=x.device) if nb else None
+        d = LinearDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, N, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), None, None, 0, None, 0, _ptr(z), N,
+                       d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dw), K, _ptr(db))
+        lib = load()
+        ws = _scratch(lib.mis_linear_bwd_workspace_bytes(C.byref(d)), x)
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        _call("linear (backward)", lib.mis_linear_bwd, x, C.byref(d))
+        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), dw, db, None, dres
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual; activation None | 'relu' | 'gelu' | 'gelu_tanh' | 'silu' | 'sigmoid', residual with the result's shape"""
-    if _grads(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, activation, residual)
-    return _linear_fwd(x, weight, bias, activation, residual, False)[2]
+    act = token_act(activation)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
+        return _Linear.apply(x, weight, bias, act, residual)
+    return _linear_fwd(x, weight, bias, act, residual, False)[2]
 
 
 # ---- gated feed-forward block ---------------------------------------------------------------------------------------------------------------
-def _gated_fwd(x, w_gate, w_up, b_gate, b_up, activation, keep):
-    wg, wu = _pair(_weight(w_gate, "gated_ffn: w_gate"), _weight(w_up, "gated_ffn: w_up"))
-    x2 = _rows(x, wg.shape[1], "gated_ffn: x")
-    M, F = x2.shape[0], wg.shape[0]
-    h = _empty(x2, M, F)
-    g, u = (_empty(x2, M, F, dtype=torch.float32), _empty(x2, M, F, dtype=torch.float32)) if keep else (None, None)
-    ops.gated_ffn_fwd(x2, wg, wu, h, b_gate, b_up, activation, g, u)
-    return x2, wg, wu, h.view(x.shape[:-1] + (F,)), g, u
+def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, keep):
+    wg, wu = _weight("gated_ffn", w_gate, "w_gate"), _weight("gated_ffn", w_up, "w_up")
+    F, K = wg.shape
+    if wu.shape != wg.shape:
+        _refuse("gated_ffn", f"w_gate and w_up must have one shape, got {_say(w_gate)} and {_say(w_up)}")
+    if F > 1 and wg.stride(0) != wu.stride(0):
+        wg, wu = wg.contiguous(), wu.contiguous()
+    x2, code = _tokens("gated_ffn", x, K)
+    _like("gated_ffn", wg, "w_gate", x2)
+    _like("gated_ffn", wu, "w_up", x2)
+    M = x2.shape[0]
+    pg, pu = _vec("gated_ffn", b_gate, "b_gate", F, x2), _vec("gated_ffn", b_up, "b_up", F, x2)
+    h = torch.empty((M, F), dtype=x2.dtype, device=x2.device)
+    z = torch.empty((2, M, F), dtype=_F32, device=x2.device) if keep else None
+    pz = z.data_ptr() if keep else None
+    d = GatedDesc(code, act, M, F, K, x2.data_ptr(), _ld(x2), wg.data_ptr(), wu.data_ptr(), _ld(wg), pg, pu, h.data_ptr(), F, pz, pz + 4 * M * F if keep else None, F)
+    _call("gated_ffn", load().mis_gated_ffn_fwd, x2, C.byref(d))
+    return x2, wg, wu, h if x.dim() == 2 else h.view(x.shape[:-1] + (F,)), z
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, b_gate, b_up, activation):
-        x2, wg, wu, h, g, u = _gated_fwd(x, w_gate, w_up, b_gate, b_up, activation, True)
-        ctx.save_for_backward(x2, wg, wu, g, u)
-        ctx.activation, ctx.shape = activation, x.shape
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
+        x2, wg, wu, h, z = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x2, wg, wu, z)
+        ctx.act, ctx.shape = act, x.shape
         return h
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
-        x, wg, wu, g, u = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        F, K = wg.shape
-        dx = _empty(x, *x.shape) if need[0] else None
-        dwg, dwu = (_empty(x, F, K), _empty(x, F, K)) if need[1] or need[2] else (None, None)
-        dbg = _empty(x, F, dtype=torch.float32) if need[3] else None
-        dbu = _empty(x, F, dtype=torch.float32) if need[4] else None
-        ops.gated_ffn_bwd(_rows(dh, F, "dh"), x, wg, wu, g, u, ctx.activation, dx, dwg, dwu, dbg, dbu)
-        return None if dx is None else dx.view(ctx.shape), dwg if need[1] else None, dwu if need[2] else None, dbg, dbu, None
+        x, wg, wu, z = ctx.saved_tensors
+        nx, ng, nu, nbg, nbu, _ = ctx.needs_input_grad
+        M, K = x.shape
+        F = wg.shape[0]
+        d2 = _rows("gated_ffn (backward)", dh, F, "dh")
+        dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if nx else None
+        dwg, dwu = (torch.empty((F, K), dtype=x.dtype, device=x.device), torch.empty((F, K), dtype=x.dtype, device=x.device)) if ng or nu else (None, None)
+        dbg = torch.empty((F,), dtype=_F32, device=x.device) if nbg else None
+        dbu = torch.empty((F,), dtype=_F32, device=x.device) if nbu else None
+        pz = z.data_ptr()
+        d = GatedDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, F, K, x.data_ptr(), _ld(x), wg.data_ptr(), wu.data_ptr(), _ld(wg), None, None, None, 0, pz, pz + 4 * M * F, F,
+                      d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dwg), _ptr(dwu), K, _ptr(dbg), _ptr(dbu))
+        lib = load()
+        ws = _scratch(lib.mis_gated_ffn_bwd_workspace_bytes(C.byref(d)), x)
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        _call("gated_ffn (backward)", lib.mis_gated_ffn_bwd, x, C.byref(d))
+        return dx if dx is None or len(ctx.shape) == 2 else dx.view(ctx.shape), dwg if ng else None, dwu if nu else None, dbg, dbu, None
 
 
 def gated_ffn(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """activation(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate, w_up (features, width), activation 'silu' | 'gelu' | 'gelu_tanh' | 'relu' | 'sigmoid' | None"""
-    if _grads(x, w_gate, w_up, b_gate, b_up):
-        return _GatedFFN.apply(x, w_gate, w_up, b_gate, b_up, activation)
-    return _gated_fwd(x, w_gate, w_up, b_gate, b_up, activation, False)[3]
+    act = token_act(activation)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or (b_gate is not None and b_gate.requires_grad) or
+                                    (b_up is not None and b_up.requires_grad)):
+        return _GatedFFN.apply(x, w_gate, w_up, b_gate, b_up, act)
+    return _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, False)[3]
