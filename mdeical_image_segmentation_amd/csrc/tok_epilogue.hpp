@@ -1,9 +1,13 @@
-// Epilogues of the token products: a lane holds runs of 8 consecutive columns of one row.
+// Epilogues of the token products: a lane holds runs of 8 consecutive columns of one row.  ACT: the activation, or -1: the descriptor's (a kernel that unrolls many rows takes it as a
+// template argument - six activations in each row make the code too long to unroll).
 #pragma once
 #include "tok_gemm.hpp"
 
+// where batch bt is stored (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
+__device__ __forceinline__ char* tg_out(const TgArgs& a, int bt) { return (char*)a.y + (long long)bt * ((char*)a.y2 - (char*)a.y); }
+
 // y = act(v + bias) + res, v (+ bias) kept in z
-template <typename T> struct TgLinearRow {
+template <typename T, int ACT = -1> struct TgLinearRow {
     const TgArgs& a;
     long long n;            // first column of the run
     int nv;                 // columns of it inside the matrix
@@ -19,7 +23,7 @@ template <typename T> struct TgLinearRow {
             for (int j = 0; j < 8; ++j) v[j] += bias[j];
         }
         if (a.z != nullptr) tok_stn<float>(a.z + m * a.ldz + n, v, nv);
-        tok_act8<sizeof(T) == 4, false>(a.act, v, nullptr);
+        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
         if (a.res != nullptr) {
             float r[8];
             tok_ldn<T>(reinterpret_cast<const T*>(a.res) + m * a.ldres + n, r, nv);
@@ -30,7 +34,7 @@ template <typename T> struct TgLinearRow {
     }
 };
 // h = act(g + bg) (u + bu), the two sums kept in z, z2
-template <typename T> struct TgGatedRow {
+template <typename T, int ACT = -1> struct TgGatedRow {
     const TgArgs& a;
     long long n;
     int nv;
@@ -52,7 +56,7 @@ template <typename T> struct TgGatedRow {
             tok_stn<float>(a.z + m * a.ldz + n, g, nv);
             tok_stn<float>(a.z2 + m * a.ldz + n, u, nv);
         }
-        tok_act8<sizeof(T) == 4, false>(a.act, g, nullptr);
+        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, g, nullptr);
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] *= u[j];
         tok_stn<T>(reinterpret_cast<T*>(a.y) + m * a.ldy + n, g, nv);

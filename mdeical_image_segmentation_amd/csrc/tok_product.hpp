@@ -144,17 +144,19 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
     const int tiles = pl.tm * pl.tn, all_steps = a.ranges * pl.spr;
 
     // items: batch-major, then k part, then tile; tiles in bands of 4 tile rows, column by column inside a band (the neighbours that run on an XCD share row and column panels in its L2)
-    auto tile_of = [&](int it, int& bt, int& sp, long long& m0, long long& n0) {
+    auto tile_of = [&](int it) __attribute__((always_inline)) {
+        TpItem w;
         const int bs = it / tiles, t = it - bs * tiles;
-        bt = bs / pl.splits;
-        sp = bs - bt * pl.splits;
+        w.bt = bs / pl.splits;
+        w.sp = bs - w.bt * pl.splits;
         const int band = t / (4 * pl.tn), in = t - band * 4 * pl.tn;
         const int h = pl.tm - band * 4 < 4 ? pl.tm - band * 4 : 4;
         const int c = in / h;
-        m0 = (long long)(band * 4 + in - c * h) * TILE;
-        n0 = (long long)c * BN;
+        w.m0 = (long long)(band * 4 + in - c * h) * TILE;
+        w.n0 = (long long)c * BN;
+        return w;
     };
-    auto steps_of = [&](int sp) { return all_steps - sp * pl.sps < pl.sps ? all_steps - sp * pl.sps : pl.sps; };
+    auto steps_of = [&](int sp) __attribute__((always_inline)) { return all_steps - sp * pl.sps < pl.sps ? all_steps - sp * pl.sps : pl.sps; };
 
     // ---- load cursor: the step that goes into the staging registers next ----
     TpStage<T, AMN, false, EPI, AL, F> ga(a.a.ld);
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
     TpStep na, nb;
     int lit = first, lrem = 0;
     const long long step_a = AMN ? CK * ES * a.a.ld : CK * ES, step_b = BMN ? CK * ES * a.b.ld : CK * ES;
-    auto place = [&](long long m0, long long n0, int bt, int at) {
+    auto place = [&](long long m0, long long n0, int bt, int at) __attribute__((always_inline)) {
         const int range = at >= pl.spr ? 1 : 0, ks = at - range * pl.spr;
         // (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
         const long long da = (const char*)a.a.p2 - (const char*)a.a.p, db = (const char*)a.b.p2 - (const char*)a.b.p;
@@ -173,28 +175,22 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         na.rows = a.M - m0;
         nb.rows = a.N - n0;
     };
-    auto load_tile = [&]() {
-        int bt, sp;
-        long long m0, n0;
-        tile_of(lit, bt, sp, m0, n0);
-        lrem = steps_of(sp);
-        place(m0, n0, bt, sp * pl.sps);
+    // the first step of item lit, or (second) of its second range
+    auto load_tile = [&](bool second) __attribute__((always_inline)) {
+        const TpItem w = tile_of(lit);
+        if (!second) lrem = steps_of(w.sp);
+        place(w.m0, w.n0, w.bt, second ? pl.spr : w.sp * pl.sps);
     };
-    auto advance = [&]() {                                    // behind the last step: rows 0, everything reads as zeros
+    auto advance = [&]() __attribute__((always_inline)) {     // behind the last step: rows 0, everything reads as zeros
         na.base += step_a;
         nb.base += step_b;
         nb.base2 += step_b;
         na.left -= CK;
         nb.left -= CK;
-        if (--lrem == 0) {
-            lit += gridDim.x;
-            if (lit < pl.items) load_tile();
+        if (--lrem == 0 || na.left <= 0) {
+            if (lrem == 0) lit += gridDim.x;
+            if (lit < pl.items) load_tile(lrem != 0);
             else na.rows = nb.rows = 0;
-        } else if (na.left <= 0) {                            // the second range of the same tile
-            int bt, sp;
-            long long m0, n0;
-            tile_of(lit, bt, sp, m0, n0);
-            place(m0, n0, bt, pl.spr);
         }
     };
 
@@ -209,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    load_tile();
+    load_tile(false);
 #pragma unroll
     for (int j = 0; j < F; ++j) {
         ga.load(na, j);
@@ -232,10 +228,9 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         tp_frag<T, BMN, true, F>(b0, smem + OP, wn, 0, f);
     }
 
-    int cit = first, crem, bt, sp, buf = 0;
-    long long m0, n0;
-    tile_of(cit, bt, sp, m0, n0);
-    crem = steps_of(sp);
+    int cit = first, buf = 0;
+    TpItem ct = tile_of(cit);
+    int crem = steps_of(ct.sp);
     while (true) {
         char* const cur = smem + buf * 2 * OP;
         char* const nxt = smem + (buf ^ 1) * 2 * OP;
@@ -281,11 +276,11 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
             static_assert(!Run::R4, "gated: k-contiguous weights only");
 #pragma unroll
             for (int b = 0; b < F / 4; ++b) {                  // MFMA tiles 4 b, 4 b + 1 hold 8 gate columns of a lane, 4 b + 2, 4 b + 3 the same columns of up
-                const TgGatedRow<T> row(a, n0 + wn * 8 * F + 32 * b + 8 * lg);
+                const TgGatedRow<T> row(a, ct.n0 + wn * 8 * F + 32 * b + 8 * lg);
                 if (row.nv > 0) {
 #pragma unroll
                     for (int p = 0; p < F; ++p) {
-                        const long long m = m0 + wm * 16 * F + 16 * p + li;
+                        const long long m = ct.m0 + wm * 16 * F + 16 * p + li;
                         float g[8], u[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -299,13 +294,13 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         } else {
 #pragma unroll
             for (int h = 0; h < F / 2; ++h) {
-                const long long n = n0 + wn * 16 * F + Run::base(h, lg);
-                const TgLinearRow<T> row(a, bt == 0 ? a.y : a.y2, n, EPI == TG_LINEAR);
-                float* const sl = pl.slab + (long long)(bt * pl.splits + sp) * a.M * a.N + n;
+                const long long n = ct.n0 + wn * 16 * F + Run::base(h, lg);
+                const TgLinearRow<T> row(a, tg_out(a, ct.bt), n, EPI == TG_LINEAR);
+                float* const sl = pl.slab + (long long)(ct.bt * pl.splits + ct.sp) * a.M * a.N + n;
                 if (row.nv > 0) {
 #pragma unroll
                     for (int p = 0; p < F; ++p) {
-                        const long long m = m0 + wm * 16 * F + ((AMN && ES == 4) ? 4 * li + p : 16 * p + li);
+                        const long long m = ct.m0 + wm * 16 * F + ((AMN && ES == 4) ? 4 * li + p : 16 * p + li);
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = acc[Run::f(h, j)][p][Run::q(h, j)];
@@ -324,8 +319,8 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         for (int f = 0; f < F; ++f)
 #pragma unroll
             for (int p = 0; p < F; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
-        tile_of(cit, bt, sp, m0, n0);
-        crem = steps_of(sp);
+        ct = tile_of(cit);
+        crem = steps_of(ct.sp);
     }
 }
 

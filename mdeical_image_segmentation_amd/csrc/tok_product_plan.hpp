@@ -2,6 +2,11 @@
 #pragma once
 #include "tok_gemm.hpp"
 
+// where a work item lies
+struct TpItem {
+    int bt, sp;             // batch, part of k
+    long long m0, n0;
+};
 struct TpPlan {
     int tm, tn;             // tiles of a product
     int splits;             // parts of the k steps (TG_SLAB, else 1)

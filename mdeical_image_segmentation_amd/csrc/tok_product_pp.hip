@@ -237,25 +237,22 @@ struct PgLane {
     int row;                // k contiguous: row of the first instruction; else first column of the chunk
     int k;                  // k contiguous: first k of the chunk; else k row of the first instruction
 };
-// one operand's 64-k step (wave-uniform)
+// one operand's 64-k step: its first element, and this lane's four byte offsets.  Valid lanes are inside the operand by construction; a lane that has to read zeros (behind the last
+// row or k) carries an offset past num_records.
 struct PgStep {
     const char* base;
-    int left;               // k present, 64 or fewer
-    int rows;               // tile rows (columns) present
+    unsigned v[4];
 };
-
-// The wave's four instructions of a step.  Valid lanes are inside the operand by construction; a lane that has to read zeros carries an offset past num_records.
-template <bool MN, int RSTEP> __device__ __forceinline__ PgDma pg_dma(const PgLane& l, const PgStep& s, char* dst, int wave) {
-    PgDma d;
-    d.rsrc = i32x4{(int)(uint32_t)(uintptr_t)s.base, (int)((uintptr_t)s.base >> 32) & 0xffff, 0x7fffffff, 0x00020000};          // raw buffer, stride 0
-    d.step = (int)l.jstep;
-    d.dst = (uint32_t)(uintptr_t)dst + wave * 1024;
+template <bool MN, int RSTEP> __device__ __forceinline__ void pg_mask(const PgLane& l, PgStep& s, int left, int rows) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const bool ok = MN ? (l.k + 16 * j < s.left && l.row < s.rows) : (l.k < s.left && l.row + RSTEP * j < s.rows);
-        d.v[j] = ok ? l.v0 : (unsigned)PP_OOB;
+        const bool ok = MN ? (l.k + 16 * j < left && l.row < rows) : (l.k < left && l.row + RSTEP * j < rows);
+        s.v[j] = ok ? l.v0 : (unsigned)PP_OOB;
     }
-    return d;
+}
+__device__ __forceinline__ PgDma pg_dma(const PgLane& l, const PgStep& s, uint32_t dst) {
+    const uintptr_t b = (uintptr_t)s.base;
+    return PgDma{{s.v[0], s.v[1], s.v[2], s.v[3]}, i32x4{(int)(uint32_t)b, (int)(b >> 32), 0x7fffffff, 0x00020000}, (int)l.jstep, dst};          // raw buffer, stride 0
 }
 __device__ __forceinline__ void pg_issue(const PgDma& d) {
     int t;
@@ -263,7 +260,7 @@ __device__ __forceinline__ void pg_issue(const PgDma& d) {
 }
 }   // namespace
 
-template <bool AMN, bool BMN, int EPI>
+template <bool AMN, bool BMN, int EPI, int ACT>
 __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpPlan pl) {
     using T = __bf16;
     constexpr int BN = EPI == TG_GATED ? 128 : 256;          // columns of C a tile covers
@@ -282,8 +279,8 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
     uint32_t fA, fB;
     if constexpr (!AMN) fA = wm * 16384 + li * 128 + ((lg ^ (li >> 1)) << 4);
     else fA = (8 * lg + (li >> 2)) * 512 + ((wm * 8 + ((li >> 2) | ((lg & 1) << 2))) << 5) + 8 * (li & 3);
-    if constexpr (!BMN) fB = PG_B0 + wn * 8192 + (8 * (li >> 2) + (li & 3)) * 128 + ((lg ^ (((li >> 1) & 1) | ((li >> 2) << 1))) << 4);
-    else fB = PG_B0 + (8 * lg + (li >> 2)) * 512 + (((wn * 4 + ((li & 3) >> 1)) ^ ((li >> 2) << 1)) << 5) + 16 * (li & 1);
+    if constexpr (!BMN) fB = wn * 8192 + (8 * (li >> 2) + (li & 3)) * 128 + ((lg ^ (((li >> 1) & 1) | ((li >> 2) << 1))) << 4);
+    else fB = (8 * lg + (li >> 2)) * 512 + (((wn * 4 + ((li & 3) >> 1)) ^ ((li >> 2) << 1)) << 5) + 16 * (li & 1);
 
     // ---- DMA source offsets of this lane ----
     PgLane la, lb;
@@ -316,71 +313,73 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
     }
 
     // items: batch-major, then k part, then tile; tiles in bands of 4 tile rows, column by column inside a band (32 neighbours of an XCD share 4 row panels and 8 column panels in its L2)
-    auto tile_of = [&](int it, int& bt, int& sp, long long& m0, long long& n0) {
+    auto tile_of = [&](int it) __attribute__((always_inline)) {
+        TpItem w;
         const int t = it % tiles, bs = it / tiles;
-        sp = bs % pl.splits;
-        bt = bs / pl.splits;
+        w.sp = bs % pl.splits;
+        w.bt = bs / pl.splits;
         const int band = t / (4 * pl.tn), in = t - band * 4 * pl.tn;
         const int h = pl.tm - band * 4 < 4 ? pl.tm - band * 4 : 4;
         const int c = in / h;
-        m0 = (long long)(band * 4 + in - c * h) * 256;
-        n0 = (long long)c * BN;
+        w.m0 = (long long)(band * 4 + in - c * h) * 256;
+        w.n0 = (long long)c * BN;
+        return w;
     };
-    auto steps_of = [&](int sp) {
+    auto steps_of = [&](int sp) __attribute__((always_inline)) {
         const int s0 = sp * pl.sps;
         return nsteps_all - s0 < pl.sps ? nsteps_all - s0 : pl.sps;
     };
 
     // ---- load cursor: `na` is the step whose A is issued next, `nb` the one whose B is (the step before, once the pipeline runs) ----
-    int lit = first, lrange = 0, lrem = 0, krem = 0;          // item, range, steps of the item from the cursor's on, k of the range from the cursor's on
+    int lit = first, lrem = 0, krem = 0;                      // item; its steps, and k of its range, from the cursor's step on
+    int rows_a = 0, rows_b = 0;                               // rows and columns of its tile that exist
     PgStep na, nb, nb1;                                       // nb1: B of na's step
-    bool va = true, vb = true;                                // whether na / nb is a step of this block
+    int va = 1, vb = 1;                                       // whether na / nb is a step of this block
     const long long step_a = AMN ? 128 * a.a.ld : 128, step_b = BMN ? 128 * a.b.ld : 128;
-    auto flags = [&]() __attribute__((always_inline)) {
-        na.left = nb1.left = krem < 64 ? krem : 64;
+    auto masks = [&]() __attribute__((always_inline)) {
+        const int left = krem < 64 ? krem : 64;
+        pg_mask<AMN, 64>(la, na, left, rows_a);
+        pg_mask<BMN, BROWS>(lb, nb1, left, rows_b);
     };
     // (tile, k part) of item lit at step `at` of its product -> na, nb1
-    auto place = [&](long long m0, long long n0, int bt, int at) {
-        lrange = at >= pl.spr ? 1 : 0;
-        const int ks = at - lrange * pl.spr;
+    auto place = [&](long long m0, long long n0, int bt, int at) __attribute__((always_inline)) {
+        const int range = at >= pl.spr ? 1 : 0, ks = at - range * pl.spr;
         // (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
-        const char* const pa = (const char*)a.a.p + (long long)(AMN ? bt : lrange) * ((const char*)a.a.p2 - (const char*)a.a.p);
-        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : lrange) * ((const char*)a.b.p2 - (const char*)a.b.p);
+        const char* const pa = (const char*)a.a.p + (long long)(AMN ? bt : range) * ((const char*)a.a.p2 - (const char*)a.a.p);
+        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : range) * ((const char*)a.b.p2 - (const char*)a.b.p);
         na.base = pa + (AMN ? m0 : m0 * a.a.ld) * 2 + ks * step_a;
         nb1.base = pb + (BMN ? n0 : n0 * a.b.ld) * 2 + ks * step_b;
         krem = (int)a.K - ks * 64;
-        na.rows = a.M - m0 < 256 ? (int)(a.M - m0) : 256;
-        nb1.rows = a.N - n0 < BN ? (int)(a.N - n0) : BN;
-        flags();
+        rows_a = a.M - m0 < 256 ? (int)(a.M - m0) : 256;
+        rows_b = a.N - n0 < BN ? (int)(a.N - n0) : BN;
+        masks();
     };
-    auto load_tile = [&]() {
-        int bt, sp;
-        long long m0, n0;
-        tile_of(lit, bt, sp, m0, n0);
-        lrem = steps_of(sp);
-        place(m0, n0, bt, sp * pl.sps);
+    // the first step of item lit, or (second) of its second range
+    auto load_tile = [&](bool second) __attribute__((always_inline)) {
+        const TpItem w = tile_of(lit);
+        if (!second) lrem = steps_of(w.sp);
+        place(w.m0, w.n0, w.bt, second ? pl.spr : w.sp * pl.sps);
     };
-    auto advance = [&]() __attribute__((always_inline)) {     // A of the cursor's step is issued: its B is next, and A of the step behind it
+    // A of the cursor's step is issued: its B is next, and A of the step behind it.  tick: straight-line, between the MFMAs; turn: what happens at the end of a range or a tile
+    auto tick = [&]() __attribute__((always_inline)) {
         nb = nb1;
         vb = va;
-        if (!va) return;
         na.base += step_a;
         nb1.base += step_b;
         krem -= 64;
-        if (--lrem == 0) {
-            lit += gridDim.x;
-            va = lit < pl.items;
-            if (va) load_tile();
-        } else if (krem <= 0) {                               // the second range of the same tile
-            int bt, sp;
-            long long m0, n0;
-            tile_of(lit, bt, sp, m0, n0);
-            place(m0, n0, bt, pl.spr);
-        } else {
-            flags();
+        lrem -= 1;
+    };
+    auto turn = [&]() __attribute__((always_inline)) {
+        if (va && (lrem == 0 || krem < 64)) {
+            if (lrem == 0) {
+                lit += gridDim.x;
+                va = lit < pl.items ? 1 : 0;
+            }
+            if (lrem != 0 && krem > 0) masks();               // the last, short step of a range
+            else if (va) load_tile(lrem != 0);
         }
     };
-    load_tile();
+    load_tile(false);
 
     f32x4 acc[4][8];
 #pragma unroll
@@ -388,34 +387,33 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
 #pragma unroll
         for (int p = 0; p < 8; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    int sA = 0, sB = 0;                                       // buffers of the current step
-    auto a_buf = [&](int ahead) { return smem + (sA + ahead >= 3 ? sA + ahead - 3 : sA + ahead) * PG_OP; };
-    auto b_buf = [&](int ahead) { return smem + PG_B0 + ((sB + ahead) & 1) * PG_OP; };
-    auto dma_a = [&](char* dst) __attribute__((always_inline)) { return pg_dma<AMN, 64>(la, na, dst, wave); };
-    auto dma_b = [&](char* dst) __attribute__((always_inline)) { return pg_dma<BMN, BROWS>(lb, nb, dst, wave); };
-    pg_issue(dma_a(smem));
-    advance();
-    pg_issue(dma_b(smem + PG_B0));
-    if (va) pg_issue(dma_a(a_buf(1)));                        // A of step 1
-    advance();                                                // nb: B of step 1, na: A of step 2
+    // LDS addresses of the current step's buffers, and of where B(s + 1) and A(s + 2) of this wave go
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem, ldsB = lds0 + PG_B0;
+    uint32_t curA = lds0, curB = ldsB, dstA = lds0 + 2 * PG_OP + wave * 1024, dstB = ldsB + PG_OP + wave * 1024;
+    pg_issue(pg_dma(la, na, lds0 + wave * 1024));
+    tick();
+    turn();
+    pg_issue(pg_dma(lb, nb, ldsB + wave * 1024));
+    if (va) pg_issue(pg_dma(la, na, lds0 + PG_OP + wave * 1024));          // A of step 1
+    tick();
+    turn();                                                   // nb: B of step 1, na: A of step 2
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (grp == 1) __builtin_amdgcn_s_barrier();               // the stagger
     __builtin_amdgcn_sched_barrier(0);
 
-    int cit = first, crem, bt, sp;
-    long long m0, n0;
-    tile_of(cit, bt, sp, m0, n0);
-    crem = steps_of(sp);
+    int cit = first;
+    TpItem ct = tile_of(cit);
+    int crem = steps_of(ct.sp);
 
     u32x4 fa[8], fb[4];
     // the fragments of half kk; with `dma` also this segment's part of the prefetch: B of step s + 1 (half 0), A of step s + 2 (half 1)
-    auto read = [&](int kk, bool dma) __attribute__((always_inline)) {
+    auto read = [&](int kk, int dma) __attribute__((always_inline)) {
         // k-contiguous: the second half of the step is 64 bytes further in the row, i.e. chunk position ^ 4; else 32 k rows further
-        const uint32_t xa = (uint32_t)(uintptr_t)smem + sA * PG_OP + (AMN ? fA + kk * 16384 : fA ^ (kk * 64));
-        const uint32_t xb = (uint32_t)(uintptr_t)smem + sB * PG_OP + (BMN ? fB + kk * 16384 : fB ^ (kk * 64));
+        const uint32_t xa = curA + (AMN ? fA + kk * 16384 : fA ^ (kk * 64));
+        const uint32_t xb = curB + (BMN ? fB + kk * 16384 : fB ^ (kk * 64));
         if (dma) {
-            const PgDma d = kk == 0 ? dma_b(b_buf(1)) : dma_a(a_buf(2));
+            const PgDma d = kk == 0 ? pg_dma(lb, nb, dstB) : pg_dma(la, na, dstA);
             if constexpr (!AMN && !BMN) pg_read_kk_dma(fa, fb, xa, xb, d);
             else if constexpr (!AMN) pg_read_km_dma(fa, fb, xa, xb, d);
             else pg_read_mm1_dma(fa, fb, xa, xb, d);
@@ -428,13 +426,15 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         __builtin_amdgcn_sched_barrier(0);
     };
     auto mma = [&]() __attribute__((always_inline)) {
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int f = 0; f < 4; ++f)
 #pragma unroll
             for (int p = 0; p < 8; ++p) mma_b128<T>(acc[f][p], fb[f], fa[p]);
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {                        // two MFMAs, then what fits beside them
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x6, 2, 0);
+        }
     };
     auto barrier = [&]() __attribute__((always_inline)) {
         __builtin_amdgcn_sched_barrier(0);
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         __builtin_amdgcn_sched_barrier(0);
     };
     // step s + 1 is complete once at most the four A(s + 2) just issued are in flight
-    auto retire = [&](bool inflight) __attribute__((always_inline)) {
+    auto retire = [&](int inflight) __attribute__((always_inline)) {
         if (inflight) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
@@ -450,30 +450,38 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
 #pragma unroll 1
     while (true) {
         // ---- segment 0 ----
-        __builtin_amdgcn_s_sleep(1);                          // keep a distance between the barrier that published this step and its first read
+        if (grp == 0) __builtin_amdgcn_s_sleep(1);            // keep a distance between the barrier that published this step and its first read
         read(0, vb);
         barrier();
+        __builtin_amdgcn_s_setprio(1);
         mma();
+        __builtin_amdgcn_s_setprio(0);
         barrier();
         // ---- segment 1 ----
-        const bool inflight = va;
+        const int inflight = va;
         read(1, va);
         if (grp == 1) retire(inflight);
         barrier();
+        __builtin_amdgcn_s_setprio(1);
+        tick();
+        curA = curA == lds0 + 2 * PG_OP ? lds0 : curA + PG_OP;
+        dstA = curA == lds0 ? lds0 + 2 * PG_OP + wave * 1024 : curA - PG_OP + wave * 1024;
+        dstB = curB + wave * 1024;
+        curB = ldsB + PG_OP - (curB - ldsB);
         mma();
-        advance();
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
         if (grp == 0) retire(inflight);
+        turn();
         barrier();
-        sA = sA == 2 ? 0 : sA + 1;
-        sB ^= 1;
         if (--crem == 0) {
             // ---- this wave's part of the tile is complete ----
             if constexpr (EPI == TG_GATED) {
-                const TgGatedRow<T> row(a, n0 + wn * 32 + 8 * lg);
+                const TgGatedRow<T, ACT> row(a, ct.n0 + wn * 32 + 8 * lg);
                 if (row.nv > 0) {
 #pragma unroll
                     for (int p = 0; p < 8; ++p) {
-                        const long long m = m0 + wm * 128 + 16 * p + li;
+                        const long long m = ct.m0 + wm * 128 + 16 * p + li;
                         float g[8], u[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -486,13 +494,13 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const long long n = n0 + wn * 64 + 32 * h + 8 * lg;
-                    const TgLinearRow<T> row(a, bt == 0 ? a.y : a.y2, n, EPI == TG_LINEAR);
-                    float* const sl = pl.slab + (long long)(bt * pl.splits + sp) * a.M * a.N + n;
+                    const long long n = ct.n0 + wn * 64 + 32 * h + 8 * lg;
+                    const TgLinearRow<T, ACT> row(a, tg_out(a, ct.bt), n, EPI == TG_LINEAR);
+                    float* const sl = pl.slab + (long long)(ct.bt * pl.splits + ct.sp) * a.M * a.N + n;
                     if (row.nv > 0) {
 #pragma unroll
                         for (int p = 0; p < 8; ++p) {
-                            const long long m = m0 + wm * 128 + 16 * p + li;
+                            const long long m = ct.m0 + wm * 128 + 16 * p + li;
                             float v[8];
 #pragma unroll
                             for (int j = 0; j < 8; ++j) v[j] = acc[2 * h + (j >> 2)][p][j & 3];
@@ -511,8 +519,8 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
                 for (int p = 0; p < 8; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
             cit += gridDim.x;
             if (cit >= pl.items) break;
-            tile_of(cit, bt, sp, m0, n0);
-            crem = steps_of(sp);
+            ct = tile_of(cit);
+            crem = steps_of(ct.sp);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -521,19 +529,29 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
 
 // ---------------------------------------------------------------------------------------------------------
 namespace {
-template <bool AMN, bool BMN, int EPI> int pg_go(const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
+template <bool AMN, bool BMN, int EPI, int ACT = MIS_ACT_NONE> int pg_go(const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
     static std::atomic<unsigned long long> attr_done{0};
-    if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tg_pp_kernel<AMN, BMN, EPI>), PG_LDS, "token product")) return rc;
+    if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tg_pp_kernel<AMN, BMN, EPI, ACT>), PG_LDS, "token product")) return rc;
     const int cus = mis_persist_cus();
-    hipLaunchKernelGGL((tg_pp_kernel<AMN, BMN, EPI>), dim3((unsigned)(pl.items < cus ? pl.items : cus)), dim3(512), PG_LDS, stream, a, pl);
+    hipLaunchKernelGGL((tg_pp_kernel<AMN, BMN, EPI, ACT>), dim3((unsigned)(pl.items < cus ? pl.items : cus)), dim3(512), PG_LDS, stream, a, pl);
     MIS_LAUNCH_CHECK("token product (256 x 256)");
     return MIS_OK;
+}
+template <int EPI> int pg_act(const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
+    switch (a.act) {
+        case MIS_ACT_RELU: return pg_go<false, false, EPI, MIS_ACT_RELU>(a, pl, stream);
+        case MIS_ACT_GELU: return pg_go<false, false, EPI, MIS_ACT_GELU>(a, pl, stream);
+        case MIS_ACT_GELU_TANH: return pg_go<false, false, EPI, MIS_ACT_GELU_TANH>(a, pl, stream);
+        case MIS_ACT_SILU: return pg_go<false, false, EPI, MIS_ACT_SILU>(a, pl, stream);
+        case MIS_ACT_SIGMOID: return pg_go<false, false, EPI, MIS_ACT_SIGMOID>(a, pl, stream);
+        default: return pg_go<false, false, EPI, MIS_ACT_NONE>(a, pl, stream);
+    }
 }
 }   // namespace
 
 int tok_product_bf16_256(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
-    if (epi == TG_GATED) return pg_go<false, false, TG_GATED>(a, pl, stream);
-    if (!a_mn && !b_mn) return pg_go<false, false, TG_LINEAR>(a, pl, stream);
+    if (epi == TG_GATED) return pg_act<TG_GATED>(a, pl, stream);
+    if (!a_mn && !b_mn) return pg_act<TG_LINEAR>(a, pl, stream);
     if (pl.splits == 1) return a_mn ? pg_go<true, true, TG_STORE>(a, pl, stream) : pg_go<false, true, TG_STORE>(a, pl, stream);
     return a_mn ? pg_go<true, true, TG_SLAB>(a, pl, stream) : pg_go<false, true, TG_SLAB>(a, pl, stream);
 }
