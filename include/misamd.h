@@ -632,6 +632,7 @@ typedef struct MisLinearDesc {
     void* workspace; size_t workspace_bytes;
 } MisLinearDesc;
 int mis_linear_fwd(const MisLinearDesc* d, void* stream);
+/* (of the descriptor as it will be passed: pointers and strides decide whether operands are copied to aligned rows) */
 size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d);
 int mis_linear_bwd(const MisLinearDesc* d, void* stream);
 

@@ -33,40 +33,47 @@ static int tg_slab_sum(int dtype, const TgArgs& a, const float* slab, int splits
 }
 
 namespace {
-// How a product is cut.  Costs in microseconds: a 64-k step of a 256 x 256 tile takes a CU 1.55 us, of each of two 128 x 128 tiles 1.25 us (8192^3: 1.33 and 0.83 PFLOP/s; f32
-// 13 times that), a tile's start and epilogue about three steps; a k part costs its slab's write and read at the copy rate.
+// How a product is cut.  Costs in microseconds per 64-k step, all the blocks of a CU at work: one 256 x 256 tile 1.55, two 128 x 128 tiles 1.25, four 64 x 64 tiles 1.0 (8192^3 at 1.39, 0.83
+// PFLOP/s; f32 takes TG_F32 times as long); a tile's start and epilogue about three steps; a k part its slab's write and read at the copy rate.
 struct TgCut {
-    bool big;               // 256 x 256 tiles, else 128 x 128
+    int tile;               // 256, 128 or 64 rows
     int splits;
     double us;
 };
-TgCut tg_cut_one(int dtype, bool big, bool may_split, long long M, long long N, long long K, int ranges, int batches, bool gated) {
-    const int T = big ? 256 : 128, cols = gated ? T / 2 : T;
-    const long long items = ((M + T - 1) / T) * ((N + cols - 1) / cols) * batches, steps = ((K + 63) / 64) * ranges;
-    if (const int forced = mis_sw(SW_TOK_SPLITS); may_split && forced > 0) return TgCut{big, (int)(forced < steps ? forced : steps), 0.0};
-    const double step = (big ? 1.55 : 1.25) * (dtype == MIS_BF16 ? 1.0 : 13.0);
-    const long long slots = big ? 256 : 512;
-    TgCut best{big, 1, 1e30};
+constexpr double TG_F32[2] = {5.6, 3.7};          // f32 against bf16: 128 x 128, 64 x 64
+TgCut tg_cut_one(int dtype, int tile, bool may_split, long long M, long long N, long long K, int ranges, int batches, bool gated) {
+    const int cols = gated ? (tile == 256 ? 128 : 64) : tile;
+    const long long items = ((M + tile - 1) / tile) * ((N + cols - 1) / cols) * batches, steps = ((K + 63) / 64) * ranges;
+    if (const int forced = mis_sw(SW_TOK_SPLITS); may_split && forced > 0) return TgCut{tile, (int)(forced < steps ? forced : steps), 0.0};
+    const double step = (tile == 256 ? 1.55 : tile == 128 ? 1.25 : (gated ? 1.2 : 1.0)) * (dtype == MIS_BF16 ? 1.0 : TG_F32[tile == 64]);
+    const long long slots = tile == 256 ? 256 : tile == 128 ? 512 : (gated ? 768 : 1024);
+    TgCut best{tile, 1, 1e30};
     for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || steps / s >= 4); ++s) {
         const double rounds = (double)((items * s + slots - 1) / slots);
         double us = rounds * ((double)((steps + s - 1) / s) + 3.0) * step;
         if (s > 1) us += 3.0 + 8.0 * s * (double)M * (double)N * batches / 4.7e6;
-        if (us < best.us * 0.97) best = TgCut{big, s, us};
+        if (us < best.us * 0.97) best = TgCut{tile, s, us};
     }
     return best;
 }
 TgCut tg_cut(int dtype, bool aligned, bool may_split, long long M, long long N, long long K, int ranges, int batches, bool gated) {
-    const TgCut small = tg_cut_one(dtype, false, may_split, M, N, K, ranges, batches, gated);
-    const int forced = mis_sw(SW_TOK_TILE);
-    if (dtype != MIS_BF16 || !aligned || forced == 1) return small;
-    const TgCut big = tg_cut_one(dtype, true, may_split, M, N, K, ranges, batches, gated);
-    return big.us <= small.us || forced == 2 ? big : small;
+    const int forced = mis_sw(SW_TOK_TILE);          // 1: 128, 2: 256 wherever the operands allow, 3: 64
+    const bool big_ok = dtype == MIS_BF16 && aligned;
+    if (forced == 1 || forced == 3 || (forced == 2 && big_ok)) return tg_cut_one(dtype, forced == 1 ? 128 : forced == 2 ? 256 : 64, may_split, M, N, K, ranges, batches, gated);
+    TgCut best = tg_cut_one(dtype, 128, may_split, M, N, K, ranges, batches, gated);
+    const TgCut small = tg_cut_one(dtype, 64, may_split, M, N, K, ranges, batches, gated);
+    if (small.us < best.us) best = small;
+    if (big_ok) {
+        const TgCut big = tg_cut_one(dtype, 256, may_split, M, N, K, ranges, batches, gated);
+        if (big.us <= best.us) best = big;
+    }
+    return best;
 }
-// 16-byte chunks from 16-byte addresses and 32-bit offsets inside a tile; a k-contiguous operand's k, the other kind's own index must be whole chunks
+// 16-byte chunks from 16-byte addresses and 32-bit offsets inside a tile; a k-contiguous operand's k, the other kind's own index must be whole chunks or padded to them
 bool tg_aligned(int dtype, const TgArgs& a, int a_mn, int b_mn) {
     const long long es = dtype == MIS_BF16 ? 2 : 4, epc = 16 / es;
     auto ok = [&](const TgOperand& o, int mn, long long I) {
-        return ((uintptr_t)o.p | (uintptr_t)o.p2 | (size_t)(o.ld * es)) % 16 == 0 && o.ld <= (1 << 20) && (mn ? I : a.K) % epc == 0;
+        return ((uintptr_t)o.p | (uintptr_t)o.p2 | (size_t)(o.ld * es)) % 16 == 0 && o.ld <= (1 << 20) && (o.padded || (mn ? I : a.K) % epc == 0);
     };
     return ok(a.a, a_mn, a.M) && ok(a.b, b_mn, a.N);
 }
@@ -86,7 +93,7 @@ int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* sl
     const bool al = tg_aligned(dtype, a, a_mn, b_mn);
     if (epi != TG_STORE && a.M <= 64 && mis_sw(SW_TOK_TILE) == 0) return tok_product_skinny(dtype, epi, a, al, stream);
     const TgCut c = tg_cut(dtype, al, epi == TG_STORE, a.M, a.N, a.K, a.ranges, a.batches, epi == TG_GATED);
-    const long long T = c.big ? 256 : 128, BN = epi == TG_GATED ? T / 2 : T, ck = dtype == MIS_BF16 ? 64 : 32;
+    const long long T = c.tile, BN = epi == TG_GATED ? (T == 256 ? 128 : 64) : T, ck = dtype == MIS_BF16 ? 64 : 32;
     const long long tm = (a.M + T - 1) / T, tn = (a.N + BN - 1) / BN, spr = (a.K + ck - 1) / ck;
     MIS_REQUIRE(tm < (1ll << 24) && tn < (1ll << 24) && spr < (1ll << 28) && tm * tn * a.batches * c.splits < (1ll << 30), MIS_EUNSUPPORTED,
                 "token product: %lld x %lld tiles of %lld steps are too many", tm, tn, spr);
@@ -97,8 +104,10 @@ int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* sl
     pl.splits = (int)((spr * a.ranges + pl.sps - 1) / pl.sps);          // (no part is empty)
     pl.slab = slab;
     pl.items = (int)(tm * tn * a.batches * pl.splits);
-    auto* const go = dtype == MIS_F32 ? (al ? tok_product_f32_128 : tok_product_f32_128_any)
-                     : c.big ? tok_product_bf16_256 : (al ? tok_product_bf16_128 : tok_product_bf16_128_any);
+    static int (*const kernels[2][2][2])(int, int, int, const TgArgs&, const TpPlan&, hipStream_t) = {          // [f32][64][any address]
+        {{tok_product_bf16_128, tok_product_bf16_128_any}, {tok_product_bf16_64, tok_product_bf16_64_any}},
+        {{tok_product_f32_128, tok_product_f32_128_any}, {tok_product_f32_64, tok_product_f32_64_any}}};
+    auto* const go = T == 256 ? tok_product_bf16_256 : kernels[dtype == MIS_F32][T == 64][!al];
     if (const int rc = go(a_mn, b_mn, epi, a, pl, stream)) return rc;
     return pl.splits > 1 ? tg_slab_sum(dtype, a, slab, pl.splits, stream) : MIS_OK;
 }

@@ -9,6 +9,7 @@ struct TgOperand {
     const void* p;          // element (i, k): p[i * ld + k] (k contiguous) or p[k * ld + i]
     const void* p2;
     long long ld;
+    bool padded;            // rows end on a whole 16-byte chunk whose surplus is readable, and zero where it lies along k
 };
 enum { TG_LINEAR = 0, TG_GATED = 1, TG_STORE = 2, TG_SLAB = 3 };          // epilogues: forward products; a rounded store (gradients); an f32 slab of one part of k (internal)
 struct TgArgs {

@@ -1,6 +1,7 @@
 // The kernel of the token products, any shape / stride / alignment: C[m][n] = sum_k A(m, k) B(n, k) (tok_gemm.hpp), included by one .hip per (type, tile).
 //
-// A block of 4 waves (2 x 2) owns a 128 x 128 piece of C (two blocks per CU), a wave F x F MFMA tiles of 16 x 16, F = 4.
+// A block of 4 waves (2 x 2) owns a 32 FM x 32 FN piece of C, a wave FM x FN MFMA tiles of 16 x 16: 128 x 128 (two blocks per CU) where that fills the chip, 64 x 64 (four) for smaller
+// products - gated 64 rows x 64 columns of gate and of up.
 //
 // A step is 128 bytes of k per row (64 bf16 / 32 f32), in two halves.  The pipeline of a wave, all of it plain code whose waits the compiler counts:
 //      half 0   MFMAs of half 0 | fragments of half 1 <- LDS | step s + 1: registers -> other LDS buffer | step s + 2: global -> registers
@@ -26,9 +27,11 @@ constexpr int TP_OOB = (int)0xFFFFFF00u;          // past every buffer below: re
 template <bool B> __device__ __forceinline__ int tp_key(int row) {
     return B ? (((row >> 1) & 1) | (((row >> 3) & 3) << 1)) : ((row >> 1) & 7);
 }
-// 32-byte position of a [k][i] bf16 row.  A side: a group of 16 lanes reads 32 bytes of 4 rows; B side: 8 of every 16 bytes of a 64-byte run of 4 rows
-template <bool B> __device__ __forceinline__ int tp_pos32(int c32, int k) {
-    return B ? (c32 ^ ((k & 3) << 1)) : (c32 ^ ((k & 3) | (((k >> 3) & 1) << 2)));
+// 32-byte position of a [k][i] bf16 row of TILE elements.  A side: a group of 16 lanes reads 32 bytes of 4 rows; B side: 8 of every 16 bytes of a 64-byte run of 4 rows.  (64 elements: two
+// rows share the 256 bytes of the banks.)
+template <bool B, int TILE> __device__ __forceinline__ int tp_pos32(int c32, int k) {
+    if constexpr (TILE == 64) return B ? (c32 ^ (k & 2)) : (c32 ^ (((k >> 1) & 1) | (((k >> 3) & 1) << 1)));
+    else return B ? (c32 ^ ((k & 3) << 1)) : (c32 ^ ((k & 3) | (((k >> 3) & 1) << 2)));
 }
 // one 16-byte chunk of which n elements exist, at any element address
 template <typename T> __device__ __forceinline__ u32x4 tp_chunk(const T* p, long long n) {
@@ -87,7 +90,7 @@ template <typename T, bool MN, bool B, int EPI, bool AL, int F> struct TpStage {
             off = (r + 32 * j) * 128 + ((c ^ tp_key<B>(r)) << 4);          // (key(r + 32 j) = key(r))
         } else if constexpr (ES == 2) {
             const int k = r + j * KR;
-            off = k * (TILE * 2) + (tp_pos32<B>(c >> 1, k) << 5) + ((c & 1) << 4);
+            off = k * (TILE * 2) + (tp_pos32<B, TILE>(c >> 1, k) << 5) + ((c & 1) << 4);
         } else {
             off = (r + j * KR) * (TILE * 4) + c * 16;
         }
@@ -108,34 +111,37 @@ template <typename T, bool MN, bool B, int F> __device__ __forceinline__ void tp
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int k = kk * 32 + 8 * lg + 4 * s + (li >> 2);
-            const uint32_t at = (uint32_t)(uintptr_t)lds + k * (TILE * 2) + (tp_pos32<B>(i >> 4, k) << 5) + ((i & 15) << 1);
+            const uint32_t at = (uint32_t)(uintptr_t)lds + k * (TILE * 2) + (tp_pos32<B, TILE>(i >> 4, k) << 5) + ((i & 15) << 1);
             h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tp_lds_s16x4*>(at));
         }
         const u32x2 lo = __builtin_bit_cast(u32x2, h[0]), hi = __builtin_bit_cast(u32x2, h[1]);
         v[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
     } else {
-        static_assert(F == 4, "f32: 64 own indices per wave");
+        // 16 F own indices per wave: lane li holds the F indices F li ... of one k, tile q the q-th of them
         if (f != 0) return;
-        u32x4 t[4];
+        float t[4][F];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) t[s] = lds_read_b128(lds, (kk * 16 + 4 * lg + s) * (TILE * 4) + (w * 64 + 4 * li) * 4);
+        for (int s = 0; s < 4; ++s) __builtin_memcpy(t[s], __builtin_assume_aligned(lds + (kk * 16 + 4 * lg + s) * (TILE * 4) + (w * 16 * F + F * li) * 4, 4 * F), 4 * F);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = u32x4{t[0][q], t[1][q], t[2][q], t[3][q]};
+        for (int q = 0; q < F; ++q) v[q] = u32x4{__float_as_uint(t[0][q]), __float_as_uint(t[1][q]), __float_as_uint(t[2][q]), __float_as_uint(t[3][q])};
     }
 }
 
 // B side index of value j (0..7) of run h of a lane: base(h) + j, held by tile f, accumulator q
-template <typename T, bool BMN> struct TpRun {
+template <typename T, bool BMN, int FN> struct TpRun {
     static constexpr bool R4 = BMN && sizeof(T) == 4;
-    static __device__ __forceinline__ int base(int h, int lg) { return R4 ? 16 * lg + 8 * h : 32 * h + 8 * lg; }
-    static constexpr int f(int h, int j) { return R4 ? (j & 3) : 2 * h + (j >> 2); }
-    static constexpr int q(int h, int j) { return R4 ? 2 * h + (j >> 2) : (j & 3); }
+    static __device__ __forceinline__ int base(int h, int lg) { return R4 ? 4 * FN * lg + 8 * h : 32 * h + 8 * lg; }
+    static constexpr int f(int h, int j) { return R4 ? (8 * h + j) % FN : 2 * h + (j >> 2); }
+    static constexpr int q(int h, int j) { return R4 ? (8 * h + j) / FN : (j & 3); }
 };
 }   // namespace
 
-template <typename T, bool AMN, bool BMN, int EPI, bool AL, int F>
-__global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, const TpPlan pl) {
-    constexpr int CK = Tr<T>::CK, ES = sizeof(T), TILE = 32 * F, BN = EPI == TG_GATED ? TILE / 2 : TILE, OP = TILE * 128;
+constexpr int tp_blocks(int fm, int fn) { return fm == 4 ? 2 : (fn == 4 ? 3 : 4); }          // per CU
+
+template <typename T, bool AMN, bool BMN, int EPI, bool AL, int FM, int FN>
+__global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(const TgArgs a, const TpPlan pl) {
+    constexpr int CK = Tr<T>::CK, ES = sizeof(T), TM = 32 * FM, TN = 32 * FN, BN = EPI == TG_GATED ? TN / 2 : TN, OPA = TM * 128, STAGE = OPA + TN * 128;
+    static_assert(FM <= FN, "");
     extern __shared__ __attribute__((aligned(1024))) char smem[];          // 2 x [A | B]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int li = lane & 15, lg = lane >> 4;
@@ -152,15 +158,15 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         const int band = t / (4 * pl.tn), in = t - band * 4 * pl.tn;
         const int h = pl.tm - band * 4 < 4 ? pl.tm - band * 4 : 4;
         const int c = in / h;
-        w.m0 = (long long)(band * 4 + in - c * h) * TILE;
+        w.m0 = (long long)(band * 4 + in - c * h) * TM;
         w.n0 = (long long)c * BN;
         return w;
     };
     auto steps_of = [&](int sp) __attribute__((always_inline)) { return all_steps - sp * pl.sps < pl.sps ? all_steps - sp * pl.sps : pl.sps; };
 
     // ---- load cursor: the step that goes into the staging registers next ----
-    TpStage<T, AMN, false, EPI, AL, F> ga(a.a.ld);
-    TpStage<T, BMN, true, EPI, AL, F> gb(a.b.ld);
+    TpStage<T, AMN, false, EPI, AL, FM> ga(a.a.ld);
+    TpStage<T, BMN, true, EPI, AL, FN> gb(a.b.ld);
     TpStep na, nb;
     int lit = first, lrem = 0;
     const long long step_a = AMN ? CK * ES * a.a.ld : CK * ES, step_b = BMN ? CK * ES * a.b.ld : CK * ES;
@@ -194,11 +200,11 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         }
     };
 
-    f32x4 acc[F][F];
+    f32x4 acc[FN][FM];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int f = 0; f < FN; ++f)
 #pragma unroll
-        for (int p = 0; p < F; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < FM; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     auto barrier = [&]() __attribute__((always_inline)) {     // this wave's LDS traffic is done, then everyone's is; loads from global memory stay in flight
         __builtin_amdgcn_sched_barrier(0);
@@ -206,101 +212,94 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         __builtin_amdgcn_sched_barrier(0);
     };
     load_tile(false);
+    // chunk f of both operands (FM <= FN)
+    auto load = [&](int f) __attribute__((always_inline)) {
+        if (f < FM) ga.load(na, f);
+        gb.load(nb, f);
+    };
+    auto put = [&](char* st, int f) __attribute__((always_inline)) {
+        if (f < FM) ga.put(st, f);
+        gb.put(st + OPA, f);
+    };
+    u32x4 a0[FM], b0[FN], a1[FM], b1[FN];
+    // fragments 2 f, 2 f + 1 of half kk
+    auto frags = [&](u32x4 (&av)[FM], u32x4 (&bv)[FN], const char* st, int kk, int f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-        ga.load(na, j);
-        gb.load(nb, j);
-    }
+        for (int g = 2 * f; g < 2 * f + 2; ++g) {
+            if (g < FM) tp_frag<T, AMN, false, FM>(av, st, wm, kk, g);
+            if (g < FN) tp_frag<T, BMN, true, FN>(bv, st + OPA, wn, kk, g);
+        }
+    };
+#pragma unroll
+    for (int f = 0; f < FN; ++f) load(f);
     advance();
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-        ga.put(smem, j);
-        gb.put(smem + OP, j);
-        ga.load(na, j);
-        gb.load(nb, j);
+    for (int f = 0; f < FN; ++f) {
+        put(smem, f);
+        load(f);
     }
     advance();
     barrier();
-    u32x4 a0[F], b0[F], a1[F], b1[F];
 #pragma unroll
-    for (int f = 0; f < F; ++f) {
-        tp_frag<T, AMN, false, F>(a0, smem, wm, 0, f);
-        tp_frag<T, BMN, true, F>(b0, smem + OP, wn, 0, f);
-    }
+    for (int f = 0; f < FN; ++f) frags(a0, b0, smem, 0, f);
 
     int cit = first, buf = 0;
     TpItem ct = tile_of(cit);
     int crem = steps_of(ct.sp);
     while (true) {
-        char* const cur = smem + buf * 2 * OP;
-        char* const nxt = smem + (buf ^ 1) * 2 * OP;
+        char* const cur = smem + buf * STAGE;
+        char* const nxt = smem + (buf ^ 1) * STAGE;
         // (sched_barrier: the scheduler interleaves inside a row of MFMAs but does not pull a whole step's loads together, which would not fit the registers)
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            if (2 * f < F) {
+        for (int f = 0; f < FN; ++f) {
+            frags(a1, b1, cur, 1, f);
+            put(nxt, f);
+            load(f);
 #pragma unroll
-                for (int g = 2 * f; g < 2 * f + 2; ++g) {
-                    tp_frag<T, AMN, false, F>(a1, cur, wm, 1, g);
-                    tp_frag<T, BMN, true, F>(b1, cur + OP, wn, 1, g);
-                }
-            }
-            ga.put(nxt, f);
-            gb.put(nxt + OP, f);
-            ga.load(na, f);
-            gb.load(nb, f);
-#pragma unroll
-            for (int p = 0; p < F; ++p) mma_b128<T>(acc[f][p], b0[f], a0[p]);
+            for (int p = 0; p < FM; ++p) mma_b128<T>(acc[f][p], b0[f], a0[p]);
             __builtin_amdgcn_sched_barrier(0);
         }
         advance();
         barrier();
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            if (2 * f < F) {
+        for (int f = 0; f < FN; ++f) {
+            frags(a0, b0, nxt, 0, f);
 #pragma unroll
-                for (int g = 2 * f; g < 2 * f + 2; ++g) {
-                    tp_frag<T, AMN, false, F>(a0, nxt, wm, 0, g);
-                    tp_frag<T, BMN, true, F>(b0, nxt + OP, wn, 0, g);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < F; ++p) mma_b128<T>(acc[f][p], b1[f], a1[p]);
+            for (int p = 0; p < FM; ++p) mma_b128<T>(acc[f][p], b1[f], a1[p]);
             __builtin_amdgcn_sched_barrier(0);
         }
         buf ^= 1;
         if (--crem > 0) continue;
 
         // ---- the tile is complete ----
-        using Run = TpRun<T, BMN>;
+        using Run = TpRun<T, BMN, FN>;
         if constexpr (EPI == TG_GATED) {
-            static_assert(!Run::R4, "gated: k-contiguous weights only");
+            // MFMA tiles 0, 1 hold 8 gate columns of a lane, 2, 3 the same columns of up
+            static_assert(!Run::R4 && FN == 4, "gated: k-contiguous weights, 64 B rows per wave");
+            const TgGatedRow<T> row(a, ct.n0 + wn * 32 + 8 * lg);
+            if (row.nv > 0) {
 #pragma unroll
-            for (int b = 0; b < F / 4; ++b) {                  // MFMA tiles 4 b, 4 b + 1 hold 8 gate columns of a lane, 4 b + 2, 4 b + 3 the same columns of up
-                const TgGatedRow<T> row(a, ct.n0 + wn * 8 * F + 32 * b + 8 * lg);
-                if (row.nv > 0) {
+                for (int p = 0; p < FM; ++p) {
+                    const long long m = ct.m0 + wm * 16 * FM + 16 * p + li;
+                    float g[8], u[8];
 #pragma unroll
-                    for (int p = 0; p < F; ++p) {
-                        const long long m = ct.m0 + wm * 16 * F + 16 * p + li;
-                        float g[8], u[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            g[j] = acc[4 * b + (j >> 2)][p][j & 3];
-                            u[j] = acc[4 * b + 2 + (j >> 2)][p][j & 3];
-                        }
-                        if (m < a.M) row(m, g, u);
+                    for (int j = 0; j < 8; ++j) {
+                        g[j] = acc[j >> 2][p][j & 3];
+                        u[j] = acc[2 + (j >> 2)][p][j & 3];
                     }
+                    if (m < a.M) row(m, g, u);
                 }
             }
         } else {
 #pragma unroll
-            for (int h = 0; h < F / 2; ++h) {
-                const long long n = ct.n0 + wn * 16 * F + Run::base(h, lg);
+            for (int h = 0; h < FN / 2; ++h) {
+                const long long n = ct.n0 + wn * 16 * FN + Run::base(h, lg);
                 const TgLinearRow<T> row(a, tg_out(a, ct.bt), n, EPI == TG_LINEAR);
                 float* const sl = pl.slab + (long long)(ct.bt * pl.splits + ct.sp) * a.M * a.N + n;
                 if (row.nv > 0) {
 #pragma unroll
-                    for (int p = 0; p < F; ++p) {
-                        const long long m = ct.m0 + wm * 16 * F + ((AMN && ES == 4) ? 4 * li + p : 16 * p + li);
+                    for (int p = 0; p < FM; ++p) {
+                        const long long m = ct.m0 + wm * 16 * FM + ((AMN && ES == 4) ? FM * li + p : 16 * p + li);
                         float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = acc[Run::f(h, j)][p][Run::q(h, j)];
@@ -316,9 +315,9 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
         cit += gridDim.x;
         if (cit >= pl.items) return;
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+        for (int f = 0; f < FN; ++f)
 #pragma unroll
-            for (int p = 0; p < F; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int p = 0; p < FM; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
         ct = tile_of(cit);
         crem = steps_of(ct.sp);
     }
@@ -326,12 +325,10 @@ __global__ __launch_bounds__(256, 2) void tok_product_kernel(const TgArgs a, con
 
 namespace {
 template <typename T, bool AMN, bool BMN, int EPI, bool AL, int F> int tp_go(const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
-    constexpr size_t LDS = 2 * 2 * 32 * F * 128;
-    static std::atomic<unsigned long long> attr_done{0};
-    if (LDS > 65536)
-        if (const int rc = mis_set_dyn_lds(attr_done, reinterpret_cast<const void*>(&tok_product_kernel<T, AMN, BMN, EPI, AL, F>), LDS, "token product")) return rc;
-    constexpr int hold = 512;                                 // blocks that the chip holds at once
-    hipLaunchKernelGGL((tok_product_kernel<T, AMN, BMN, EPI, AL, F>), dim3((unsigned)(pl.items < hold ? pl.items : hold)), dim3(256), LDS, stream, a, pl);
+    constexpr int FM = F, FN = EPI == TG_GATED ? 4 : F;
+    constexpr size_t LDS = 2 * 32 * (FM + FN) * 128;          // at most 64 KiB
+    constexpr int hold = 256 * tp_blocks(FM, FN);             // blocks that the chip holds at once
+    hipLaunchKernelGGL((tok_product_kernel<T, AMN, BMN, EPI, AL, FM, FN>), dim3((unsigned)(pl.items < hold ? pl.items : hold)), dim3(256), LDS, stream, a, pl);
     MIS_LAUNCH_CHECK("token product");
     return MIS_OK;
 }

@@ -1,4 +1,4 @@
-// float token products, 128 x 128 tiles, operands at any element address (tok_product.hpp)
+// f32 token products, 128 x 128 tiles, operands at any element address (tok_product.hpp)
 #include "tok_product.hpp"
 
 int tok_product_f32_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream) { return tp_pick<float, 4, false>(a_mn, b_mn, epi, a, pl, stream); }

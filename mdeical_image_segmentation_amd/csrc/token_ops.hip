@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
                 tok_act8<PRECISE, true>(act, v, e);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] *= e[i];
-                if (dz != nullptr) tok_stn<T>(dz + m * lddz + n, d, nv);
+                if (dz != nullptr) tok_st8<T>(dz + m * lddz + n, d);          // (a row's pitch is whole runs of 8; behind column N: zeros)
             } else if constexpr (MODE == 1) {
                 float g[8], e[8], u[8], du[8];
                 tok_ldn<float>(z + m * ldz + n, g, nv);
@@ -54,8 +54,8 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
                     d[i] = d[i] * u[i] * e[i];
                     s2[i] += du[i];
                 }
-                tok_stn<T>(dz + m * lddz + n, d, nv);
-                tok_stn<T>(dz + m * lddz + (lddz >> 1) + n, du, nv);
+                tok_st8<T>(dz + m * lddz + n, d);
+                tok_st8<T>(dz + m * lddz + (lddz >> 1) + n, du);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i] += d[i];
@@ -75,6 +75,17 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
 #pragma unroll
         for (int r = 0; r < 16; ++r) t += red[w][r][c];
         out[rb * N + col] = t;
+    }
+}
+
+// rows of `cols` values, ld apart -> the same rows at a pitch of whole runs of 8, zeros behind them
+template <typename T> __global__ __launch_bounds__(256) void tok_pack_kernel(const T* __restrict__ src, long long ld, long long rows, long long cols, T* __restrict__ dst, long long pitch) {
+    const long long per = pitch >> 3;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (long long)gridDim.x * 256) {
+        const long long r = i / per, c = (i - r * per) * 8;
+        float v[8];
+        tok_ldn<T>(src + r * ld + c, v, cols - c >= 8 ? 8 : (int)(cols - c));
+        tok_st8<T>(dst + r * pitch + c, v);
     }
 }
 
@@ -129,11 +140,8 @@ int to_dz(int dtype, const void* dy, long long lddy, const float* z, const float
     MIS_LAUNCH_CHECK("token gradient");
     return MIS_OK;
 }
-// the dz buffer's row pitch: whole 16-byte chunks, so that the products read it aligned whatever N is
-inline long long to_pitch(int dtype, long long n) {
-    const long long e = dtype == MIS_BF16 ? 8 : 4;
-    return (n + e - 1) / e * e;
-}
+// row pitch of copies and of dz: whole runs of 8, so that the products read 16-byte chunks whatever the width is
+inline long long to_pitch(long long n) { return (n + 7) / 8 * 8; }
 inline size_t es_of(int dtype) { return dtype == MIS_BF16 ? 2 : 4; }
 
 constexpr long long TO_MAX = 1ll << 40;          // elements of one tensor: keeps every byte offset and workspace size far inside 64 bits
@@ -150,15 +158,29 @@ int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
 #define TO_PTR(who, p, what) MIS_REQUIRE((p) != nullptr, MIS_EINVAL, "%s: " what " is null", who)
 
 size_t most(size_t a, size_t b) { return a > b ? a : b; }
+// Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first:
+// 1531 x 717 x 1209 bf16, both products: 110 us on the operands as they lie, see the table beside TO_PACK for the copied ones.  dz and (dg | du) lie so from the start.
+constexpr double TO_PACK = 1 << 26;          // multiply-adds of a product from which on a copy pays
+bool whole(const void* p, long long ld, long long n, size_t es) { return ((uintptr_t)p | (size_t)(ld * (long long)es)) % 16 == 0 && n % (16 / (long long)es) == 0; }
 struct LinWs {
-    size_t dz, part, slab, total;
+    bool act, pack_dy, pack_w, pack_x;
+    size_t dz, w, x, part, slab, total;
 };
 LinWs lin_ws(const MisLinearDesc* d) {
     LinWs w{};
     size_t at = 0;
-    const bool act = d->act != MIS_ACT_NONE;
+    const size_t es = es_of(d->dtype);
+    const bool large = (double)d->M * d->N * d->K >= TO_PACK, prod = d->dx != nullptr || d->dw != nullptr;
+    w.act = d->act != MIS_ACT_NONE;
+    w.pack_dy = !w.act && prod && large && !whole(d->dy, d->lddy, d->N, es);
+    w.pack_w = d->dx != nullptr && large && !whole(d->w, d->ldw, d->K, es);
+    w.pack_x = d->dw != nullptr && large && !whole(d->x, d->ldx, d->K, es);
     w.dz = at;
-    if (act && (d->dx != nullptr || d->dw != nullptr)) at += tok_align((size_t)d->M * to_pitch(d->dtype, d->N) * es_of(d->dtype));
+    if ((w.act && prod) || w.pack_dy) at += tok_align((size_t)d->M * to_pitch(d->N) * es);
+    w.w = at;
+    if (w.pack_w) at += tok_align((size_t)d->N * to_pitch(d->K) * es);
+    w.x = at;
+    if (w.pack_x) at += tok_align((size_t)d->M * to_pitch(d->K) * es);
     w.part = at;
     if (d->dbias != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->N * 4);
     w.slab = at;            // one product after the other
@@ -167,13 +189,22 @@ LinWs lin_ws(const MisLinearDesc* d) {
     return w;
 }
 struct GatWs {
-    size_t dz, pg, pu, slab, total;
+    bool pack_w, pack_x;
+    size_t dz, w, x, pg, pu, slab, total;
 };
 GatWs gat_ws(const MisGatedDesc* d) {
     GatWs w{};
     size_t at = 0;
+    const size_t es = es_of(d->dtype);
+    const bool large = (double)d->M * d->F * d->K >= TO_PACK;
+    w.pack_w = d->dx != nullptr && large && !(whole(d->wg, d->ldw, d->K, es) && whole(d->wu, d->ldw, d->K, es));
+    w.pack_x = d->dwg != nullptr && large && !whole(d->x, d->ldx, d->K, es);
     w.dz = at;
-    at += tok_align((size_t)d->M * 2 * to_pitch(d->dtype, d->F) * es_of(d->dtype));
+    at += tok_align((size_t)d->M * 2 * to_pitch(d->F) * es);
+    w.w = at;
+    if (w.pack_w) at += 2 * tok_align((size_t)d->F * to_pitch(d->K) * es);
+    w.x = at;
+    if (w.pack_x) at += tok_align((size_t)d->M * to_pitch(d->K) * es);
     w.pg = at;
     if (d->dbg != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
     w.pu = at;
@@ -182,6 +213,14 @@ GatWs gat_ws(const MisGatedDesc* d) {
     at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, d->M, d->K, d->F, 2, 1) : 0, d->dwg != nullptr ? tg_slab_bytes(d->dtype, d->F, d->K, d->M, 1, 2) : 0);
     w.total = at;
     return w;
+}
+int to_pack(int dtype, const void* src, long long ld, long long rows, long long cols, void* dst, hipStream_t stream) {
+    const long long pitch = to_pitch(cols), n = (rows * (pitch / 8) + 255) / 256;
+    const dim3 grid((unsigned)(n < 8192 ? n : 8192));
+    if (dtype == MIS_BF16) hipLaunchKernelGGL(tok_pack_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)src, ld, rows, cols, (__bf16*)dst, pitch);
+    else hipLaunchKernelGGL(tok_pack_kernel<float>, grid, dim3(256), 0, stream, (const float*)src, ld, rows, cols, (float*)dst, pitch);
+    MIS_LAUNCH_CHECK("token rows");
+    return MIS_OK;
 }
 // an empty batch has zero gradients
 __global__ void tok_zero_kernel(char* p, long long pitch, long long rows, long long bytes) {
@@ -211,8 +250,8 @@ extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
     if (d->z != nullptr) TO_LD(who, d->ldz, d->N, "z");
     TgArgs a{};
     a.ranges = a.batches = 1;
-    a.a = TgOperand{d->x, d->x, d->ldx};
-    a.b = TgOperand{d->w, d->w, d->ldw};
+    a.a = TgOperand{d->x, d->x, d->ldx, false};
+    a.b = TgOperand{d->w, d->w, d->ldw, false};
     a.M = d->M; a.N = d->N; a.K = d->K;
     a.act = d->act; a.bias = d->bias; a.res = d->res; a.ldres = d->ldres;
     a.y = a.y2 = d->y; a.ldy = d->ldy;
@@ -246,22 +285,29 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     const LinWs w = lin_ws(d);
     MIS_REQUIRE(w.total == 0 || (d->workspace != nullptr && d->workspace_bytes >= w.total), MIS_EINVAL, "%s: the workspace has %zu bytes, %zu are needed", who, d->workspace_bytes, w.total);
     char* const ws = (char*)d->workspace;
-    const void* dz = d->dy;
-    long long lddz = d->lddy;
+    TgOperand dz{d->dy, d->dy, d->lddy, false};
     float* const part = d->dbias != nullptr ? (float*)(ws + w.part) : nullptr;
-    if (act && (prod || part != nullptr)) {
-        lddz = to_pitch(d->dtype, d->N);
-        TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->z, nullptr, d->ldz, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, lddz, part, nullptr, stream));
-        dz = ws + w.dz;
-    } else if (part != nullptr) {
-        TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, nullptr, 0, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
+    if (w.act) {
+        dz = TgOperand{ws + w.dz, ws + w.dz, to_pitch(d->N), true};
+        if (prod || part != nullptr)
+            TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->z, nullptr, d->ldz, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, dz.ld, part, nullptr, stream));
+    } else {
+        if (part != nullptr) TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, nullptr, 0, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
+        if (w.pack_dy) {
+            TO_TRY(to_pack(d->dtype, d->dy, d->lddy, d->M, d->N, ws + w.dz, stream));
+            dz = TgOperand{ws + w.dz, ws + w.dz, to_pitch(d->N), true};
+        }
     }
     if (part != nullptr) TO_TRY(tok_column_sums(part, nullptr, to_nblk(d->M), d->N, d->dbias, nullptr, stream));
     if (d->dx != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
-        a.a = TgOperand{dz, dz, lddz};
-        a.b = TgOperand{d->w, d->w, d->ldw};
+        a.a = dz;
+        a.b = TgOperand{d->w, d->w, d->ldw, false};
+        if (w.pack_w) {
+            TO_TRY(to_pack(d->dtype, d->w, d->ldw, d->N, d->K, ws + w.w, stream));
+            a.b = TgOperand{ws + w.w, ws + w.w, to_pitch(d->K), true};
+        }
         a.M = d->M; a.N = d->K; a.K = d->N;
         a.y = a.y2 = d->dx; a.ldy = d->lddx;
         TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
@@ -269,8 +315,12 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     if (d->dw != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
-        a.a = TgOperand{dz, dz, lddz};
-        a.b = TgOperand{d->x, d->x, d->ldx};
+        a.a = dz;
+        a.b = TgOperand{d->x, d->x, d->ldx, false};
+        if (w.pack_x) {
+            TO_TRY(to_pack(d->dtype, d->x, d->ldx, d->M, d->K, ws + w.x, stream));
+            a.b = TgOperand{ws + w.x, ws + w.x, to_pitch(d->K), true};
+        }
         a.M = d->N; a.N = d->K; a.K = d->M;
         a.y = a.y2 = d->dw; a.ldy = d->lddw;
         TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
@@ -290,8 +340,8 @@ extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
     if (d->g != nullptr) TO_LD(who, d->ldz, d->F, "g / u");
     TgArgs a{};
     a.ranges = a.batches = 1;
-    a.a = TgOperand{d->x, d->x, d->ldx};
-    a.b = TgOperand{d->wg, d->wu, d->ldw};
+    a.a = TgOperand{d->x, d->x, d->ldx, false};
+    a.b = TgOperand{d->wg, d->wu, d->ldw, false};
     a.M = d->M; a.N = d->F; a.K = d->K;
     a.act = d->act; a.bias = d->bg; a.bias2 = d->bu;
     a.y = a.y2 = d->h; a.ldy = d->ldh;
@@ -331,7 +381,7 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     const GatWs w = gat_ws(d);
     MIS_REQUIRE(d->workspace != nullptr && d->workspace_bytes >= w.total, MIS_EINVAL, "%s: the workspace has %zu bytes, %zu are needed", who, d->workspace_bytes, w.total);
     char* const ws = (char*)d->workspace;
-    const long long F = d->F, pitch = to_pitch(d->dtype, F), lddz = 2 * pitch;
+    const long long F = d->F, pitch = to_pitch(F), lddz = 2 * pitch;
     float* const pg = d->dbg != nullptr ? (float*)(ws + w.pg) : nullptr;
     float* const pu = d->dbu != nullptr ? (float*)(ws + w.pu) : nullptr;
     void* const dz = ws + w.dz;          // [M][dg (F, padded to pitch) | du]
@@ -341,8 +391,14 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     if (d->dx != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
-        a.a = TgOperand{dz, du, lddz};
-        a.b = TgOperand{d->wg, d->wu, d->ldw};
+        a.a = TgOperand{dz, du, lddz, true};
+        a.b = TgOperand{d->wg, d->wu, d->ldw, false};
+        if (w.pack_w) {
+            char* const pu2 = ws + w.w + tok_align((size_t)F * to_pitch(d->K) * es);
+            TO_TRY(to_pack(d->dtype, d->wg, d->ldw, F, d->K, ws + w.w, stream));
+            TO_TRY(to_pack(d->dtype, d->wu, d->ldw, F, d->K, pu2, stream));
+            a.b = TgOperand{ws + w.w, pu2, to_pitch(d->K), true};
+        }
         a.M = d->M; a.N = d->K; a.K = F;
         a.ranges = 2;
         a.y = a.y2 = d->dx; a.ldy = d->lddx;
@@ -351,8 +407,12 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     if (d->dwg != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
-        a.a = TgOperand{dz, du, lddz};
-        a.b = TgOperand{d->x, d->x, d->ldx};
+        a.a = TgOperand{dz, du, lddz, true};
+        a.b = TgOperand{d->x, d->x, d->ldx, false};
+        if (w.pack_x) {
+            TO_TRY(to_pack(d->dtype, d->x, d->ldx, d->M, d->K, ws + w.x, stream));
+            a.b = TgOperand{ws + w.x, ws + w.x, to_pitch(d->K), true};
+        }
         a.M = F; a.N = d->K; a.K = d->M;
         a.y = d->dwg; a.y2 = d->dwu; a.ldy = d->lddw; a.batches = 2;
         TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));

@@ -304,13 +304,13 @@ def test_a_block_of_all_three(B, S, D, F, dtype):
 
 
 # the 256-row kernel and the parts along k at sizes that reach every edge of a tile: one tile, ragged ends in m, n and k, more tiles than CUs, k shorter than a step, two ranges of k
-@pytest.mark.parametrize("tile, splits", [(2, 0), (2, 1), (2, 3), (1, 1), (1, 5)])
-@pytest.mark.parametrize("M, K, N", [(8, 8, 8), (256, 64, 256), (264, 72, 248), (512, 1000, 384), (1000, 136, 520), (4504, 72, 4104)])
+@pytest.mark.parametrize("tile, splits", [(2, 0), (2, 1), (2, 3), (1, 1), (1, 5), (3, 1), (3, 4)])
+@pytest.mark.parametrize("M, K, N", [(8, 8, 8), (256, 64, 256), (264, 72, 248), (512, 1000, 384), (1000, 136, 520), (777, 333, 291), (4504, 72, 4104)])
 def test_products_of_every_kind(M, K, N, tile, splits, switches):
     switches("MIS_TOK_TILE", tile)
     switches("MIS_TOK_SPLITS", splits)
     g = gen(M + K)
-    for dtype in TYPES if tile == 1 and M < 4000 else TYPES[1:]:
+    for dtype in TYPES if tile != 2 and M < 4000 else TYPES[1:]:
         x, w, b, res, dy = randn(g, M, K, dtype=dtype), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N), randn(g, M, N, dtype=dtype), randn(g, M, N, dtype=dtype)
         check_all(run_linear(x, w, b, "gelu", res, dy), O.linear(x, w, b, "gelu", res, dy), f"linear {M}x{K}x{N}")
         v = randn(g, N, K, dtype=dtype, scale=K ** -0.5)
