@@ -594,7 +594,8 @@ int mis_comm_finalize(void);
 
 /* ---- token operators: the channel-mixing half of a transformer stage (norm -> gated feed-forward -> projection onto the residual stream) on a level's pixels / voxels ----
  * A token is one row of `width` consecutive values; rows lie `ld` elements apart (ld >= width, any alignment of the element type; 16-byte aligned rows are faster).  dtype is that
- * of the activations AND the weights; biases, norm parameters and their gradients are f32, and so is what a forward pass keeps for its backward pass (mean, rstd, z, g, u).
+ * of the activations AND the weights; biases, norm parameters and their gradients are f32.  What a forward product keeps for its backward pass
+ * goes to `kept`, 16-byte aligned, mis_*_kept_bytes long, in a form of the library's own that the same dtype, act, sizes and biases (null or not) read back.
  * Rows: any number from 0 (a forward call then does nothing, a backward call writes zero parameter gradients).  Outputs must not overlap inputs.
  * Workspaces belong to the call until the stream has passed it.  Sums have a fixed order: equal calls give equal bits. */
 
@@ -624,13 +625,14 @@ typedef struct MisLinearDesc {
     const float* bias;       /* [N] or NULL */
     const void* res; long long ldres;      /* or NULL */
     void* y; long long ldy;
-    float* z; long long ldz;               /* x w^T + bias, [M][N] f32: written by the forward pass when not NULL, read by the backward pass when act != MIS_ACT_NONE */
+    void* kept;              /* written by the forward pass when not NULL, read by the backward pass; nothing is kept (0 bytes) when act is MIS_ACT_NONE */
     const void* dy; long long lddy;        /* backward pass: in; the gradient of res is dy itself */
     void* dx; long long lddx;              /* out, each NULL: not wanted */
     void* dw; long long lddw;
     float* dbias;
     void* workspace; size_t workspace_bytes;
 } MisLinearDesc;
+size_t mis_linear_kept_bytes(const MisLinearDesc* d);
 int mis_linear_fwd(const MisLinearDesc* d, void* stream);
 /* (of the descriptor as it will be passed: pointers and strides decide whether operands are copied to aligned rows) */
 size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d);
@@ -645,13 +647,14 @@ typedef struct MisGatedDesc {
     const void* wg; const void* wu; long long ldw;
     const float* bg; const float* bu;      /* [F] or NULL */
     void* h; long long ldh;
-    float* g; float* u; long long ldz;     /* the two pre-activations [M][F] f32: written by the forward pass when not NULL, read by the backward pass */
+    void* kept;              /* written by the forward pass when not NULL, read by the backward pass */
     const void* dh; long long lddh;
     void* dx; long long lddx;
     void* dwg; void* dwu; long long lddw;  /* together or neither */
     float* dbg; float* dbu;
     void* workspace; size_t workspace_bytes;
 } MisGatedDesc;
+size_t mis_gated_ffn_kept_bytes(const MisGatedDesc* d);
 int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream);
 size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d);
 int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream);

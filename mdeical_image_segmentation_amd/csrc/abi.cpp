@@ -55,13 +55,13 @@ const AbiField pack2_fields[] = {
 const AbiField linear_fields[] = {
     F(MisLinearDesc, dtype), F(MisLinearDesc, act), F(MisLinearDesc, M), F(MisLinearDesc, N), F(MisLinearDesc, K), F(MisLinearDesc, x), F(MisLinearDesc, ldx),
     F(MisLinearDesc, w), F(MisLinearDesc, ldw), F(MisLinearDesc, bias), F(MisLinearDesc, res), F(MisLinearDesc, ldres), F(MisLinearDesc, y), F(MisLinearDesc, ldy),
-    F(MisLinearDesc, z), F(MisLinearDesc, ldz), F(MisLinearDesc, dy), F(MisLinearDesc, lddy), F(MisLinearDesc, dx), F(MisLinearDesc, lddx), F(MisLinearDesc, dw),
+    F(MisLinearDesc, kept), F(MisLinearDesc, dy), F(MisLinearDesc, lddy), F(MisLinearDesc, dx), F(MisLinearDesc, lddx), F(MisLinearDesc, dw),
     F(MisLinearDesc, lddw), F(MisLinearDesc, dbias), F(MisLinearDesc, workspace), F(MisLinearDesc, workspace_bytes),
 };
 const AbiField gated_fields[] = {
     F(MisGatedDesc, dtype), F(MisGatedDesc, act), F(MisGatedDesc, M), F(MisGatedDesc, F), F(MisGatedDesc, K), F(MisGatedDesc, x), F(MisGatedDesc, ldx),
     F(MisGatedDesc, wg), F(MisGatedDesc, wu), F(MisGatedDesc, ldw), F(MisGatedDesc, bg), F(MisGatedDesc, bu), F(MisGatedDesc, h), F(MisGatedDesc, ldh),
-    F(MisGatedDesc, g), F(MisGatedDesc, u), F(MisGatedDesc, ldz), F(MisGatedDesc, dh), F(MisGatedDesc, lddh), F(MisGatedDesc, dx), F(MisGatedDesc, lddx),
+    F(MisGatedDesc, kept), F(MisGatedDesc, dh), F(MisGatedDesc, lddh), F(MisGatedDesc, dx), F(MisGatedDesc, lddx),
     F(MisGatedDesc, dwg), F(MisGatedDesc, dwu), F(MisGatedDesc, lddw), F(MisGatedDesc, dbg), F(MisGatedDesc, dbu), F(MisGatedDesc, workspace),
     F(MisGatedDesc, workspace_bytes),
 };

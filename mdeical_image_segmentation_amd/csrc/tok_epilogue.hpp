@@ -6,7 +6,7 @@
 // where batch bt is stored (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
 __device__ __forceinline__ char* tg_out(const TgArgs& a, int bt) { return (char*)a.y + (long long)bt * ((char*)a.y2 - (char*)a.y); }
 
-// y = act(v + bias) + res, v (+ bias) kept in z
+// y = act(v + bias) + res
 template <typename T, int ACT = -1> struct TgLinearRow {
     const TgArgs& a;
     long long n;            // first column of the run
@@ -22,8 +22,14 @@ template <typename T, int ACT = -1> struct TgLinearRow {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += bias[j];
         }
-        if (a.z != nullptr) tok_stn<float>(a.z + m * a.ldz + n, v, nv);
-        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
+        if (a.keep == TG_KEEP_F32) tok_stn<float>(reinterpret_cast<float*>(a.kept + m * a.kept_ld) + n, v, nv);
+        if (sizeof(T) == 2 && a.keep == TG_KEEP_RUNS) {
+            float d[8];
+            tok_act8<false, true>(ACT < 0 ? a.act : ACT, v, d);
+            *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
+        } else {
+            tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
+        }
         if (a.res != nullptr) {
             float r[8];
             tok_ldn<T>(reinterpret_cast<const T*>(a.res) + m * a.ldres + n, r, nv);
@@ -33,7 +39,7 @@ template <typename T, int ACT = -1> struct TgLinearRow {
         store(m, v);
     }
 };
-// h = act(g + bg) (u + bu), the two sums kept in z, z2
+// h = act(g + bg) (u + bu)
 template <typename T, int ACT = -1> struct TgGatedRow {
     const TgArgs& a;
     long long n;
@@ -52,11 +58,20 @@ template <typename T, int ACT = -1> struct TgGatedRow {
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[j] += bu[j];
         }
-        if (a.z != nullptr) {
-            tok_stn<float>(a.z + m * a.ldz + n, g, nv);
-            tok_stn<float>(a.z2 + m * a.ldz + n, u, nv);
+        if (a.keep == TG_KEEP_F32) {
+            tok_stn<float>(reinterpret_cast<float*>(a.kept + m * a.kept_ld) + n, g, nv);
+            tok_stn<float>(reinterpret_cast<float*>(a.kept2 + m * a.kept_ld) + n, u, nv);
         }
-        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, g, nullptr);
+        if (sizeof(T) == 2 && a.keep == TG_KEEP_RUNS) {
+            float d[8];
+            tok_act8<false, true>(ACT < 0 ? a.act : ACT, g, d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] *= u[j];
+            *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
+            *reinterpret_cast<u32x4*>(a.kept2 + m * a.kept_ld + n * 2) = tok_run_pack(g);
+        } else {
+            tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, g, nullptr);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] *= u[j];
         tok_stn<T>(reinterpret_cast<T*>(a.y) + m * a.ldy + n, g, nv);

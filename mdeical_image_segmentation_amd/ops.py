@@ -1108,34 +1108,50 @@ def _linear_desc(c, x, w, act):
     return d
 
 
-def linear_fwd(x, w, y, bias=None, act=None, res=None, z=None):
-    """y = act(x w^T + bias) + res: x (M, K), w (N, K), y (M, N), bias (N,) f32, res like y; z (M, N) f32 receives x w^T + bias for linear_bwd (mis_linear_fwd)"""
+def _kept(c, d, kept, nbytes):
+    """pointer of the buffer that carries a forward pass's values to its backward pass"""
+    if kept.device != c.device or kept.dtype != torch.uint8 or not kept.is_contiguous() or kept.numel() < nbytes:
+        raise MisError(f"{c.who}: kept must be a contiguous uint8 tensor of {nbytes} bytes on {c.device}, got {tuple(kept.shape)} {kept.dtype} on {kept.device}")
+    return kept.data_ptr()
+
+
+def linear_kept_bytes(x, w, bias=None, act=None):
+    """size of the buffer `kept` of linear_fwd / linear_bwd (0: nothing is kept)"""
+    d = _linear_desc(_TokenCall("linear_kept_bytes", x), x, w, act)
+    d.bias = None if bias is None else bias.data_ptr()
+    return load().mis_linear_kept_bytes(C.byref(d))
+
+
+def linear_fwd(x, w, y, bias=None, act=None, res=None, kept=None):
+    """y = act(x w^T + bias) + res: x (M, K), w (N, K), y (M, N), bias (N,) f32, res like y; kept: uint8 buffer of linear_kept_bytes for linear_bwd (mis_linear_fwd)"""
     c = _TokenCall("linear_fwd", x)
     d = _linear_desc(c, x, w, act)
     d.bias = c.vec(bias, "bias", d.N)
     d.y, d.ldy = c.mat(y, "y", d.M, d.N)
     if res is not None:
         d.res, d.ldres = c.mat(res, "res", d.M, d.N)
-    if z is not None:
-        d.z, d.ldz = c.mat(z, "z", d.M, d.N, torch.float32)
-    c.run(load().mis_linear_fwd, C.byref(d))
+    lib = load()
+    if kept is not None:
+        d.kept = _kept(c, d, kept, lib.mis_linear_kept_bytes(C.byref(d)))
+    c.run(lib.mis_linear_fwd, C.byref(d))
 
 
-def linear_bwd(dy, x, w, act=None, z=None, dx=None, dw=None, dbias=None):
-    """the wanted ones of dx (M, K), dw (N, K), dbias (N,) f32 from dy (M, N) and, with an activation, the forward pass's z (mis_linear_bwd); written, not accumulated"""
+def linear_bwd(dy, x, w, bias=None, act=None, kept=None, dx=None, dw=None, dbias=None):
+    """the wanted ones of dx (M, K), dw (N, K), dbias (N,) f32 from dy (M, N), the forward pass's bias and, with an activation, its `kept` (mis_linear_bwd); written, not accumulated"""
     c = _TokenCall("linear_bwd", x)
     d = _linear_desc(c, x, w, act)
+    d.bias = c.vec(bias, "bias", d.N)
     d.dy, d.lddy = c.mat(dy, "dy", d.M, d.N)
-    if d.act and z is None:
-        raise MisError("linear_bwd: with an activation the forward pass has to keep z")
-    if z is not None:
-        d.z, d.ldz = c.mat(z, "z", d.M, d.N, torch.float32)
+    lib = load()
+    if d.act and kept is None:
+        raise MisError("linear_bwd: with an activation the forward pass has to keep its values")
+    if kept is not None:
+        d.kept = _kept(c, d, kept, lib.mis_linear_kept_bytes(C.byref(d)))
     if dx is not None:
         d.dx, d.lddx = c.mat(dx, "dx", d.M, d.K)
     if dw is not None:
         d.dw, d.lddw = c.mat(dw, "dw", d.N, d.K)
     d.dbias = c.vec(dbias, "dbias", d.N)
-    lib = load()
     ws = c.scratch(lib.mis_linear_bwd_workspace_bytes(C.byref(d)))
     if ws is not None:
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -1156,32 +1172,33 @@ def _gated_desc(c, x, wg, wu, act):
     return d
 
 
-def gated_ffn_fwd(x, wg, wu, h, bg=None, bu=None, act="silu", g=None, u=None):
-    """h = act(x wg^T + bg) * (x wu^T + bu): x (M, K), wg / wu (F, K), h (M, F), bg / bu (F,) f32; g, u (M, F) f32 receive the two pre-activations for gated_ffn_bwd
-    (mis_gated_ffn_fwd)"""
+def gated_ffn_kept_bytes(x, wg, wu, bg=None, bu=None):
+    """size of the buffer `kept` of gated_ffn_fwd / gated_ffn_bwd"""
+    d = _gated_desc(_TokenCall("gated_ffn_kept_bytes", x), x, wg, wu, None)
+    d.bg, d.bu = (None if b is None else b.data_ptr() for b in (bg, bu))
+    return load().mis_gated_ffn_kept_bytes(C.byref(d))
+
+
+def gated_ffn_fwd(x, wg, wu, h, bg=None, bu=None, act="silu", kept=None):
+    """h = act(x wg^T + bg) * (x wu^T + bu): x (M, K), wg / wu (F, K), h (M, F), bg / bu (F,) f32; kept: uint8 buffer of gated_ffn_kept_bytes for gated_ffn_bwd (mis_gated_ffn_fwd)"""
     c = _TokenCall("gated_ffn_fwd", x)
     d = _gated_desc(c, x, wg, wu, act)
     d.bg, d.bu = c.vec(bg, "bg", d.F), c.vec(bu, "bu", d.F)
     d.h, d.ldh = c.mat(h, "h", d.M, d.F)
-    if (g is None) != (u is None):
-        raise MisError("gated_ffn_fwd: g and u are kept together")
-    if g is not None:
-        d.g, d.ldz = c.mat(g, "g", d.M, d.F, torch.float32)
-        d.u, ldu = c.mat(u, "u", d.M, d.F, torch.float32)
-        if ldu != d.ldz:
-            raise MisError("gated_ffn_fwd: g and u must have the same row stride")
-    c.run(load().mis_gated_ffn_fwd, C.byref(d))
+    lib = load()
+    if kept is not None:
+        d.kept = _kept(c, d, kept, lib.mis_gated_ffn_kept_bytes(C.byref(d)))
+    c.run(lib.mis_gated_ffn_fwd, C.byref(d))
 
 
-def gated_ffn_bwd(dh, x, wg, wu, g, u, act="silu", dx=None, dwg=None, dwu=None, dbg=None, dbu=None):
-    """the wanted ones of dx (M, K), dwg / dwu (F, K; together), dbg, dbu (F,) f32 from dh (M, F) and the forward pass's g, u (mis_gated_ffn_bwd); written, not accumulated"""
+def gated_ffn_bwd(dh, x, wg, wu, kept, bg=None, bu=None, act="silu", dx=None, dwg=None, dwu=None, dbg=None, dbu=None):
+    """the wanted ones of dx (M, K), dwg / dwu (F, K; together), dbg, dbu (F,) f32 from dh (M, F) and the forward pass's biases and `kept` (mis_gated_ffn_bwd); written, not accumulated"""
     c = _TokenCall("gated_ffn_bwd", x)
     d = _gated_desc(c, x, wg, wu, act)
+    d.bg, d.bu = c.vec(bg, "bg", d.F), c.vec(bu, "bu", d.F)
     d.dh, d.lddh = c.mat(dh, "dh", d.M, d.F)
-    d.g, d.ldz = c.mat(g, "g", d.M, d.F, torch.float32)
-    d.u, ldu = c.mat(u, "u", d.M, d.F, torch.float32)
-    if ldu != d.ldz:
-        raise MisError("gated_ffn_bwd: g and u must have the same row stride")
+    lib = load()
+    d.kept = _kept(c, d, kept, lib.mis_gated_ffn_kept_bytes(C.byref(d)))
     if dx is not None:
         d.dx, d.lddx = c.mat(dx, "dx", d.M, d.K)
     if (dwg is None) != (dwu is None):
@@ -1192,7 +1209,6 @@ def gated_ffn_bwd(dh, x, wg, wu, g, u, act="silu", dx=None, dwg=None, dwu=None, 
         if ldd != d.lddw:
             raise MisError("gated_ffn_bwd: dwg and dwu must have the same row stride")
     d.dbg, d.dbu = c.vec(dbg, "dbg", d.F), c.vec(dbu, "dbu", d.F)
-    lib = load()
     ws = c.scratch(lib.mis_gated_ffn_bwd_workspace_bytes(C.byref(d)))
     if ws is not None:
         d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()

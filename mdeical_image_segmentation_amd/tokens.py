@@ -174,17 +174,19 @@ def _linear_fwd(x, weight, bias, act, residual, keep):
         pr, ldr = r2.data_ptr(), _ld(r2)
     pb = _vec("linear", bias, "bias", N, x2)
     y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
-    z = torch.empty((M, N), dtype=_F32, device=x2.device) if keep and act else None
-    d = LinearDesc(code, act, M, N, K, x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), pb, pr, ldr or 0, y.data_ptr(), N, _ptr(z), N)
-    _call("linear", load().mis_linear_fwd, x2, C.byref(d))
-    return x2, w, y if x.dim() == 2 else y.view(shape), z
+    d = LinearDesc(code, act, M, N, K, x2.data_ptr(), _ld(x2), w.data_ptr(), _ld(w), pb, pr, ldr or 0, y.data_ptr(), N)
+    lib = load()
+    kept = _scratch(lib.mis_linear_kept_bytes(C.byref(d)), x2) if keep and act else None
+    d.kept = _ptr(kept)
+    _call("linear", lib.mis_linear_fwd, x2, C.byref(d))
+    return x2, w, y if x.dim() == 2 else y.view(shape), kept
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        x2, w, y, z = _linear_fwd(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(x2, w, z)
+        x2, w, y, kept = _linear_fwd(x, weight, bias, act, residual, True)
+        ctx.save_for_backward(x2, w, bias, kept)
         ctx.act, ctx.shape = act, x.shape
         return y
 
@@ -194,14 +196,14 @@ class _Linear(torch.autograd.Function):
         dres = dy if nr else None
         if not (nx or nw or nb):
             return None, None, None, None, dres
-        x, w, z = ctx.saved_tensors
+        x, w, bias, kept = ctx.saved_tensors
         M, K = x.shape
         N = w.shape[0]
         d2 = _rows("linear (backward)", dy, N, "dy")
         dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if nx else None
         dw = torch.empty((N, K), dtype=x.dtype, device=x.device) if nw else None
         db = torch.empty((N,), dtype=_F32, device=x.device) if nb else None
-        d = LinearDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, N, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), None, None, 0, None, 0, _ptr(z), N,
+        d = LinearDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, N, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(bias), None, 0, None, 0, _ptr(kept),
                        d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dw), K, _ptr(db))
         lib = load()
         ws = _scratch(lib.mis_linear_bwd_workspace_bytes(C.byref(d)), x)
@@ -233,24 +235,25 @@ def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, keep):
     M = x2.shape[0]
     pg, pu = _vec("gated_ffn", b_gate, "b_gate", F, x2), _vec("gated_ffn", b_up, "b_up", F, x2)
     h = torch.empty((M, F), dtype=x2.dtype, device=x2.device)
-    z = torch.empty((2, M, F), dtype=_F32, device=x2.device) if keep else None
-    pz = z.data_ptr() if keep else None
-    d = GatedDesc(code, act, M, F, K, x2.data_ptr(), _ld(x2), wg.data_ptr(), wu.data_ptr(), _ld(wg), pg, pu, h.data_ptr(), F, pz, pz + 4 * M * F if keep else None, F)
-    _call("gated_ffn", load().mis_gated_ffn_fwd, x2, C.byref(d))
-    return x2, wg, wu, h if x.dim() == 2 else h.view(x.shape[:-1] + (F,)), z
+    d = GatedDesc(code, act, M, F, K, x2.data_ptr(), _ld(x2), wg.data_ptr(), wu.data_ptr(), _ld(wg), pg, pu, h.data_ptr(), F)
+    lib = load()
+    kept = _scratch(lib.mis_gated_ffn_kept_bytes(C.byref(d)), x2) if keep else None
+    d.kept = _ptr(kept)
+    _call("gated_ffn", lib.mis_gated_ffn_fwd, x2, C.byref(d))
+    return x2, wg, wu, h if x.dim() == 2 else h.view(x.shape[:-1] + (F,)), kept
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        x2, wg, wu, h, z = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, True)
-        ctx.save_for_backward(x2, wg, wu, z)
+        x2, wg, wu, h, kept = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, True)
+        ctx.save_for_backward(x2, wg, wu, b_gate, b_up, kept)
         ctx.act, ctx.shape = act, x.shape
         return h
 
     @_once
     def backward(ctx, dh):
-        x, wg, wu, z = ctx.saved_tensors
+        x, wg, wu, bg, bu, kept = ctx.saved_tensors
         nx, ng, nu, nbg, nbu, _ = ctx.needs_input_grad
         M, K = x.shape
         F = wg.shape[0]
@@ -259,8 +262,7 @@ class _GatedFFN(torch.autograd.Function):
         dwg, dwu = (torch.empty((F, K), dtype=x.dtype, device=x.device), torch.empty((F, K), dtype=x.dtype, device=x.device)) if ng or nu else (None, None)
         dbg = torch.empty((F,), dtype=_F32, device=x.device) if nbg else None
         dbu = torch.empty((F,), dtype=_F32, device=x.device) if nbu else None
-        pz = z.data_ptr()
-        d = GatedDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, F, K, x.data_ptr(), _ld(x), wg.data_ptr(), wu.data_ptr(), _ld(wg), None, None, None, 0, pz, pz + 4 * M * F, F,
+        d = GatedDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, F, K, x.data_ptr(), _ld(x), wg.data_ptr(), wu.data_ptr(), _ld(wg), _ptr(bg), _ptr(bu), None, 0, _ptr(kept),
                       d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dwg), _ptr(dwu), K, _ptr(dbg), _ptr(dbu))
         lib = load()
         ws = _scratch(lib.mis_gated_ffn_bwd_workspace_bytes(C.byref(d)), x)

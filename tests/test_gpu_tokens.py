@@ -148,11 +148,13 @@ def test_linear_strides(M, K, N, dtype):
     check_all(run_linear(x, w.t().contiguous().t(), b, "gelu", res.t().contiguous().t(), dy), want, "linear transposed views")
     # outputs into slices: nothing beside them is written
     y, dx, dw = (torch.full(s, 7.0, dtype=dtype, device="cuda") for s in ((M + 1, N + 4), (M + 1, K + 4), (N + 1, K + 4)))
-    z, db = torch.full((M + 1, N + 3), 7.0, device="cuda"), torch.empty(N, device="cuda")
-    ops.linear_fwd(odd(x), w, y[:M, 1:N + 1], b, "gelu", res, z[:M, 2:N + 2])
-    ops.linear_bwd(odd(dy), odd(x), w, "gelu", z[:M, 2:N + 2], dx[:M, 3:K + 3], dw[:N, 1:K + 1], db)
+    n = ops.linear_kept_bytes(x, w, b, "gelu")
+    kept, db = torch.full((n + 64,), 7, dtype=torch.uint8, device="cuda"), torch.empty(N, device="cuda")
+    ops.linear_fwd(odd(x), w, y[:M, 1:N + 1], b, "gelu", res, kept)
+    assert (kept[n:] == 7).all()
+    ops.linear_bwd(odd(dy), odd(x), w, b, "gelu", kept, dx[:M, 3:K + 3], dw[:N, 1:K + 1], db)
     check_all({"y": y[:M, 1:N + 1], "dx": dx[:M, 3:K + 3], "dw": dw[:N, 1:K + 1], "db": db}, want, "linear into slices")
-    for t, r, c0, c1 in ((y, M, 1, N + 1), (dx, M, 3, K + 3), (dw, N, 1, K + 1), (z, M, 2, N + 2)):
+    for t, r, c0, c1 in ((y, M, 1, N + 1), (dx, M, 3, K + 3), (dw, N, 1, K + 1)):
         assert (t[r] == 7).all() and (t[:, :c0] == 7).all() and (t[:, c1:] == 7).all()
 
 
@@ -209,6 +211,26 @@ def test_gated_ffn_strides_and_packed_weights(M, K, F, dtype):
         check_all(run_gated(x, both[:F], both[F:], None, None, act, dy), want, "gated, halves of one weight")
 
 
+@pytest.mark.parametrize("scale", [1e-30, 1e-4, 1.0, 1e4, 1e30])
+def test_what_is_kept_holds_any_scale_and_one_bad_value_spoils_only_its_own_gradient(scale):
+    # bf16 without biases keeps 16-bit runs with one exponent: gradients at any scale of the values, and next to an infinity
+    g = gen(31)
+    x, wg, wu, dy = randn(g, 70, 64, dtype=torch.bfloat16), randn(g, 50, 64, dtype=torch.bfloat16, scale=0.1), randn(g, 50, 64, dtype=torch.bfloat16, scale=0.1 * scale), \
+        randn(g, 70, 50, dtype=torch.bfloat16)
+    want = O.gated(x, wg, wu, None, None, "silu", dy)
+    got = run_gated(x, wg, wu, None, None, "silu", dy)
+    check_all(got, want, "gated")
+    bad = wu.clone()
+    bad[3, 0] = float("inf")
+    got2 = run_gated(x, wg, bad, None, None, "silu", dy)
+    rows = [i for i in range(50) if i != 3]
+    # the seven neighbours keep 7 bits of their factors: one more rounding of 2^-8 in each term of dwg
+    dg = (dy.double().abs() * (O.act("silu", x.double() @ wg.double().t())[1] * (x.double() @ wu.double().t())).abs())
+    value, bound = want["dwg"]
+    O.check(got2["dwg"][rows], (value[rows], (bound + 2.0 ** -7 * dg.t() @ x.double().abs())[rows]), "dwg beside an infinity")
+    assert not torch.isfinite(got2["dwg"][3]).any()
+
+
 def test_gated_ffn_one_weight_twice():
     g = gen(9)
     x, w, dy = randn(g, 30, 48), randn(g, 40, 48), randn(g, 30, 40)
@@ -253,7 +275,8 @@ def test_refusals_on_the_gpu():
                  lambda: tokens.linear(x, w, torch.zeros(5, device="cuda")), lambda: tokens.linear(x, w.cpu()), lambda: tokens.linear(x, w, torch.zeros(6)),
                  lambda: tokens.linear(x, w, residual=torch.zeros(6, device="cuda")), lambda: tokens.linear(x, w, residual=torch.zeros(4, 6, device="cuda").bfloat16()),
                  lambda: tokens.gated_ffn(x, w, w[:5]), lambda: tokens.layer_norm(x, torch.ones(7, device="cuda")), lambda: tokens.layer_norm(x.double()),
-                 lambda: ops.linear_fwd(x, w, torch.empty(6, 4, device="cuda").t()), lambda: ops.linear_bwd(torch.ones(4, 6, device="cuda"), x, w, "gelu"),
+                 lambda: ops.linear_fwd(x, w, torch.empty(6, 4, device="cuda").t()), lambda: ops.linear_bwd(torch.ones(4, 6, device="cuda"), x, w, None, "gelu"),
+                 lambda: ops.linear_fwd(x, w, torch.empty(4, 6, device="cuda"), None, "gelu", None, torch.empty(8, dtype=torch.uint8, device="cuda")),
                  lambda: ops.linear_fwd(x[:1].expand(4, 8), w, torch.empty(4, 6, device="cuda"))):
         with pytest.raises(MisError):
             call()

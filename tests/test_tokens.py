@@ -28,8 +28,8 @@ def _lin(**kw):
     d = _lib.LinearDesc()
     d.dtype, d.M, d.N, d.K = _lib.MIS_F32, 4, 6, 8
     d.ldx = d.ldw = d.lddx = d.lddw = 8
-    d.ldy = d.lddy = d.ldz = d.ldres = 6
-    d.x = d.w = d.y = d.dy = d.z = d.dx = 4096          # never reached: each call below is refused before a launch
+    d.ldy = d.lddy = d.ldres = 6
+    d.x = d.w = d.y = d.dy = d.kept = d.dx = 4096          # never reached: each call below is refused before a launch
     for k, v in kw.items():
         setattr(d, k, v)
     return d
@@ -39,8 +39,8 @@ def _gat(**kw):
     d = _lib.GatedDesc()
     d.dtype, d.act, d.M, d.F, d.K = _lib.MIS_BF16, 4, 4, 6, 8
     d.ldx = d.ldw = d.lddx = d.lddw = 8
-    d.ldh = d.lddh = d.ldz = 6
-    d.x = d.wg = d.wu = d.h = d.dh = d.g = d.u = d.dx = 4096
+    d.ldh = d.lddh = 6
+    d.x = d.wg = d.wu = d.h = d.dh = d.kept = d.dx = 4096
     for k, v in kw.items():
         setattr(d, k, v)
     return d
@@ -48,7 +48,7 @@ def _gat(**kw):
 
 @pytest.mark.parametrize("kw, word", [({"dtype": 2}, b"dtype"), ({"act": 6}, b"activation"), ({"act": -1}, b"activation"), ({"M": -1}, b"rows"), ({"N": 0}, b"width"), ({"K": 0}, b"width"),
                                       ({"x": None}, b"null"), ({"w": None}, b"null"), ({"y": None}, b"null"), ({"ldx": 7}, b"stride"), ({"ldw": 7}, b"stride"), ({"ldy": 5}, b"stride"),
-                                      ({"ldz": 5}, b"stride"), ({"res": 4096, "ldres": 5}, b"stride"), ({"M": 1 << 60}, b"too many")])
+                                      ({"kept": 4100}, b"aligned"), ({"res": 4096, "ldres": 5}, b"stride"), ({"M": 1 << 60}, b"too many")])
 def test_linear_fwd_refuses(kw, word):
     lib = _lib.load()
     assert lib.mis_linear_fwd(C.byref(_lin(**kw)), None) < 0
@@ -56,7 +56,7 @@ def test_linear_fwd_refuses(kw, word):
 
 
 @pytest.mark.parametrize("kw, word", [({"dtype": 9}, b"dtype"), ({"dy": None}, b"null"), ({"lddy": 5}, b"stride"), ({"lddx": 7}, b"stride"), ({"dw": 4096, "lddw": 7}, b"stride"),
-                                      ({"dw": 4096, "x": None}, b"null"), ({"act": 2, "z": None}, b"keeps"), ({"act": 2}, b"workspace"), ({"dbias": 4096}, b"workspace"),
+                                      ({"dw": 4096, "x": None}, b"null"), ({"act": 2, "kept": None}, b"keeps"), ({"act": 2, "kept": 4104}, b"aligned"), ({"dtype": 1, "act": 2, "dbias": 4096}, b"without"), ({"act": 2}, b"workspace"), ({"dbias": 4096}, b"workspace"),
                                       ({"act": 2, "workspace": 4096, "workspace_bytes": 64}, b"workspace")])
 def test_linear_bwd_refuses(kw, word):
     lib = _lib.load()
@@ -65,14 +65,14 @@ def test_linear_bwd_refuses(kw, word):
 
 
 @pytest.mark.parametrize("kw, word", [({"dtype": 2}, b"dtype"), ({"act": 9}, b"activation"), ({"F": 0}, b"width"), ({"wu": None}, b"null"), ({"h": None}, b"null"), ({"ldh": 5}, b"stride"),
-                                      ({"u": None}, b"together"), ({"ldz": 5}, b"stride")])
+                                      ({"kept": 4104}, b"aligned")])
 def test_gated_fwd_refuses(kw, word):
     lib = _lib.load()
     assert lib.mis_gated_ffn_fwd(C.byref(_gat(**kw)), None) < 0
     assert word in lib.mis_last_error()
 
 
-@pytest.mark.parametrize("kw, word", [({"dh": None}, b"null"), ({"g": None}, b"keeps"), ({"u": None}, b"keeps"), ({"dwg": 4096}, b"together"), ({"lddh": 5}, b"stride"), ({}, b"workspace")])
+@pytest.mark.parametrize("kw, word", [({"dh": None}, b"null"), ({"kept": None}, b"keeps"), ({"kept": 4104}, b"aligned"), ({"dbg": 4096}, b"without"), ({"dwg": 4096}, b"together"), ({"lddh": 5}, b"stride"), ({}, b"workspace")])
 def test_gated_bwd_refuses(kw, word):
     lib = _lib.load()
     assert lib.mis_gated_ffn_bwd(C.byref(_gat(**kw)), None) < 0
