@@ -86,9 +86,9 @@ template <bool PRECISE, bool D> __device__ __forceinline__ void tok_act8(int act
         case MIS_ACT_SILU:
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float x = z[i], s = tok_sigmoid<PRECISE>(x);
-                if constexpr (D) d[i] = s * (1.f + x * (1.f - s));
-                z[i] = x * s;
+                const float s = tok_sigmoid<PRECISE>(z[i]);
+                z[i] *= s;
+                if constexpr (D) d[i] = fmaf(z[i], 1.f - s, s);
             }
             break;
         case MIS_ACT_SIGMOID:
@@ -119,14 +119,16 @@ __device__ __forceinline__ u32x4 tok_run_pack(const float (&v)[8]) {
         const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
         top = a > top ? a : top;
     }
-    const int E = (int)(top >> 23);
+    const bool fine = top < 0x7f800000u;
+    // (+ 0x200: a largest value that would round up to 2^14 takes the next exponent; below 2^-114 the step stays 2^-127)
+    int E = fine ? (int)((top + 0x200u) >> 23) : 255;
+    E = E < 13 ? 13 : (fine && E > 254 ? 254 : E);
     uint32_t q[8];
-    if (E < 255) {
+    if (fine) {
+        // v 2^(140 - E) + 1.5 2^23: the sum's low bits are the rounded integer in two's complement
+        const float scale = __uint_as_float((uint32_t)(267 - E) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float r = rintf(ldexpf(v[i], 140 - E));
-            q[i] = (uint32_t)(int)fminf(fmaxf(r, -16383.f), 16383.f);
-        }
+        for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fmaf(v[i], scale, 12582912.f));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -137,7 +139,10 @@ __device__ __forceinline__ u32x4 tok_run_pack(const float (&v)[8]) {
     }
     u32x4 w;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) w[d] = (q[2 * d] & 0x7fffu) | ((q[2 * d + 1] & 0x7fffu) << 15) | ((uint32_t)(E >> (2 * d)) << 30);
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t two = (q[2 * d] & 0x7fffu) | (~0x7fffu & (q[2 * d + 1] << 15));
+        w[d] = (two & 0x3fffffffu) | (0xc0000000u & ((uint32_t)E << (30 - 2 * d)));
+    }
     return w;
 }
 __device__ __forceinline__ void tok_run_unpack(const u32x4& w, float (&v)[8]) {

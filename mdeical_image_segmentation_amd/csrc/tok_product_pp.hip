@@ -475,7 +475,9 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         turn();
         barrier();
         if (--crem == 0) {
-            // ---- this wave's part of the tile is complete ----
+            // ---- the tile is complete: group 0 waits for group 1's last M, and both store at once (one after the other they would leave each SIMD to one wave's dependent VALU
+            // instructions: 32768 x 1024 x 2 x 4096 with SiLU 600 -> 536 us) ----
+            if (grp == 0) barrier();
             if constexpr (EPI == TG_GATED) {
                 const TgGatedRow<T, ACT> row(a, ct.n0 + wn * 32 + 8 * lg);
                 if (row.nv > 0) {
@@ -521,10 +523,9 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
             if (cit >= pl.items) break;
             ct = tile_of(cit);
             crem = steps_of(ct.sp);
-            __builtin_amdgcn_sched_barrier(0);
+            if (grp == 1) barrier();                          // the stagger again
         }
     }
-    if (grp == 0) __builtin_amdgcn_s_barrier();               // pairs with group 1's last barrier
 }
 
 // ---------------------------------------------------------------------------------------------------------
