@@ -360,23 +360,30 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         if (!second) lrem = steps_of(w.sp);
         place(w.m0, w.n0, w.bt, second ? pl.spr : w.sp * pl.sps);
     };
-    // A of the cursor's step is issued: its B is next, and A of the step behind it.  tick: straight-line, between the MFMAs; turn: what happens at the end of a range or a tile
-    auto tick = [&]() __attribute__((always_inline)) {
-        nb = nb1;
+    // A of the cursor's step is issued: its B is next, and A of the step behind it.  One untaken branch but at the ends of ranges and tiles and on the step behind one (when B takes over
+    // the masks that A got): a chain of taken branches here cost 390 cycles a step, 8192^3 789 us instead of 759.
+    int changed = 0;
+    auto advance = [&]() __attribute__((always_inline)) {
+        const int rare = changed | (va & ((lrem == 1 ? 1 : 0) | (krem < 128 ? 1 : 0)));
+        nb.base = nb1.base;
         vb = va;
         na.base += step_a;
         nb1.base += step_b;
         krem -= 64;
         lrem -= 1;
-    };
-    auto turn = [&]() __attribute__((always_inline)) {
-        if (va && (lrem == 0 || krem < 64)) {
-            if (lrem == 0) {
-                lit += gridDim.x;
-                va = lit < pl.items ? 1 : 0;
+        if (__builtin_expect(rare, 0)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) nb.v[j] = nb1.v[j];
+            changed = 0;
+            if (va && (lrem == 0 || krem < 64)) {
+                if (lrem == 0) {
+                    lit += gridDim.x;
+                    va = __builtin_amdgcn_readfirstlane(lit < pl.items ? 1 : 0);
+                }
+                if (lrem != 0 && krem > 0) masks();           // the last, short step of a range
+                else if (va) load_tile(lrem != 0);
+                changed = 1;
             }
-            if (lrem != 0 && krem > 0) masks();               // the last, short step of a range
-            else if (va) load_tile(lrem != 0);
         }
     };
     load_tile(false);
@@ -391,12 +398,11 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, ldsB = lds0 + PG_B0;
     uint32_t curA = lds0, curB = ldsB, dstA = lds0 + 2 * PG_OP + wave * 1024, dstB = ldsB + PG_OP + wave * 1024;
     pg_issue(pg_dma(la, na, lds0 + wave * 1024));
-    tick();
-    turn();
+    changed = 1;
+    advance();
     pg_issue(pg_dma(lb, nb, ldsB + wave * 1024));
     if (va) pg_issue(pg_dma(la, na, lds0 + PG_OP + wave * 1024));          // A of step 1
-    tick();
-    turn();                                                   // nb: B of step 1, na: A of step 2
+    advance();                                                // nb: B of step 1, na: A of step 2
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (grp == 1) __builtin_amdgcn_s_barrier();               // the stagger
@@ -463,7 +469,6 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         if (grp == 1) retire(inflight);
         barrier();
         __builtin_amdgcn_s_setprio(1);
-        tick();
         curA = curA == lds0 + 2 * PG_OP ? lds0 : curA + PG_OP;
         dstA = curA == lds0 ? lds0 + 2 * PG_OP + wave * 1024 : curA - PG_OP + wave * 1024;
         dstB = curB + wave * 1024;
@@ -471,8 +476,8 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         mma();
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
+        advance();
         if (grp == 0) retire(inflight);
-        turn();
         barrier();
         if (--crem == 0) {
             // ---- the tile is complete: group 0 waits for group 1's last M, and both store at once (one after the other they would leave each SIMD to one wave's dependent VALU
