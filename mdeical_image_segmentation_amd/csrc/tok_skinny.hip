@@ -3,7 +3,14 @@
 // The weights are read once and are all there is to read, so the kernel is a stream of them: a block owns 16 columns (gated: the same 16 of gate and of up; 32 for more than 16 rows), its
 // waves take turns along k in units of 128 bytes per row, and a weight fragment goes from global memory straight into the MFMA's row side - no LDS, no barrier - against the rows of x,
 // which come out of the L2.  The waves' partial sums meet in LDS in wave order, then the epilogue runs on runs of 8 columns.  As many waves per block as bring ~2000 of them onto the
-// chip: 8 rows, 2 x 8192 x 2048 bf16 weights (67 MB): see the table of measurements beside the rule below.
+// chip, at most 8 where a lane holds more than one tile of rows (16 leave it 128 registers, and the fragments of 64 rows spill: 8192 x 8192 bf16, 64 rows, 163 us instead of 53).
+//
+// Bound by the weights: one row of 8192 x 8192 bf16 (134 MB) 32.6 us, 4.1 TB/s; f32 57 us, 4.7 TB/s.  Up to which rows, against the 64 x 64 tiles (tok_product.hpp), us here / there:
+//      rows   bf16 2048 -> 8192   8192 -> 8192   gated 8192 -> 2 x 8192   f32 2048 -> 8192   8192 -> 8192
+//        1          7.8 / 17.8      32.6 / 60.4         39.3 / 91.5            15 / 54           57 / 206
+//       32         10.7 / 19.3      34.5 / 63.2         65.6 / 101             24 / 54           73 / 211
+//       64         15.8 / 19.3      53.1 / 64.6         92.1 / 99              40 / 55          141 / 213
+// Beyond 64 every further tile of rows would read the weights again.
 #include "tok_epilogue.hpp"
 #include "tok_product_plan.hpp"
 
@@ -26,7 +33,7 @@ template <typename T, bool AL> __device__ __forceinline__ u32x4 sk_chunk(const T
 
 // NT tiles of 16 columns (gated: gate, up), MT tiles of 16 rows, blockDim.x / 64 waves along k
 template <typename T, int NT, int MT, bool GATED, bool AL>
-__global__ __launch_bounds__(1024) void tok_skinny_kernel(const TgArgs a) {
+__global__ __launch_bounds__(MT == 1 ? 1024 : 512) void tok_skinny_kernel(const TgArgs a) {
     constexpr int EPC = Tr<T>::EPC, S = 4 * EPC;          // k of one MFMA step: 64 bytes per row
     extern __shared__ __attribute__((aligned(16))) float part[];          // [wave][NT][MT][16 m][16 n]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), W = blockDim.x >> 6;
@@ -125,7 +132,7 @@ template <typename T, int NT, int MT, bool GATED, bool AL> int sk_go(const TgArg
     const long long cols = GATED ? 16 : 16 * NT, blocks = (a.N + cols - 1) / cols, units = (a.K + 8 * Tr<T>::EPC - 1) / (8 * Tr<T>::EPC);
     MIS_REQUIRE(blocks < (1ll << 31), MIS_EUNSUPPORTED, "token product: %lld columns are more than a grid holds", a.N);
     int W = 1;
-    while (W < 16 && blocks * W < 2048 && 2 * W <= units) W *= 2;
+    while (W < (MT == 1 ? 16 : 8) && blocks * W < 2048 && 2 * W <= units) W *= 2;
     hipLaunchKernelGGL((tok_skinny_kernel<T, NT, MT, GATED, AL>), dim3((unsigned)blocks), dim3(64 * W), (size_t)W * NT * MT * 1024, stream, a);
     MIS_LAUNCH_CHECK("token product (few rows)");
     return MIS_OK;
