@@ -3,10 +3,16 @@
 //   dx = rstd (t - mean(t) - xh mean(t xh)), t = dy gamma;   dgamma = sum_rows dy xh, dbeta = sum_rows dy
 // All statistics and sums are f32; the variance is that of the centred values (no E[x^2] - mu^2 cancellation).
 //
-// About ten operations a value: bandwidth bounds both directions, so a row is read once and lives in registers (8 values x NV per lane) between the passes over it.  Rows up to 2048 wide
-// belong to one wave (no barrier at all), rows up to 8192 to the four waves of a block; wider ones are read again for each pass and stay in the caches.
-// Backward: one kernel reads x and dy once, writes dx and keeps this wave's part of dgamma and dbeta in registers over all its rows; the blocks' partial rows are then added in a
-// fixed order.
+// About ten operations a value: bandwidth bounds both directions, so a row is read once and lives in registers (runs of 8 values per lane) between the passes over it.  A row belongs to as
+// few lanes as hold it: 8 to 64 lanes of a wave up to 2048 values (no barrier at all), the four waves of a block up to 8192; wider ones are read again for each pass and stay in the caches.
+// Backward: one kernel reads x and dy once, writes dx and keeps these lanes' part of dgamma and dbeta in registers over all its rows; the blocks' partial rows are then added in a
+// fixed order.  Rows x width, us forward / backward and the rates of x + y, x + dy + dx (a large copy: 4.7 TB/s):
+//                       bf16                                     f32
+//      65536 x 96        9.0 / 15.1   2.8, 2.5 TB/s             10.5 / 18.2   4.8, 4.1 TB/s      (64 lanes a row: 22.8 / 34.4, 23.6 / 29.8)
+//      32768 x 1024     24.3 / 41.6   5.5, 4.8                  42.9 / 77.7   6.3, 5.2
+//      16384 x 2048     26.4 / 45.0   5.1, 4.5                  44.2 / 85.4   6.1, 4.7           (four waves a row: 29.2 / 57.8, 40.3 / 77.7)
+//      8192 x 4096      23.7 / 44.5   5.7, 4.5                  43.4 / 82.2   6.2, 4.9           (read again: 28.6 / 72.1, 59.6 / 141)
+//      2048 x 16384     39.7 / 80.4   3.4, 2.5                  75.9 / 141    3.5, 2.9
 #include <type_traits>
 
 #include "tok_common.hpp"
@@ -25,12 +31,15 @@ __device__ __forceinline__ float ln_block_sum(float v, float* red) {
 }   // namespace
 
 namespace {
-constexpr int LN_PART = 512;          // blocks of the backward pass = partial rows of the parameter gradients
-
-// sum over the W waves that share a row; `red` (W > 1) is reusable behind the next barrier
-template <int W> __device__ __forceinline__ float ln_row_sum(float v, float* red) {
-    v = wave_sum(v);
-    if constexpr (W == 4) {
+// sum over the L lanes that share a row (256: the block; `red` is then reusable behind the next barrier)
+template <int L> __device__ __forceinline__ float ln_row_sum(float v, float* red) {
+    if constexpr (L < 64) {
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    } else {
+        v = wave_sum(v);
+    }
+    if constexpr (L == 256) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = (red[0] + red[1]) + (red[2] + red[3]);
@@ -39,37 +48,37 @@ template <int W> __device__ __forceinline__ float ln_row_sum(float v, float* red
 }
 }   // namespace
 
-// W waves per row (1: four rows a block; 4: one), NV runs of 8 values per lane: D <= 512 W NV
-template <typename T, int W, int NV>
+// L lanes per row (8, 16, 32, 64: 256 / L rows a block; 256: one), NV runs of 8 values per lane: D <= 8 L NV
+template <typename T, int L, int NV>
 __global__ __launch_bounds__(LN_THREADS) void ln_fwd_row_kernel(const T* __restrict__ x, long long ldx, long long M, int D, float eps, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, T* __restrict__ y, long long ldy, float* __restrict__ mean,
                                                                 float* __restrict__ rstd) {
     __shared__ float red[2][4];
-    const int lane = W == 1 ? (threadIdx.x & 63) : (int)threadIdx.x;
-    const long long r = W == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long long)blockIdx.x;
-    if (r >= M) return;                                      // (W = 4: block-uniform)
+    const int lane = threadIdx.x & (L - 1);
+    const long long r = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (r >= M) return;                                      // (a row's lanes go together)
     float f[NV][8];
     float s = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * W * 64 + lane) * 8;
+        const int c = (v * L + lane) * 8;
         tok_ldn<T>(x + r * ldx + c, f[v], D - c);            // (0 past the row's end)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += f[v][i];
     }
-    const float mu = ln_row_sum<W>(s, red[0]) / D;
+    const float mu = ln_row_sum<L>(s, red[0]) / D;
     s = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            f[v][i] = (v * W * 64 + lane) * 8 + i < D ? f[v][i] - mu : 0.f;
+            f[v][i] = (v * L + lane) * 8 + i < D ? f[v][i] - mu : 0.f;
             s += f[v][i] * f[v][i];
         }
-    const float rs = 1.f / sqrtf(ln_row_sum<W>(s, red[1]) / D + eps);
+    const float rs = 1.f / sqrtf(ln_row_sum<L>(s, red[1]) / D + eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * W * 64 + lane) * 8;
+        const int c = (v * L + lane) * 8;
         if (c < D) {
             float g[8], b[8];
             if (gamma != nullptr) tok_ldn<float>(gamma + c, g, D - c);
@@ -89,32 +98,30 @@ __global__ __launch_bounds__(LN_THREADS) void ln_fwd_row_kernel(const T* __restr
     }
 }
 
-template <typename T, int W, int NV>
+template <typename T, int L, int NV>
 __global__ __launch_bounds__(LN_THREADS) void ln_bwd_row_kernel(const T* __restrict__ dy, long long lddy, const T* __restrict__ x, long long ldx, long long M, int D,
                                                                 const float* __restrict__ gamma, const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                 T* __restrict__ dx, long long lddx, float* __restrict__ pg, float* __restrict__ pb) {
     __shared__ float red[2][2][4];
-    __shared__ float acc[W == 1 ? 4 : 1][W == 1 ? 512 : 1];
-    const int lane = W == 1 ? (threadIdx.x & 63) : (int)threadIdx.x, wave = threadIdx.x >> 6;
-    const long long per = W == 1 ? 4 : 1;
+    __shared__ float acc[L == 256 ? 1 : LN_THREADS * 8];
+    const int lane = threadIdx.x & (L - 1), sub = threadIdx.x / L;
+    constexpr int per = 256 / L;
     float g[NV][8], sg[NV][8], sb[NV][8];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c = (v * W * 64 + lane) * 8;
+        const int c = (v * L + lane) * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[v][i] = 1.f, sg[v][i] = sb[v][i] = 0.f;
         if (gamma != nullptr && c < D) tok_ldn<float>(gamma + c, g[v], D - c);
     }
     int flip = 0;
-    for (long long r0 = blockIdx.x * per; r0 < M; r0 += gridDim.x * per) {
-        const long long r = r0 + (W == 1 ? wave : 0);
-        if (W == 1 && r >= M) break;                         // (this wave's last round; W = 4: block-uniform by the loop)
+    for (long long r = (long long)blockIdx.x * per + sub; r < M; r += (long long)gridDim.x * per) {          // (a row's lanes go together)
         const float mu = mean[r], rs = rstd[r];
         float f[NV][8], d[NV][8];
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * W * 64 + lane) * 8;
+            const int c = (v * L + lane) * 8;
             tok_ldn<T>(x + r * ldx + c, f[v], D - c);
             tok_ldn<T>(dy + r * lddy + c, d[v], D - c);      // (0 past the row's end: nothing is added there)
         }
@@ -131,11 +138,11 @@ __global__ __launch_bounds__(LN_THREADS) void ln_bwd_row_kernel(const T* __restr
                 s2 += d[v][i] * xh;
             }
         if (dx != nullptr) {
-            const float m1 = ln_row_sum<W>(s1, red[flip][0]) / D, m2 = ln_row_sum<W>(s2, red[flip][1]) / D;
+            const float m1 = ln_row_sum<L>(s1, red[flip][0]) / D, m2 = ln_row_sum<L>(s2, red[flip][1]) / D;
             flip ^= 1;                                       // (the next round's sums go elsewhere: two barriers lie between two uses)
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const int c = (v * W * 64 + lane) * 8;
+                const int c = (v * L + lane) * 8;
                 if (c < D) {
                     float o[8];
 #pragma unroll
@@ -145,22 +152,25 @@ __global__ __launch_bounds__(LN_THREADS) void ln_bwd_row_kernel(const T* __restr
             }
         }
     }
-    // this block's partial rows; the four waves of W = 1 are added in their order
+    // this block's partial rows; those of its 256 / L rows are added in their order
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float* const out = which == 0 ? pg : pb;
         if (out == nullptr) continue;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int c = (v * W * 64 + lane) * 8;
-            if constexpr (W == 1) {
+            const int c = (v * L + lane) * 8;
+            if constexpr (L < 256) {
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[wave][i * 64 + lane] = which == 0 ? sg[v][i] : sb[v][i];
+                for (int i = 0; i < 8; ++i) acc[(sub * 8 + i) * L + lane] = which == 0 ? sg[v][i] : sb[v][i];
                 __syncthreads();
-                for (int q = threadIdx.x; q < 512; q += LN_THREADS) {
-                    const int i = q >> 6, l = q & 63, col = (v * 64 + l) * 8 + i;
-                    if (col < D) out[(long long)blockIdx.x * D + col] = (acc[0][q] + acc[1][q]) + (acc[2][q] + acc[3][q]);
+                for (int q = threadIdx.x; q < 8 * L; q += LN_THREADS) {
+                    const int col = (v * L + q % L) * 8 + q / L;
+                    float t = acc[q];
+#pragma unroll
+                    for (int k = 1; k < per; ++k) t += acc[k * 8 * L + q];
+                    if (col < D) out[(long long)blockIdx.x * D + col] = t;
                 }
             } else if (c < D) {
                 tok_stn<float>(out + (long long)blockIdx.x * D + c, which == 0 ? sg[v] : sb[v], D - c);
@@ -298,36 +308,37 @@ inline long long ln_rows(long long M) {
     while ((M + r - 1) / r > 512) r *= 2;
     return r;
 }
-// waves per row and runs per lane that a width takes; 0: the kernels for any width
-inline int ln_waves(int D) { return D <= 2048 ? 1 : (D <= 8192 ? 4 : 0); }
-inline int ln_runs(int D) { return (D + 512 * ln_waves(D) - 1) / (512 * ln_waves(D)); }
-inline long long ln_parts(long long M, int D) {
-    const int w = ln_waves(D);
-    if (w == 0) return (M + ln_rows(M) - 1) / ln_rows(M);
-    const long long blocks = w == 1 ? (M + 3) / 4 : M;
-    return blocks < LN_PART ? blocks : LN_PART;
+// lanes per row and runs per lane that a width takes; 0: the kernels for any width
+inline int ln_lanes(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : (D <= 256 ? 32 : (D <= 2048 ? 64 : (D <= 8192 ? 256 : 0)))); }
+inline int ln_runs(int D) { return (D + 8 * ln_lanes(D) - 1) / (8 * ln_lanes(D)); }
+// Blocks of the backward pass = partial rows of the parameter gradients: 1024 where the registers let four blocks onto a CU and 16-byte loads (bf16: a lane has half of f32's bytes in
+// flight) need them, else 512.  512 / 1024 / 2048 blocks, us: bf16 8192 x 2056 49 / 34 / 43, 32768 x 1024 46 / 42 / 49, 16384 x 2048 45 / 53 / 53; f32 32768 x 1024 78 / 82 / 87,
+// 4096 x 8192 91 / 99 / 99
+constexpr int LN_PART = 512, LN_PART_LIGHT = 1024;
+inline long long ln_parts(int dtype, long long M, int D) {
+    const int n = ln_lanes(D);
+    if (n == 0) return (M + ln_rows(M) - 1) / ln_rows(M);
+    const long long blocks = (M * n + 255) / 256, most = D <= 256 || (dtype == MIS_BF16 && ln_runs(D) <= 2) ? LN_PART_LIGHT : LN_PART;
+    return blocks < most ? blocks : most;
 }
+template <int V> using ln_int = std::integral_constant<int, V>;
 template <typename T, typename F> int ln_by_width(int D, F&& f) {
-    const int w = ln_waves(D), n = ln_runs(D);
-    if (w == 1) {
-        if (n == 1) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-        if (n == 2) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
-        if (n == 3) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 3>{});
-        return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-    }
-    if (n == 2) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});          // (4 waves, 1 run: up to 2048, which one wave takes)
-    if (n == 3) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 3>{});
-    return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    const int w = ln_lanes(D), n = ln_runs(D);
+    if (w == 8) return f(ln_int<8>{}, ln_int<1>{});
+    if (w == 16) return f(ln_int<16>{}, ln_int<1>{});
+    if (w == 32) return f(ln_int<32>{}, ln_int<1>{});
+    if (w == 64) return n == 1 ? f(ln_int<64>{}, ln_int<1>{}) : n == 2 ? f(ln_int<64>{}, ln_int<2>{}) : n == 3 ? f(ln_int<64>{}, ln_int<3>{}) : f(ln_int<64>{}, ln_int<4>{});
+    return n == 2 ? f(ln_int<256>{}, ln_int<2>{}) : n == 3 ? f(ln_int<256>{}, ln_int<3>{}) : f(ln_int<256>{}, ln_int<4>{});          // (one run of a block: up to 2048, which a wave takes)
 }
 template <typename T>
 int ln_fwd(const void* x, long long ldx, long long M, int D, float eps, const float* gamma, const float* beta, void* y, long long ldy, float* mean, float* rstd, hipStream_t stream) {
-    if (ln_waves(D) == 0) {
+    if (ln_lanes(D) == 0) {
         hipLaunchKernelGGL((ln_fwd_kernel<T>), dim3((unsigned)M), dim3(LN_THREADS), 0, stream, (const T*)x, ldx, D, eps, gamma, beta, (T*)y, ldy, mean, rstd);
         return MIS_OK;
     }
     return ln_by_width<T>(D, [&](auto w, auto n) {
-        constexpr int W = decltype(w)::value, NV = decltype(n)::value;
-        hipLaunchKernelGGL((ln_fwd_row_kernel<T, W, NV>), dim3((unsigned)(W == 1 ? (M + 3) / 4 : M)), dim3(LN_THREADS), 0, stream, (const T*)x, ldx, M, D, eps, gamma, beta, (T*)y, ldy,
+        constexpr int L = decltype(w)::value, NV = decltype(n)::value;
+        hipLaunchKernelGGL((ln_fwd_row_kernel<T, L, NV>), dim3((unsigned)((M * L + 255) / 256)), dim3(LN_THREADS), 0, stream, (const T*)x, ldx, M, D, eps, gamma, beta, (T*)y, ldy,
                            mean, rstd);
         return MIS_OK;
     });
@@ -335,8 +346,8 @@ int ln_fwd(const void* x, long long ldx, long long M, int D, float eps, const fl
 template <typename T>
 int ln_bwd(const void* dy, long long lddy, const void* x, long long ldx, long long M, int D, const float* gamma, const float* mean, const float* rstd, void* dx, long long lddx, float* pg,
            float* pb, hipStream_t stream) {
-    const long long parts = ln_parts(M, D);
-    if (ln_waves(D) == 0) {
+    const long long parts = ln_parts(sizeof(T) == 2 ? MIS_BF16 : MIS_F32, M, D);
+    if (ln_lanes(D) == 0) {
         if (dx != nullptr)
             hipLaunchKernelGGL((ln_bwd_dx_kernel<T>), dim3((unsigned)M), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, D, gamma, mean, rstd, (T*)dx, lddx);
         if (pg != nullptr || pb != nullptr)
@@ -345,8 +356,8 @@ int ln_bwd(const void* dy, long long lddy, const void* x, long long ldx, long lo
         return MIS_OK;
     }
     return ln_by_width<T>(D, [&](auto w, auto n) {
-        constexpr int W = decltype(w)::value, NV = decltype(n)::value;
-        hipLaunchKernelGGL((ln_bwd_row_kernel<T, W, NV>), dim3((unsigned)parts), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, M, D, gamma, mean, rstd, (T*)dx, lddx, pg, pb);
+        constexpr int L = decltype(w)::value, NV = decltype(n)::value;
+        hipLaunchKernelGGL((ln_bwd_row_kernel<T, L, NV>), dim3((unsigned)parts), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, M, D, gamma, mean, rstd, (T*)dx, lddx, pg, pb);
         return MIS_OK;
     });
 }
@@ -374,7 +385,7 @@ extern "C" int mis_layernorm_fwd(int dtype, const void* x, long long ldx, long l
 
 extern "C" size_t mis_layernorm_bwd_workspace_bytes(int dtype, long long M, int D) {
     if (ln_check("mis_layernorm_bwd", dtype, M, D) != MIS_OK || M == 0) return 0;
-    return 2 * tok_align((size_t)ln_parts(M, D) * D * 4);
+    return 2 * tok_align((size_t)ln_parts(dtype, M, D) * D * 4);
 }
 
 extern "C" int mis_layernorm_bwd(int dtype, const void* dy, long long lddy, const void* x, long long ldx, long long M, int D, const float* gamma, const float* mean,
@@ -383,7 +394,7 @@ extern "C" int mis_layernorm_bwd(int dtype, const void* dy, long long lddy, cons
     if (const int rc = ln_check("mis_layernorm_bwd", dtype, M, D)) return rc;
     MIS_REQUIRE(M == 0 || (dy != nullptr && x != nullptr && mean != nullptr && rstd != nullptr), MIS_EINVAL, "mis_layernorm_bwd: null pointer");
     MIS_REQUIRE(lddy >= D && ldx >= D && (dx == nullptr || lddx >= D), MIS_EINVAL, "mis_layernorm_bwd: a row stride is below the width");
-    const long long parts = M > 0 ? ln_parts(M, D) : 0;
+    const long long parts = M > 0 ? ln_parts(dtype, M, D) : 0;
     const bool params = dgamma != nullptr || dbeta != nullptr;
     const size_t half = tok_align((size_t)parts * D * 4);
     MIS_REQUIRE(!params || M == 0 || (workspace != nullptr && workspace_bytes >= 2 * half), MIS_EINVAL, "mis_layernorm_bwd: the workspace has %zu bytes, %zu are needed",
