@@ -33,25 +33,35 @@ static int tg_slab_sum(int dtype, const TgArgs& a, const float* slab, int splits
 }
 
 namespace {
-// How a product is cut.  Costs in microseconds per 64-k step, all the blocks of a CU at work: one 256 x 256 tile 1.55, two 128 x 128 tiles 1.25, four 64 x 64 tiles 1.0 (8192^3 at 1.39, 0.83
-// PFLOP/s; f32 takes TG_F32 times as long); a tile's start and epilogue about three steps; a k part its slab's write and read at the copy rate.
+// How a product is cut: the cheapest of the tiles and numbers of k parts by this model.  A 64-k step of the blocks that a CU holds takes (us; blocks per CU: 1 .. what fits)
+//      bf16   256 x 256  1.2 (few CUs at work) to 1.5     128 x 128  0.8, 1.25     64 x 64  0.5, 0.7, 0.85, 1.05     gated 64 x (64 + 64)  0.65, 1.0, 1.35
+//      f32                                                128 x 128  4.1, 6.9      64 x 64  1.6, 2.4, 3.2, 4.0       gated 64 x (64 + 64)  2.4, 3.9, 5.4
+// a tile's start and epilogue as much as 3 (256: 5) steps, a cut along k 5 us and its slab's write and read, mostly in the caches, at 7 TB/s.  us, measured with each tile (* the model's choice):
+//                                       256      128       64                                          256      128       64
+//      512 x 512 x 512       x W^T       17       11     *8.1      2048 x 2048 x 2048       dz W       40      *37       42
+//      1024 x 4096 x 1024    x W^T       80       52      *34      4096 x 4096 x 1024       dz W      *34       48       82
+//      2048 x 2048 x 2048    x W^T       45      *30       39      8192 x 1024 x 4096       dz^T x    *75       96      160
+//      4096 x 4096 x 1024    x W^T       80      *53       70      8192 x 1024 x 4096       gated    *116      162      208
+//      8192 x 1024 x 4096    x W^T      *66       90      149      f32 1024 x 4096 x 1024   x W^T       -      290     *106
+//      8192 x 2048 x 8192    x W^T     *217      329      555      f32 8192 x 1024 x 4096   x W^T       -     *528      561
 struct TgCut {
     int tile;               // 256, 128 or 64 rows
     int splits;
     double us;
 };
-constexpr double TG_F32[2] = {5.6, 3.7};          // f32 against bf16: 128 x 128, 64 x 64
 TgCut tg_cut_one(int dtype, int tile, bool may_split, long long M, long long N, long long K, int ranges, int batches, bool gated) {
     const int cols = gated ? (tile == 256 ? 128 : 64) : tile;
     const long long items = ((M + tile - 1) / tile) * ((N + cols - 1) / cols) * batches, steps = ((K + 63) / 64) * ranges;
     if (const int forced = mis_sw(SW_TOK_SPLITS); may_split && forced > 0) return TgCut{tile, (int)(forced < steps ? forced : steps), 0.0};
-    const double step = (tile == 256 ? 1.55 : tile == 128 ? 1.25 : (gated ? 1.2 : 1.0)) * (dtype == MIS_BF16 ? 1.0 : TG_F32[tile == 64]);
-    const long long slots = tile == 256 ? 256 : tile == 128 ? 512 : (gated ? 768 : 1024);
+    const bool f32 = dtype == MIS_F32;
+    const int fit = tile == 256 ? 1 : tile == 128 ? 2 : gated ? 3 : 4;          // blocks that a CU holds
+    const double one = tile == 128 ? (f32 ? 1.3 : 0.35) : gated ? (f32 ? 0.9 : 0.28) : (f32 ? 0.75 : 0.32), more = tile == 128 ? (f32 ? 2.8 : 0.45) : gated ? (f32 ? 1.5 : 0.36) : (f32 ? 0.82 : 0.18);
     TgCut best{tile, 1, 1e30};
     for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || steps / s >= 4); ++s) {
-        const double rounds = (double)((items * s + slots - 1) / slots);
-        double us = rounds * ((double)((steps + s - 1) / s) + 3.0) * step;
-        if (s > 1) us += 3.0 + 8.0 * s * (double)M * (double)N * batches / 4.7e6;
+        const long long n = items * s, per = (n + 255) / 256;          // (256 CUs)
+        const double step = tile == 256 ? 1.2 + 0.3 * (n < 256 ? n / 256.0 : 1.0) : one + more * (double)(per < fit ? per : fit);
+        double us = (double)((n + 256 * fit - 1) / (256 * fit)) * ((double)((steps + s - 1) / s) + (tile == 256 ? 5.0 : 3.0)) * step;
+        if (s > 1) us += 5.0 + 8.0 * s * (double)M * (double)N * batches / 7e6;
         if (us < best.us * 0.97) best = TgCut{tile, s, us};
     }
     return best;
@@ -65,7 +75,7 @@ TgCut tg_cut(int dtype, bool aligned, bool may_split, long long M, long long N, 
     if (small.us < best.us) best = small;
     if (big_ok) {
         const TgCut big = tg_cut_one(dtype, 256, may_split, M, N, K, ranges, batches, gated);
-        if (big.us <= best.us) best = big;
+        if (big.us <= best.us * 1.03) best = big;          // (half the traffic from the L2)
     }
     return best;
 }
