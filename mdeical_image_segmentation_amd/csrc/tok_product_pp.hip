@@ -13,7 +13,6 @@
 // four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
 // LDS images and swizzles are those of tok_product.hpp with 256 rows: [row][128 B] for a k-contiguous operand, [k][512 B] for the other kind, read with the transposing ds_read_b64_tr_b16.
 // The fragment reads and their wait are one asm statement: hipcc would put a vmcnt(0), i.e. a wait for the prefetch, in front of a plain LDS read while an LDS-DMA is in flight.
-#include <stdlib.h>
 
 #include "conv_pp_common.hpp"
 #include "dispatch_cfg.hpp"

@@ -178,17 +178,24 @@ int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
     MIS_REQUIRE(dtype == MIS_F32 || dtype == MIS_BF16, MIS_EINVAL, "%s: dtype must be MIS_F32 or MIS_BF16", who);
     MIS_REQUIRE(tok_act_ok(act), MIS_EINVAL, "%s: unknown activation %d", who, act);
     MIS_REQUIRE(M >= 0 && N >= 1 && K >= 1, MIS_EINVAL, "%s: needs rows >= 0 and widths >= 1 (got %lld, %d, %d)", who, M, N, K);
-    MIS_REQUIRE(M < TO_MAX / N && M < TO_MAX / K, MIS_EUNSUPPORTED, "%s: %lld rows of %d / %d values are too many", who, M, N, K);
+    MIS_REQUIRE(M < (1ll << 31) && M < TO_MAX / N && M < TO_MAX / K, MIS_EUNSUPPORTED, "%s: %lld rows of %d / %d values are too many", who, M, N, K);
     return MIS_OK;
 }
 #define TO_LD(who, ld, n, what) MIS_REQUIRE((ld) >= (n) && (ld) < TO_MAX, MIS_EINVAL, "%s: the row stride of " what " (%lld) is below its width", who, (long long)(ld))
-// (the grid of the largest product of a call; the launchers check it too, but only after earlier launches of the call)
 #define TO_PTR(who, p, what) MIS_REQUIRE((p) != nullptr, MIS_EINVAL, "%s: " what " is null", who)
 
 size_t most(size_t a, size_t b) { return a > b ? a : b; }
-// Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first:
-// 1531 x 717 x 1209 bf16, both products: 110 us on the operands as they lie, see the table beside TO_PACK for the copied ones.  dz and (dg | du) lie so from the start.
-constexpr double TO_PACK = 1 << 26;          // multiply-adds of a product from which on a copy pays
+// Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first.
+// dx and dW of an odd-sized linear, M x K x N, us with copies / without (dz and (dg | du) lie so from the start):
+//                                bf16              f32
+//      251 x 257 x 255          25 / 19           27 / 26
+//      640 x 637 x 651          32 / 32           43 / 42
+//      821 x 801 x 809          39 / 33           53 / 49
+//      1023 x 1021 x 1027       51 / 55           80 / 81
+//      1531 x 717 x 1209        54 / 57           89 / 94
+//      2047 x 2049 x 2051      117 / 202         413 / 454
+//      4099 x 1027 x 4097      140 / 478         766 / 878
+constexpr double TO_PACK = 1 << 30;          // multiply-adds of a product from which on a copy pays
 bool whole(const void* p, long long ld, long long n, size_t es) { return ((uintptr_t)p | (size_t)(ld * (long long)es)) % 16 == 0 && n % (16 / (long long)es) == 0; }
 struct LinWs {
     bool act, pack_dy, pack_w, pack_x;
