@@ -596,7 +596,7 @@ int mis_comm_finalize(void);
  * A token is one row of `width` consecutive values; rows lie `ld` elements apart (ld >= width, any alignment of the element type; 16-byte aligned rows are faster).  dtype is that
  * of the activations AND the weights; biases, norm parameters and their gradients are f32.  What a forward product keeps for its backward pass
  * goes to `kept`, 16-byte aligned, mis_*_kept_bytes long, in a form of the library's own that the same dtype, act, sizes and biases (null or not) read back.
- * Rows: any number from 0 (a forward call then does nothing, a backward call writes zero parameter gradients).  Outputs must not overlap inputs.
+ * Rows: from 0 (a forward call then does nothing, a backward call writes zero parameter gradients) to below 2^31.  Outputs must not overlap inputs.
  * Workspaces belong to the call until the stream has passed it.  Sums have a fixed order: equal calls give equal bits. */
 
 /* y = (x - mean) * rstd * gamma + beta over each row's D values, rstd = 1 / sqrt(var + eps); gamma / beta NULL: 1 / 0; mean / rstd ([M] f32) NULL: not kept */

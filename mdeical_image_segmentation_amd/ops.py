@@ -1023,7 +1023,8 @@ def gather3d_bwd(dy, dx, ranges):
                                ranges[1].data_ptr(), ranges[2].data_ptr(), stream_ptr()), "mis_gather3d_bwd")
 
 
-# ---- token operators (csrc/layernorm.hip, tok_gemm.hip, token_ops.hip): rows of a 2-D tensor; `tokens` holds the differentiable functions over them ----
+# ---- token operators (csrc/layernorm.hip, tok_gemm.hip, token_ops.hip): rows of a 2-D tensor; `tokens` holds the differentiable functions over them.
+# Outputs must not overlap inputs; `kept` is read back with the type, sizes, activation and biases that it was written with ----
 ACT_CODES_TOKEN = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
 
 
@@ -1043,11 +1044,15 @@ class _TokenCall:
         self.who, self.device, self.dtype = who, ref.device, ref.dtype
         self.code = dtype_code(ref.dtype)
 
+    @staticmethod
+    def say(t):
+        return f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+
     def mat(self, t, name, rows, cols, dtype=None):
         """(pointer, row stride) of a [rows][cols] matrix"""
         dtype = self.dtype if dtype is None else dtype
-        if t.device != self.device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-            raise MisError(f"{self.who}: {name} must be a ({rows}, {cols}) {dtype} tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+            raise MisError(f"{self.who}: {name} must be a ({rows}, {cols}) {dtype} tensor on {self.device}, got {self.say(t)}")
         s0, s1 = t.stride()
         if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
             raise MisError(f"{self.who}: {name} must have unit stride inside its rows and rows that do not overlap, got strides {(s0, s1)}")
@@ -1057,8 +1062,8 @@ class _TokenCall:
         """pointer of a contiguous f32 vector, None for None"""
         if t is None:
             return None
-        if t.device != self.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-            raise MisError(f"{self.who}: {name} must be a contiguous ({n},) float32 tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+            raise MisError(f"{self.who}: {name} must be a contiguous ({n},) float32 tensor on {self.device}, got {self.say(t)}")
         return t.data_ptr()
 
     def run(self, fn, *args):
@@ -1098,8 +1103,8 @@ def layernorm_bwd(dy, x, mean, rstd, gamma=None, dx=None, dgamma=None, dbeta=Non
 
 
 def _linear_desc(c, x, w, act):
-    if x.dim() != 2 or w.dim() != 2:
-        raise MisError(f"{c.who}: x and w must be matrices, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 2:
+        raise MisError(f"{c.who}: x and w must be matrices, got {c.say(x)} and {c.say(w)}")
     d = _lib.LinearDesc()
     d.dtype, d.act = c.code, token_act(act)
     d.M, d.K, d.N = x.shape[0], x.shape[1], w.shape[0]
@@ -1110,15 +1115,16 @@ def _linear_desc(c, x, w, act):
 
 def _kept(c, d, kept, nbytes):
     """pointer of the buffer that carries a forward pass's values to its backward pass"""
-    if kept.device != c.device or kept.dtype != torch.uint8 or not kept.is_contiguous() or kept.numel() < nbytes:
-        raise MisError(f"{c.who}: kept must be a contiguous uint8 tensor of {nbytes} bytes on {c.device}, got {tuple(kept.shape)} {kept.dtype} on {kept.device}")
+    if not isinstance(kept, torch.Tensor) or kept.device != c.device or kept.dtype != torch.uint8 or not kept.is_contiguous() or kept.numel() < nbytes:
+        raise MisError(f"{c.who}: kept must be a contiguous uint8 tensor of {nbytes} bytes on {c.device}, got {c.say(kept)}")
     return kept.data_ptr()
 
 
 def linear_kept_bytes(x, w, bias=None, act=None):
     """size of the buffer `kept` of linear_fwd / linear_bwd (0: nothing is kept)"""
-    d = _linear_desc(_TokenCall("linear_kept_bytes", x), x, w, act)
-    d.bias = None if bias is None else bias.data_ptr()
+    c = _TokenCall("linear_kept_bytes", x)
+    d = _linear_desc(c, x, w, act)
+    d.bias = c.vec(bias, "bias", d.N)
     return load().mis_linear_kept_bytes(C.byref(d))
 
 
@@ -1159,8 +1165,8 @@ def linear_bwd(dy, x, w, bias=None, act=None, kept=None, dx=None, dw=None, dbias
 
 
 def _gated_desc(c, x, wg, wu, act):
-    if x.dim() != 2 or wg.dim() != 2:
-        raise MisError(f"{c.who}: x, wg and wu must be matrices, got {tuple(x.shape)}, {tuple(wg.shape)}, {tuple(wu.shape)}")
+    if x.dim() != 2 or not isinstance(wg, torch.Tensor) or wg.dim() != 2:
+        raise MisError(f"{c.who}: x, wg and wu must be matrices, got {c.say(x)}, {c.say(wg)}, {c.say(wu)}")
     d = _lib.GatedDesc()
     d.dtype, d.act = c.code, token_act(act)
     d.M, d.K, d.F = x.shape[0], x.shape[1], wg.shape[0]
@@ -1174,8 +1180,9 @@ def _gated_desc(c, x, wg, wu, act):
 
 def gated_ffn_kept_bytes(x, wg, wu, bg=None, bu=None):
     """size of the buffer `kept` of gated_ffn_fwd / gated_ffn_bwd"""
-    d = _gated_desc(_TokenCall("gated_ffn_kept_bytes", x), x, wg, wu, None)
-    d.bg, d.bu = (None if b is None else b.data_ptr() for b in (bg, bu))
+    c = _TokenCall("gated_ffn_kept_bytes", x)
+    d = _gated_desc(c, x, wg, wu, None)
+    d.bg, d.bu = c.vec(bg, "bg", d.F), c.vec(bu, "bu", d.F)
     return load().mis_gated_ffn_kept_bytes(C.byref(d))
 
 

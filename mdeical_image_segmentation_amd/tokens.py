@@ -56,7 +56,7 @@ def _tokens(who, x, width):
     return x2, MIS_BF16 if dt is _BF16 else MIS_F32
 
 
-def _weight(who, w, name, x=None):
+def _weight(who, w, name):
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         _refuse(who, f"{name} must be an (out, in) matrix, got {_say(w)}")
     return w if w.is_contiguous() else _unit(w)
@@ -97,6 +97,15 @@ def _call(who, fn, x, *args):
 
 def _scratch(nbytes, x):
     return torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+
+
+def _wanted(*ts):
+    """whether a gradient is (what is not a tensor is refused by the forward pass's checks)"""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return False
 
 
 def _once(backward):
@@ -152,7 +161,7 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension; weight, bias (width,) float32 or None"""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if _wanted(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _norm_fwd(x, weight, bias, float(eps), False)[1]
 
@@ -167,7 +176,7 @@ def _linear_fwd(x, weight, bias, act, residual, keep):
     shape = (M, N) if x.dim() == 2 else x.shape[:-1] + (N,)
     pr = ldr = None
     if residual is not None:
-        if residual.shape != shape:
+        if not isinstance(residual, torch.Tensor) or residual.shape != shape:
             _refuse("linear", f"residual must have the result's shape {tuple(shape)}, got {_say(residual)}")
         r2 = _rows("linear", residual, N, "residual")
         _like("linear", r2, "residual", x2)
@@ -216,7 +225,7 @@ class _Linear(torch.autograd.Function):
 def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual; activation None | 'relu' | 'gelu' | 'gelu_tanh' | 'silu' | 'sigmoid', residual with the result's shape"""
     act = token_act(activation)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or (residual is not None and residual.requires_grad)):
+    if _wanted(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, act, residual)
     return _linear_fwd(x, weight, bias, act, residual, False)[2]
 
@@ -275,7 +284,6 @@ class _GatedFFN(torch.autograd.Function):
 def gated_ffn(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """activation(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate, w_up (features, width), activation 'silu' | 'gelu' | 'gelu_tanh' | 'relu' | 'sigmoid' | None"""
     act = token_act(activation)
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or (b_gate is not None and b_gate.requires_grad) or
-                                    (b_up is not None and b_up.requires_grad)):
+    if _wanted(x, w_gate, w_up, b_gate, b_up):
         return _GatedFFN.apply(x, w_gate, w_up, b_gate, b_up, act)
     return _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, False)[3]

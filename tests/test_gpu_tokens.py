@@ -340,6 +340,46 @@ def test_products_of_every_kind(M, K, N, tile, splits, switches):
         check_all(run_gated(x, w, v, b, None, "silu", dy), O.gated(x, w, v, b, None, "silu", dy), f"gated {M}x{K}x{N}")
 
 
+# few rows and a long k: the weights' kernel with one, two and four tiles of rows, several waves along k, rows and weights at any address
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K, N", [(1, 4104, 24), (16, 1031, 40), (17, 2048, 72), (32, 1031, 33), (33, 520, 70), (48, 1031, 16), (64, 2048, 129), (65, 1031, 40)])
+def test_few_rows(M, K, N, dtype):
+    g = gen(M * K + N)
+    x, w, v, b, res = randn(g, M, K, dtype=dtype), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N), randn(g, M, N, dtype=dtype)
+    for xx, ww, vv in ((x, w, v), (odd(x), odd(w), odd(v))):
+        O.check(tokens.linear(xx, ww, b, "silu", res), O.linear(x, w, b, "silu", res)["y"], f"linear {M}x{K}x{N}")
+        O.check(tokens.gated_ffn(xx, ww, vv, b, None, "gelu"), O.gated(x, w, v, b, None, "gelu")["y"], f"gated {M}x{K}x{N}")
+
+
+# widths at the edges of the lanes that share a row, more rows than the backward pass has blocks for at once
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, D", [(33000, 64), (17000, 65), (16400, 128), (9000, 129), (8200, 256), (4100, 257), (4100, 1024), (2100, 1025), (1100, 2056), (600, 6150)])
+def test_layer_norm_widths_of_every_kind(M, D, dtype):
+    g = gen(M + D)
+    x, w, b, dy = randn(g, M, D, dtype=dtype), randn(g, D) * 0.2 + 1, randn(g, D), randn(g, M, D, dtype=dtype)
+    check_all(run_layer_norm(x, w, b, dy), O.layer_norm(x, w, b, 1e-5, dy), f"layer_norm {M}x{D}")
+
+
+# over 2^30 multiply-adds and odd: the backward products run on copies at aligned rows
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_odd_products(dtype):
+    g = gen(31)
+    M, K, N = 1051, 1021, 1027
+    x, w, v, b, dy = randn(g, M, K, dtype=dtype), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N), randn(g, M, N, dtype=dtype)
+    check_all(run_linear(x, w, b, "none", None, dy), O.linear(x, w, b, "none", None, dy), "linear")
+    check_all(run_linear(odd(x), odd(w), None, "silu", None, odd(dy)), O.linear(x, w, None, "silu", None, dy), "linear at odd strides")
+    check_all(run_gated(x, odd(w), odd(v), b, b, "gelu", dy), O.gated(x, w, v, b, b, "gelu", dy), "gated")
+
+
+def test_what_is_no_tensor_is_refused_on_the_gpu():
+    x, w, y = torch.randn(4, 8, device="cuda"), torch.randn(6, 8, device="cuda"), torch.empty(4, 6, device="cuda")
+    for call in (lambda: tokens.linear(x, w, 1.0), lambda: tokens.linear(x, w, residual=1.0), lambda: tokens.layer_norm(x, "w"), lambda: tokens.gated_ffn(x, w, w, b_up=3), lambda: ops.linear_fwd(x, w, None),
+                 lambda: ops.linear_fwd(x, 3, y), lambda: ops.linear_fwd(x, w, y, "silu"), lambda: ops.linear_fwd(x, w, y, None, "silu", None, 5), lambda: ops.gated_ffn_fwd(x, w, 3, y),
+                 lambda: ops.linear_kept_bytes(x, w, 4, "silu"), lambda: ops.layernorm_fwd(x, x, 1.0)):
+        with pytest.raises(MisError):
+            call()
+
+
 def test_equal_calls_give_equal_bits():
     for dtype in TYPES:
         g = gen(1)

@@ -24,6 +24,21 @@ def test_wrong_shapes_and_names_are_refused(call):
         call(torch.randn(4, 8), torch.randn(6, 8))
 
 
+@pytest.mark.parametrize("call", [
+    lambda x, w: tokens.layer_norm(3.0), lambda x, w: tokens.linear([1.0], w), lambda x, w: tokens.linear(x, 2), lambda x, w: tokens.gated_ffn(x, w, None), lambda x, w: tokens.gated_ffn(None, w, w),
+    lambda x, w: ops.linear_fwd("x", w, w), lambda x, w: ops.layernorm_bwd(x, None, x, x)])
+def test_what_is_no_tensor_is_refused(call):
+    with pytest.raises(MisError):
+        call(torch.randn(4, 8, requires_grad=True), torch.randn(6, 8))
+
+
+@pytest.mark.parametrize("M", [1 << 31, (1 << 40) - 1])
+def test_more_rows_than_an_int_holds_are_refused(M):
+    lib = _lib.load()
+    for d, f in ((_lin(M=M, N=1, K=1), lib.mis_linear_fwd), (_lin(M=M, N=1, K=1), lib.mis_linear_bwd), (_gat(M=M, F=1, K=1), lib.mis_gated_ffn_fwd), (_gat(M=M, F=1, K=1), lib.mis_gated_ffn_bwd)):
+        assert f(C.byref(d), None) < 0 and b"too many" in lib.mis_last_error()
+
+
 def _lin(**kw):
     d = _lib.LinearDesc()
     d.dtype, d.M, d.N, d.K = _lib.MIS_F32, 4, 6, 8
