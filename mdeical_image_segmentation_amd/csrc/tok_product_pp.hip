@@ -12,6 +12,9 @@
 // steps ahead (all 160 KiB of LDS); a buffer's last readers passed the barrier in front of the slot that refills it, and slot 3 retires step s + 1 by a counted wait that leaves the
 // four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
 // LDS images and swizzles are those of tok_product.hpp with 256 rows: [row][128 B] for a k-contiguous operand, [k][512 B] for the other kind, read with the transposing ds_read_b64_tr_b16.
+// Bound: per step 192 KiB of fragments leave and 64 KiB enter the LDS, 2048 cycles at its 128 B a cycle - as many as the MFMAs take, so every cycle of a segment that is neither shows.
+// 8192^3 759 us, 1.45 PFLOP/s (x W^T; dz W 767, dz^T x 818); 32768 x 1024 x 8192, 16 steps a tile: 492 us, 1.12, of which 4 to 5 steps' time a tile is the store of its 128 KiB.  A wave
+// tile of 128 x 128 would need a third less from the LDS, but 256 accumulators and 64 fragment registers a lane do not fit beside the addresses.
 // The fragment reads and their wait are one asm statement: hipcc would put a vmcnt(0), i.e. a wait for the prefetch, in front of a plain LDS read while an LDS-DMA is in flight.
 
 #include "conv_pp_common.hpp"

@@ -10,7 +10,8 @@
 
 namespace {
 constexpr int TO_COLS = 128;          // columns of a block (16 threads x 8)
-// rows of a block: 64, more when that would leave over 512 partial rows for the second pass
+// rows of a block: 64, more when that would leave over 512 partial rows for the second pass (32768 x 4096 bf16 with a bias: 512 partial rows 152 us, 128 of them 139; 16384 x 1024 20 / 19;
+// with 128 a narrow gradient of many rows is too few blocks)
 inline long long to_rows(long long M) {
     long long r = 64;
     while ((M + r - 1) / r > 512) r *= 2;
@@ -19,6 +20,7 @@ inline long long to_rows(long long M) {
 inline long long to_nblk(long long M) { return (M + to_rows(M) - 1) / to_rows(M); }
 }   // namespace
 
+// Bandwidth: per value 2 bytes of dy, 2 (runs) or 4 of z, 2 of dz; gated twice the last two.  32768 x 4096 gated bf16: 1.34 GB in 303 us, 4.4 TB/s; from f32 pre-activations 1.9 GB in 412.
 // dz = dy act'(z) (MODE 0: linear), (dg | du) (MODE 1: gated), nothing but the column sums of dy (MODE 2).  RUNS: the factors are kept instead of z.  A thread: 8 columns, every 16th row
 // of its block.
 template <typename T, int MODE, bool RUNS>
