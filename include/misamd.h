@@ -633,6 +633,8 @@ typedef struct MisLinearDesc {
     void* workspace; size_t workspace_bytes;
 } MisLinearDesc;
 size_t mis_linear_kept_bytes(const MisLinearDesc* d);
+/* of the forward pass: few rows of a long x are cut along x's width where a workspace is given (0 bytes: not cut anyhow, always so up to 64 rows); without one they are not */
+size_t mis_linear_fwd_workspace_bytes(const MisLinearDesc* d);
 int mis_linear_fwd(const MisLinearDesc* d, void* stream);
 /* (of the descriptor as it will be passed: pointers and strides decide whether operands are copied to aligned rows) */
 size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d);
@@ -655,6 +657,7 @@ typedef struct MisGatedDesc {
     void* workspace; size_t workspace_bytes;
 } MisGatedDesc;
 size_t mis_gated_ffn_kept_bytes(const MisGatedDesc* d);
+size_t mis_gated_ffn_fwd_workspace_bytes(const MisGatedDesc* d);          /* (as for the linear product) */
 int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream);
 size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d);
 int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream);

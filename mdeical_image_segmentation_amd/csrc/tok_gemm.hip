@@ -1,49 +1,71 @@
 // Dispatch of the token products (tok_gemm.hpp): tile size, parts along k, and the sum of the parts.
 #include "dispatch_cfg.hpp"
+#include "tok_epilogue.hpp"
 #include "tok_product_plan.hpp"
 
-// y = sum of a product's k parts in their order, rounded; batch 1 goes to y2
-template <typename T> __global__ __launch_bounds__(256) void tg_slab_kernel(const TgArgs a, const float* __restrict__ slab, int splits) {
+// A product's k parts added in their order, then its epilogue: a rounded store (batch 1 goes to y2), bias + activation + residual, or act(batch 0) * batch 1
+template <typename T, int EPI> __global__ __launch_bounds__(256) void tg_slab_kernel(const TgArgs a, const float* __restrict__ slab, int splits) {
     const long long per = (a.N + 7) >> 3;
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.M * per * a.batches) return;
+    if (id >= a.M * per * (EPI == TG_STORE ? a.batches : 1)) return;
     const long long row = id / per, n = (id - row * per) * 8;
     const int nv = a.N - n >= 8 ? 8 : (int)(a.N - n);
-    const int bt = row >= a.M ? 1 : 0;
+    const int bt = EPI == TG_STORE && row >= a.M ? 1 : 0;
     const long long m = row - bt * a.M;
-    const float* p = slab + ((long long)bt * splits * a.M + m) * a.N + n;
-    float v[8];
-    tok_ldn<float>(p, v, nv);
-    for (int s = 1; s < splits; ++s) {
-        float t[8];
-        tok_ldn<float>(p + (long long)s * a.M * a.N, t, nv);
+    auto sum = [&](int batch, float (&v)[8]) __attribute__((always_inline)) {
+        const float* p = slab + ((long long)batch * splits * a.M + m) * a.N + n;
+        tok_ldn<float>(p, v, nv);
+        for (int s = 1; s < splits; ++s) {
+            float t[8];
+            tok_ldn<float>(p + (long long)s * a.M * a.N, t, nv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += t[j];
+            for (int j = 0; j < 8; ++j) v[j] += t[j];
+        }
+    };
+    float v[8];
+    sum(bt, v);
+    if constexpr (EPI == TG_STORE) {
+        tok_stn<T>(reinterpret_cast<T*>(tg_out(a, bt)) + m * a.ldy + n, v, nv);
+    } else if constexpr (EPI == TG_LINEAR) {
+        const TgLinearRow<T> r(a, a.y, n, true);
+        r(m, v);
+    } else {
+        float u[8];
+        sum(1, u);
+        const TgGatedRow<T> r(a, n);
+        r(m, v, u);
     }
-    tok_stn<T>(reinterpret_cast<T*>(bt == 0 ? a.y : a.y2) + m * a.ldy + n, v, nv);
-}
-
-static int tg_slab_sum(int dtype, const TgArgs& a, const float* slab, int splits, hipStream_t stream) {
-    const long long n = (a.M * ((a.N + 7) / 8) * a.batches + 255) / 256;
-    MIS_REQUIRE(n < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
-    if (dtype == MIS_BF16) hipLaunchKernelGGL(tg_slab_kernel<__bf16>, dim3((unsigned)n), dim3(256), 0, stream, a, slab, splits);
-    else hipLaunchKernelGGL(tg_slab_kernel<float>, dim3((unsigned)n), dim3(256), 0, stream, a, slab, splits);
-    MIS_LAUNCH_CHECK("token product (sum of k parts)");
-    return MIS_OK;
 }
 
 namespace {
+template <typename T> void tg_slab_go(int epi, unsigned blocks, const TgArgs& a, const float* slab, int splits, hipStream_t stream) {
+    if (epi == TG_STORE) hipLaunchKernelGGL((tg_slab_kernel<T, TG_STORE>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
+    else if (epi == TG_LINEAR) hipLaunchKernelGGL((tg_slab_kernel<T, TG_LINEAR>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
+    else hipLaunchKernelGGL((tg_slab_kernel<T, TG_GATED>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
+}
+int tg_slab_sum(int dtype, int epi, const TgArgs& a, const float* slab, int splits, hipStream_t stream) {
+    const long long n = (a.M * ((a.N + 7) / 8) * (epi == TG_STORE ? a.batches : 1) + 255) / 256;
+    MIS_REQUIRE(n < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
+    if (dtype == MIS_BF16) tg_slab_go<__bf16>(epi, (unsigned)n, a, slab, splits, stream);
+    else tg_slab_go<float>(epi, (unsigned)n, a, slab, splits, stream);
+    MIS_LAUNCH_CHECK("token product (sum of k parts)");
+    return MIS_OK;
+}
+}   // namespace
+
+namespace {
 // How a product is cut: the cheapest of the tiles and numbers of k parts by this model.  A 64-k step of the blocks that a CU holds takes (us; blocks per CU: 1 .. what fits)
-//      bf16   256 x 256  1.2 (few CUs at work) to 1.5     128 x 128  0.8, 1.25     64 x 64  0.5, 0.7, 0.85, 1.05     gated 64 x (64 + 64)  0.65, 1.0, 1.35
+//      bf16   256 x 256  1.2 (few CUs at work) to 1.5     128 x 128  0.75, 1.15    64 x 64  0.45, 0.6, 0.7, 0.85     gated 64 x (64 + 64)  0.6, 0.9, 1.2
 //      f32                                                128 x 128  4.1, 6.9      64 x 64  1.6, 2.4, 3.2, 4.0       gated 64 x (64 + 64)  2.4, 3.9, 5.4
-// a tile's start and epilogue as much as 3 (256: 5) steps, a cut along k 5 us and its slab's write and read, mostly in the caches, at 7 TB/s.  us, measured with each tile (* the model's choice):
+// a tile's start and epilogue as much as 3 (256: 5) steps, a cut along k 5 us and its slab's write and read, mostly in the caches, at 7 TB/s.  M x K x N, us, each tile at its best number
+// of parts (* the model's choice):
 //                                       256      128       64                                          256      128       64
-//      512 x 512 x 512       x W^T       17       11     *8.1      2048 x 2048 x 2048       dz W       40      *37       42
-//      1024 x 4096 x 1024    x W^T       80       52      *34      4096 x 4096 x 1024       dz W      *34       48       82
-//      2048 x 2048 x 2048    x W^T       45      *30       39      8192 x 1024 x 4096       dz^T x    *75       96      160
-//      4096 x 4096 x 1024    x W^T       80      *53       70      8192 x 1024 x 4096       gated    *116      162      208
-//      8192 x 1024 x 4096    x W^T      *66       90      149      f32 1024 x 4096 x 1024   x W^T       -      290     *106
-//      8192 x 2048 x 8192    x W^T     *217      329      555      f32 8192 x 1024 x 4096   x W^T       -     *528      561
+//      512 x 512 x 512       x W^T       17       11     *8.9      2048 x 2048 x 2048       dz W       40      *31       34
+//      1024 x 4096 x 1024    x W^T       32       25      *24      4096 x 4096 x 1024       dz W      *34       44       67
+//      2048 x 2048 x 2048    x W^T       45      *28       31      8192 x 1024 x 4096       dz^T x    *75       94      129
+//      8192 x 1024 x 4096    x W^T      *66       83      125      8192 x 1024 x 4096       gated    *113      153      187
+//      8192 x 2048 x 8192    x W^T     *217      306      463      f32 8192 x 1024 x 4096   x W^T       -     *522      550
+// A forward product in parts (its epilogue then runs where they are added), us against one piece: 128 x 4096 x 1024 bf16 14 / 29, 128 x 8192 x 8192 38 / 64, f32 512 x 4096 x 1024 47 / 105.
 struct TgCut {
     int tile;               // 256, 128 or 64 rows
     int splits;
@@ -55,7 +77,7 @@ TgCut tg_cut_one(int dtype, int tile, bool may_split, long long M, long long N, 
     if (const int forced = mis_sw(SW_TOK_SPLITS); may_split && forced > 0) return TgCut{tile, (int)(forced < steps ? forced : steps), 0.0};
     const bool f32 = dtype == MIS_F32;
     const int fit = tile == 256 ? 1 : tile == 128 ? 2 : gated ? 3 : 4;          // blocks that a CU holds
-    const double one = tile == 128 ? (f32 ? 1.3 : 0.35) : gated ? (f32 ? 0.9 : 0.28) : (f32 ? 0.75 : 0.32), more = tile == 128 ? (f32 ? 2.8 : 0.45) : gated ? (f32 ? 1.5 : 0.36) : (f32 ? 0.82 : 0.18);
+    const double one = tile == 128 ? (f32 ? 1.3 : 0.35) : gated ? (f32 ? 0.9 : 0.28) : (f32 ? 0.75 : 0.3), more = tile == 128 ? (f32 ? 2.8 : 0.4) : gated ? (f32 ? 1.5 : 0.31) : (f32 ? 0.82 : 0.14);
     TgCut best{tile, 1, 1e30};
     for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || steps / s >= 4); ++s) {
         const long long n = items * s, per = (n + 255) / 256;          // (256 CUs)
@@ -75,7 +97,7 @@ TgCut tg_cut(int dtype, bool aligned, bool may_split, long long M, long long N, 
     if (small.us < best.us) best = small;
     if (big_ok) {
         const TgCut big = tg_cut_one(dtype, 256, may_split, M, N, K, ranges, batches, gated);
-        if (big.us <= best.us * 1.03) best = big;          // (half the traffic from the L2)
+        if (big.us <= best.us * 1.13) best = big;          // (half the traffic from the L2: 4096 x 4096 x 1024 dz^T x, two parts, 51 us against 61 where the model sees 56 and 50)
     }
     return best;
 }
@@ -89,20 +111,36 @@ bool tg_aligned(int dtype, const TgArgs& a, int a_mn, int b_mn) {
 }
 }   // namespace
 
-size_t tg_slab_bytes(int dtype, long long M, long long N, long long K, int ranges, int batches) {
+namespace {
+// a forward product: in one piece with its epilogue, or - few tiles and a long k - its plain products in parts, with the epilogue where they are added
+TgCut tg_cut_of(int dtype, bool aligned, int epi, bool slab, long long M, long long N, long long K, int ranges, int batches) {
+    if (epi == TG_STORE) return tg_cut(dtype, aligned, true, M, N, K, ranges, batches, false);
+    const TgCut whole = tg_cut(dtype, aligned, false, M, N, K, 1, 1, epi == TG_GATED);
+    if (!slab) return whole;
+    const TgCut parts = tg_cut(dtype, aligned, true, M, N, K, 1, epi == TG_GATED ? 2 : 1, false);
+    return parts.splits > 1 && parts.us < 0.9 * whole.us ? parts : whole;
+}
+bool tg_few_rows(int epi, long long M) { return epi != TG_STORE && M <= 64 && mis_sw(SW_TOK_TILE) == 0; }
+}   // namespace
+
+size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, int ranges, int batches) {
+    if (M == 0 || tg_few_rows(epi, M)) return 0;
     size_t most = 0;
     for (int al = 0; al < 2; ++al) {
-        const TgCut c = tg_cut(dtype, al == 1, true, M, N, K, ranges, batches, false);
-        const size_t n = c.splits > 1 ? tok_align((size_t)c.splits * batches * M * N * 4) : 0;
+        const TgCut c = tg_cut_of(dtype, al == 1, epi, true, M, N, K, ranges, batches);
+        const size_t n = c.splits > 1 ? tok_align((size_t)c.splits * (epi == TG_GATED ? 2 : batches) * M * N * 4) : 0;
         if (n > most) most = n;
     }
     return most;
 }
 
-int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream) {
-    const bool al = tg_aligned(dtype, a, a_mn, b_mn);
-    if (epi != TG_STORE && a.M <= 64 && mis_sw(SW_TOK_TILE) == 0) return tok_product_skinny(dtype, epi, a, al, stream);
-    const TgCut c = tg_cut(dtype, al, epi == TG_STORE, a.M, a.N, a.K, a.ranges, a.batches, epi == TG_GATED);
+int tg_launch(int dtype, int a_mn, int b_mn, int epi_, const TgArgs& args, float* slab, hipStream_t stream) {
+    const bool al = tg_aligned(dtype, args, a_mn, b_mn);
+    if (tg_few_rows(epi_, args.M)) return tok_product_skinny(dtype, epi_, args, al, stream);
+    const TgCut c = tg_cut_of(dtype, al, epi_, slab != nullptr, args.M, args.N, args.K, args.ranges, args.batches);
+    TgArgs a = args;
+    if (epi_ == TG_GATED && c.splits > 1) a.batches = 2;
+    const int epi = c.splits > 1 ? TG_SLAB : epi_;
     const long long T = c.tile, BN = epi == TG_GATED ? (T == 256 ? 128 : 64) : T, ck = dtype == MIS_BF16 ? 64 : 32;
     const long long tm = (a.M + T - 1) / T, tn = (a.N + BN - 1) / BN, spr = (a.K + ck - 1) / ck;
     MIS_REQUIRE(tm < (1ll << 24) && tn < (1ll << 24) && spr < (1ll << 28) && tm * tn * a.batches * c.splits < (1ll << 30), MIS_EUNSUPPORTED,
@@ -119,5 +157,5 @@ int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* sl
         {{tok_product_f32_128, tok_product_f32_128_any}, {tok_product_f32_64, tok_product_f32_64_any}}};
     auto* const go = T == 256 ? tok_product_bf16_256 : kernels[dtype == MIS_F32][T == 64][!al];
     if (const int rc = go(a_mn, b_mn, epi, a, pl, stream)) return rc;
-    return pl.splits > 1 ? tg_slab_sum(dtype, a, slab, pl.splits, stream) : MIS_OK;
+    return epi == TG_SLAB ? tg_slab_sum(dtype, epi_, a, slab, pl.splits, stream) : MIS_OK;
 }

@@ -3,8 +3,8 @@
 #pragma once
 #include "tok_common.hpp"
 
-// A product may run over two ranges of k (dx = dg Wg + du Wu: range 0 on p, range 1 on p2, K long each) or be two products of one shape (dWg = dg^T x, dWu = du^T x: batch 1 reads a.p2 and
-// writes y2).  The gated forward product takes the rows of the "up" projection from b.p2.
+// A product may run over two ranges of k (dx = dg Wg + du Wu: range 0 on p, range 1 on p2, K long each) or be two products of one shape (dWg = dg^T x, dWu = du^T x: batch 1 reads p2 and
+// writes y2).  The gated forward product takes the rows of the "up" projection from b.p2; cut along k it is two products of one shape, joined where their parts are added.
 struct TgOperand {
     const void* p;          // element (i, k): p[i * ld + k] (k contiguous) or p[k * ld + i]
     const void* p2;
@@ -31,7 +31,7 @@ struct TgArgs {
     char* kept2;
     long long kept_ld;
 };
-// dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_LINEAR, TG_GATED or TG_STORE.  Enqueues on `stream`.  A TG_STORE product may be cut along
-// k: its parts go to `slab` (tg_slab_bytes) and are added in their order.
+// dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_LINEAR, TG_GATED or TG_STORE.  Enqueues on `stream`.  A product may be cut along
+// k: its parts go to `slab` (tg_slab_bytes; null: a forward product is not cut) and are added in their order.
 int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream);
-size_t tg_slab_bytes(int dtype, long long M, long long N, long long K, int ranges, int batches);
+size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, int ranges, int batches);

@@ -347,8 +347,8 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
     auto place = [&](long long m0, long long n0, int bt, int at) __attribute__((always_inline)) {
         const int range = at >= pl.spr ? 1 : 0, ks = at - range * pl.spr;
         // (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
-        const char* const pa = (const char*)a.a.p + (long long)(AMN ? bt : range) * ((const char*)a.a.p2 - (const char*)a.a.p);
-        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : range) * ((const char*)a.b.p2 - (const char*)a.b.p);
+        const char* const pa = (const char*)a.a.p + (long long)(EPI == TG_GATED ? 0 : bt | range) * ((const char*)a.a.p2 - (const char*)a.a.p);
+        const char* const pb = (const char*)a.b.p + (long long)(EPI == TG_GATED ? (wave >> 2) : bt | range) * ((const char*)a.b.p2 - (const char*)a.b.p);
         na.base = pa + (AMN ? m0 : m0 * a.a.ld) * 2 + ks * step_a;
         nb1.base = pb + (BMN ? n0 : n0 * a.b.ld) * 2 + ks * step_b;
         krem = (int)a.K - ks * 64;
@@ -559,7 +559,8 @@ template <int EPI> int pg_act(const TgArgs& a, const TpPlan& pl, hipStream_t str
 
 int tok_product_bf16_256(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream) {
     if (epi == TG_GATED) return pg_act<TG_GATED>(a, pl, stream);
-    if (!a_mn && !b_mn) return pg_act<TG_LINEAR>(a, pl, stream);
-    if (pl.splits == 1) return a_mn ? pg_go<true, true, TG_STORE>(a, pl, stream) : pg_go<false, true, TG_STORE>(a, pl, stream);
+    if (epi == TG_LINEAR) return pg_act<TG_LINEAR>(a, pl, stream);
+    if (!b_mn) return pg_go<false, false, TG_SLAB>(a, pl, stream);
+    if (epi == TG_STORE) return a_mn ? pg_go<true, true, TG_STORE>(a, pl, stream) : pg_go<false, true, TG_STORE>(a, pl, stream);
     return a_mn ? pg_go<true, true, TG_SLAB>(a, pl, stream) : pg_go<false, true, TG_SLAB>(a, pl, stream);
 }

@@ -221,7 +221,7 @@ LinWs lin_ws(const MisLinearDesc* d) {
     w.part = at;
     if (d->dbias != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->N * 4);
     w.slab = at;            // one product after the other
-    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, d->M, d->K, d->N, 1, 1) : 0, d->dw != nullptr ? tg_slab_bytes(d->dtype, d->N, d->K, d->M, 1, 1) : 0);
+    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->N, 1, 1) : 0, d->dw != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->N, d->K, d->M, 1, 1) : 0);
     w.total = at;
     return w;
 }
@@ -247,7 +247,7 @@ GatWs gat_ws(const MisGatedDesc* d) {
     w.pu = at;
     if (d->dbu != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
     w.slab = at;
-    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, d->M, d->K, d->F, 2, 1) : 0, d->dwg != nullptr ? tg_slab_bytes(d->dtype, d->F, d->K, d->M, 1, 2) : 0);
+    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->F, 2, 1) : 0, d->dwg != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->F, d->K, d->M, 1, 2) : 0);
     w.total = at;
     return w;
 }
@@ -280,6 +280,11 @@ extern "C" size_t mis_linear_kept_bytes(const MisLinearDesc* d) {
     return keep_of(d->dtype, d->bias != nullptr, d->M, d->N, 1).total;
 }
 
+extern "C" size_t mis_linear_fwd_workspace_bytes(const MisLinearDesc* d) {
+    if (d == nullptr || check_dims("mis_linear_fwd", d->dtype, d->act, d->M, d->N, d->K) != MIS_OK) return 0;
+    return tg_slab_bytes(d->dtype, TG_LINEAR, d->M, d->N, d->K, 1, 1);
+}
+
 extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
     const hipStream_t stream = (hipStream_t)stream_;
     const char* who = "mis_linear_fwd";
@@ -301,7 +306,8 @@ extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
         const Keep k = keep_of(d->dtype, d->bias != nullptr, d->M, d->N, 1);
         a.keep = k.how; a.kept = (char*)d->kept; a.kept_ld = k.ld;
     }
-    return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, nullptr, stream);
+    const size_t need = mis_linear_fwd_workspace_bytes(d);
+    return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, need > 0 && d->workspace != nullptr && d->workspace_bytes >= need ? (float*)d->workspace : nullptr, stream);
 }
 
 extern "C" size_t mis_linear_bwd_workspace_bytes(const MisLinearDesc* d) {
@@ -383,6 +389,11 @@ extern "C" size_t mis_gated_ffn_kept_bytes(const MisGatedDesc* d) {
     return keep_of(d->dtype, d->bg != nullptr || d->bu != nullptr, d->M, d->F, 2).total;
 }
 
+extern "C" size_t mis_gated_ffn_fwd_workspace_bytes(const MisGatedDesc* d) {
+    if (d == nullptr || check_dims("mis_gated_ffn_fwd", d->dtype, d->act, d->M, d->F, d->K) != MIS_OK) return 0;
+    return tg_slab_bytes(d->dtype, TG_GATED, d->M, d->F, d->K, 1, 1);
+}
+
 extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
     const hipStream_t stream = (hipStream_t)stream_;
     const char* who = "mis_gated_ffn_fwd";
@@ -403,7 +414,8 @@ extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
         const Keep k = keep_of(d->dtype, d->bg != nullptr || d->bu != nullptr, d->M, d->F, 2);
         a.keep = k.how; a.kept = (char*)d->kept; a.kept2 = a.kept + k.one; a.kept_ld = k.ld;
     }
-    return tg_launch(d->dtype, 0, 0, TG_GATED, a, nullptr, stream);
+    const size_t need = mis_gated_ffn_fwd_workspace_bytes(d);
+    return tg_launch(d->dtype, 0, 0, TG_GATED, a, need > 0 && d->workspace != nullptr && d->workspace_bytes >= need ? (float*)d->workspace : nullptr, stream);
 }
 
 extern "C" size_t mis_gated_ffn_bwd_workspace_bytes(const MisGatedDesc* d) {

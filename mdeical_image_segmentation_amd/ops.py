@@ -1139,6 +1139,9 @@ def linear_fwd(x, w, y, bias=None, act=None, res=None, kept=None):
     lib = load()
     if kept is not None:
         d.kept = _kept(c, d, kept, lib.mis_linear_kept_bytes(C.byref(d)))
+    ws = c.scratch(lib.mis_linear_fwd_workspace_bytes(C.byref(d)))
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
     c.run(lib.mis_linear_fwd, C.byref(d))
 
 
@@ -1195,6 +1198,9 @@ def gated_ffn_fwd(x, wg, wu, h, bg=None, bu=None, act="silu", kept=None):
     lib = load()
     if kept is not None:
         d.kept = _kept(c, d, kept, lib.mis_gated_ffn_kept_bytes(C.byref(d)))
+    ws = c.scratch(lib.mis_gated_ffn_fwd_workspace_bytes(C.byref(d)))
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
     c.run(lib.mis_gated_ffn_fwd, C.byref(d))
 
 

@@ -20,6 +20,7 @@ from ._lib import MIS_BF16, MIS_F32, GatedDesc, LinearDesc, MisError, check, loa
 from .ops import token_act
 
 _F32, _BF16 = torch.float32, torch.bfloat16
+_FEW = 64          # rows up to which a forward product needs no workspace (misamd.h): single tokens save the question
 
 
 def _refuse(who, what):
@@ -187,6 +188,9 @@ def _linear_fwd(x, weight, bias, act, residual, keep):
     lib = load()
     kept = _scratch(lib.mis_linear_kept_bytes(C.byref(d)), x2) if keep and act else None
     d.kept = _ptr(kept)
+    ws = _scratch(lib.mis_linear_fwd_workspace_bytes(C.byref(d)), x2) if M > _FEW else None
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
     _call("linear", lib.mis_linear_fwd, x2, C.byref(d))
     return x2, w, y if x.dim() == 2 else y.view(shape), kept
 
@@ -248,6 +252,9 @@ def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, keep):
     lib = load()
     kept = _scratch(lib.mis_gated_ffn_kept_bytes(C.byref(d)), x2) if keep else None
     d.kept = _ptr(kept)
+    ws = _scratch(lib.mis_gated_ffn_fwd_workspace_bytes(C.byref(d)), x2) if M > _FEW else None
+    if ws is not None:
+        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
     _call("gated_ffn", lib.mis_gated_ffn_fwd, x2, C.byref(d))
     return x2, wg, wu, h if x.dim() == 2 else h.view(x.shape[:-1] + (F,)), kept
 
