@@ -351,6 +351,19 @@ def test_few_rows(M, K, N, dtype):
         O.check(tokens.gated_ffn(xx, ww, vv, b, None, "gelu"), O.gated(x, w, v, b, None, "gelu")["y"], f"gated {M}x{K}x{N}")
 
 
+# a few tiles and a long k: cut along k, the epilogue where the parts are added
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, K, N", [(65, 2048, 33), (100, 4096, 256), (128, 1031, 72), (200, 3000, 131)])
+def test_long_widths(M, K, N, dtype):
+    g = gen(M * K + N)
+    x, w, v, b, res, dy = (randn(g, M, K, dtype=dtype), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N, K, dtype=dtype, scale=K ** -0.5), randn(g, N), randn(g, M, N, dtype=dtype),
+                           randn(g, M, N, dtype=dtype))
+    check_all(run_linear(x, w, b, "gelu", res, dy), O.linear(x, w, b, "gelu", res, dy), f"linear {M}x{K}x{N}")
+    check_all(run_linear(odd(x), odd(w), None, "silu", None, dy), O.linear(x, w, None, "silu", None, dy), f"linear {M}x{K}x{N}")
+    check_all(run_gated(x, w, v, b, None, "silu", dy), O.gated(x, w, v, b, None, "silu", dy), f"gated {M}x{K}x{N}")
+    check_all(run_gated(x, w, v, None, None, "gelu_tanh", dy), O.gated(x, w, v, None, None, "gelu_tanh", dy), f"gated {M}x{K}x{N}")
+
+
 # widths at the edges of the lanes that share a row, more rows than the backward pass has blocks for at once
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M, D", [(33000, 64), (17000, 65), (16400, 128), (9000, 129), (8200, 256), (4100, 257), (4100, 1024), (2100, 1025), (1100, 2056), (600, 6150)])
