@@ -90,6 +90,18 @@ def check_margins(obj):
     return n
 
 
+# The 256 x 256 token product (tok_product_pp.hip): its prefetch is retired by counted waits, and a scratch access would be counted among the loads.
+SCRATCHLESS_KERNELS = {"tok_product_pp.o": "tg_pp_kernel"}
+
+
+def check_scratchless(obj):
+    kernels = {k: v for k, v in disasm(obj).items() if SCRATCHLESS_KERNELS[obj] in k}
+    assert kernels, f"no {SCRATCHLESS_KERNELS[obj]} in {obj}"
+    for name, ins in kernels.items():
+        assert not any(i.startswith("scratch_") for i in ins), f"{name}: scratch instructions (its counted waits would count them)"
+    return len(kernels)
+
+
 def main():
     if not os.path.exists(OBJDUMP):
         print(f"codegen guard: {OBJDUMP} is missing - the guard cannot run, and the build must not pass without it", file=sys.stderr)
@@ -113,6 +125,16 @@ def main():
             continue
         try:
             print(f"codegen guard: {obj}: {check_margins(obj)} barriers, each followed by an s_sleep or >= 4 MFMAs before the next LDS read - ok")
+        except AssertionError as e:
+            print(f"codegen guard FAILED: {obj}: {e}", file=sys.stderr)
+            rc = 1
+    for obj in sorted(SCRATCHLESS_KERNELS):
+        if not os.path.exists(os.path.join(CSRC, obj)):
+            print(f"codegen guard: {obj} has not been built", file=sys.stderr)
+            rc = 2
+            continue
+        try:
+            print(f"codegen guard: {obj}: {check_scratchless(obj)} kernels without scratch - ok")
         except AssertionError as e:
             print(f"codegen guard FAILED: {obj}: {e}", file=sys.stderr)
             rc = 1
