@@ -4,7 +4,7 @@
 // products - gated 64 rows x 64 columns of gate and of up.
 //
 // A step is 128 bytes of k per row (64 bf16 / 32 f32), in two halves.  The pipeline of a wave, all of it plain code whose waits the compiler counts:
-//      half 0   MFMAs of half 0 | fragments of half 1 <- LDS | step s + 1: registers -> other LDS buffer | step s + 2: global -> registers
+//      half 0   MFMAs of half 0 | fragments of half 1 <- LDS | step s + 1: registers -> other LDS buffer | step s + 2 or s + 3: global -> registers
 //      barrier
 //      half 1   MFMAs of half 1 | fragments of half 0 of step s + 1 <- other LDS buffer
 // One barrier a step: a buffer is overwritten a step after its last reads, which were waited for in front of the barrier between.  The steps are flat over a block's tiles (the grid is what
@@ -14,8 +14,8 @@
 //   LDS image, k contiguous:   [row][128 B], 16-byte chunks at position c ^ key(row): a fragment read touches each bank once
 //   LDS image, own index cont.: [k][TILE elements]; bf16 fragments by the transposing read (16 lanes: 4 k x 4 runs of 4), f32 ones by plain 16-byte reads, which give one k of four
 //                              MFMA tiles (tile v then holds the indices 4 r + v)
-// Bound, f32: the MFMAs (16 x 16 x 4, 32 cycles): 8192 x 1024 x 4096 528 us, 130 of the 154 TFLOP/s that a large f32 product of the library reaches.  bf16: two blocks' LDS traffic (as many bytes
-// per MFMA and half as many again as the 256 x 256 tiles'): 2048^3 30 us, 0.57 PFLOP/s, where those tiles leave three quarters of the chip idle (45 us).  Operands at any address go by
+// Bound, f32: the MFMAs (16 x 16 x 4, 32 cycles): 8192 x 1024 x 4096 510 us, 135 of the 154 TFLOP/s that a large f32 product of the library reaches.  bf16: two blocks' LDS traffic (as many bytes
+// per MFMA and half as many again as the 256 x 256 tiles'): 2048^3 27 us, 0.63 PFLOP/s, where those tiles leave three quarters of the chip idle (45 us).  Operands at any address go by
 // element-aligned loads with a mask per chunk: 2047 x 2049 x 2051 dz W 87 us against 63 on aligned copies.
 // Sums are f32 (MFMA accumulators); k order inside a step is the same for both operands, which is all the sum needs.
 #pragma once
@@ -58,13 +58,13 @@ struct TpStep {
 };
 
 // Staging of one operand: F chunks of 16 bytes per thread.  k contiguous: chunk c = t & 7 of the rows (t >> 3) + 32 j; own index contiguous: chunk t % CPR of the k rows t / CPR + j KR.
-template <typename T, bool MN, bool B, int EPI, bool AL, int F> struct TpStage {
+template <typename T, bool MN, bool B, int EPI, bool AL, int F, int SETS> struct TpStage {
     static constexpr int ES = sizeof(T), EPC = Tr<T>::EPC, TILE = 32 * F, CPR = TILE / EPC, KR = 256 / CPR;
     static constexpr bool PAIR = B && EPI == TG_GATED;
     int c, r;               // chunk, first row / k row
     unsigned voff;          // byte offset of chunk 0 (AL)
     long long ld;
-    u32x4 v[F];
+    u32x4 v[SETS][F];
     __device__ __forceinline__ TpStage(long long ld_) : ld(ld_) {
         const int t = threadIdx.x;
         c = MN ? t % CPR : t & 7;
@@ -72,22 +72,22 @@ template <typename T, bool MN, bool B, int EPI, bool AL, int F> struct TpStage {
         voff = (unsigned)(r * ld * ES) + c * 16;
     }
     // chunk j of the step; one that does not exist reads as zeros
-    __device__ __forceinline__ void load(const TpStep& s, int j) {
+    __device__ __forceinline__ void load(const TpStep& s, int set, int j) {
         if constexpr (AL) {
             // (chunks are whole here: a lane is in or out)
             const __amdgpu_buffer_rsrc_t q = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(PAIR && (j & 1) ? s.base2 : s.base), 0, 0x7fffffff, 0x00020000);
             const bool ok = MN ? (r + j * KR < s.left && c * EPC < s.rows) : (c * EPC < s.left && r + rowstep(j) < s.rows);
-            v[j] = __builtin_amdgcn_raw_buffer_load_b128(q, ok ? (int)voff : TP_OOB, (int)(rowstep(j) * ld * ES), 0);
+            v[set][j] = __builtin_amdgcn_raw_buffer_load_b128(q, ok ? (int)voff : TP_OOB, (int)(rowstep(j) * ld * ES), 0);
         } else {
             const T* p = reinterpret_cast<const T*>(PAIR && (j & 1) ? s.base2 : s.base) + (long long)(r + rowstep(j)) * ld + c * EPC;
-            if constexpr (MN) v[j] = tp_chunk<T>(p, r + j * KR < s.left ? s.rows - c * EPC : 0);
-            else v[j] = tp_chunk<T>(p, r + rowstep(j) < s.rows ? s.left - c * EPC : 0);
+            if constexpr (MN) v[set][j] = tp_chunk<T>(p, r + j * KR < s.left ? s.rows - c * EPC : 0);
+            else v[set][j] = tp_chunk<T>(p, r + rowstep(j) < s.rows ? s.left - c * EPC : 0);
         }
     }
     static constexpr int TILE_K = Tr<T>::CK;
     // rows (k rows) that chunk j lies behind chunk 0; gated B: rows 64 b + q of the tile are column 32 b + (q & 31), of gate for q < 32, else of up
     static constexpr int rowstep(int j) { return MN ? j * KR : (PAIR ? (j >> 1) * 32 : j * 32); }
-    __device__ __forceinline__ void put(char* lds, int j) const {
+    __device__ __forceinline__ void put(char* lds, int set, int j) const {
         int off;
         if constexpr (!MN) {
             off = (r + 32 * j) * 128 + ((c ^ tp_key<B>(r)) << 4);          // (key(r + 32 j) = key(r))
@@ -97,7 +97,7 @@ template <typename T, bool MN, bool B, int EPI, bool AL, int F> struct TpStage {
         } else {
             off = (r + j * KR) * (TILE * 4) + c * 16;
         }
-        lds_write_b128(lds, off, v[j]);
+        lds_write_b128(lds, off, v[set][j]);
     }
 };
 
@@ -165,13 +165,17 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
         w.n0 = (long long)c * BN;
         return w;
     };
+    // (an item has an even number of steps, the last of an odd number reads nothing but zeros: the loop below is two steps long)
     auto steps_of = [&](int sp) __attribute__((always_inline)) { return all_steps - sp * pl.sps < pl.sps ? all_steps - sp * pl.sps : pl.sps; };
 
     // ---- load cursor: the step that goes into the staging registers next ----
-    TpStage<T, AMN, false, EPI, AL, FM> ga(a.a.ld);
-    TpStage<T, BMN, true, EPI, AL, FN> gb(a.b.ld);
+    // Steps that wait in registers: two (2048^3 bf16 dz W 31 -> 27 us, 64 x 64 tiles 5 to 15 %, f32 2 to 4 %) where they fit - operands at any address, bf16 dz^T x in 128 x 128 tiles and gated
+    // 64 x (64 + 64) spill with them (8192 x 1024 x 4096: 88 -> 111 us, gated 175 -> 312)
+    constexpr int SETS = AL && !(EPI == TG_GATED && FM == 2) && !(AMN && ES == 2 && FM == 4) ? 2 : 1;
+    TpStage<T, AMN, false, EPI, AL, FM, SETS> ga(a.a.ld);
+    TpStage<T, BMN, true, EPI, AL, FN, SETS> gb(a.b.ld);
     TpStep na, nb;
-    int lit = first, lrem = 0;
+    int lit = first, lrem = 0, lpad = 0;
     const long long step_a = AMN ? CK * ES * a.a.ld : CK * ES, step_b = BMN ? CK * ES * a.b.ld : CK * ES;
     auto place = [&](long long m0, long long n0, int bt, int at) __attribute__((always_inline)) {
         const int range = at >= pl.spr ? 1 : 0, ks = at - range * pl.spr;
@@ -190,7 +194,9 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
     auto load_tile = [&](bool second) __attribute__((always_inline)) {
         const bool live = lit < pl.items;
         const TpItem w = tile_of(live ? lit : first);
-        lrem = second ? lrem : steps_of(w.sp);
+        const int n = steps_of(w.sp);
+        lrem = second ? lrem : n + (n & 1);
+        lpad = n & 1;
         place(w.m0, w.n0, w.bt, second ? pl.spr : w.sp * pl.sps);
         na.rows = live ? na.rows : 0;
         nb.rows = live ? nb.rows : 0;
@@ -201,9 +207,12 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
         nb.base2 += step_b;
         na.left -= CK;
         nb.left -= CK;
-        if (--lrem == 0 || na.left <= 0) {
+        --lrem;
+        if (lrem == lpad) na.left = nb.left = lrem == 0 ? na.left : 0;
+        if (lrem == 0 || (na.left <= 0 && lrem != lpad)) {
             lit += lrem == 0 ? (int)gridDim.x : 0;
             load_tile(lrem != 0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);               // (lgkmcnt(0): a scalar load in flight here would turn the loop's waits for LDS reads into waits for all of them)
         }
     };
 
@@ -220,13 +229,13 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
     };
     load_tile(false);
     // chunk f of both operands (FM <= FN)
-    auto load = [&](int f) __attribute__((always_inline)) {
-        if (f < FM) ga.load(na, f);
-        gb.load(nb, f);
+    auto load = [&](int set, int f) __attribute__((always_inline)) {
+        if (f < FM) ga.load(na, set, f);
+        gb.load(nb, set, f);
     };
-    auto put = [&](char* st, int f) __attribute__((always_inline)) {
-        if (f < FM) ga.put(st, f);
-        gb.put(st + OPA, f);
+    auto put = [&](char* st, int set, int f) __attribute__((always_inline)) {
+        if (f < FM) ga.put(st, set, f);
+        gb.put(st + OPA, set, f);
     };
     u32x4 a0[FM], b0[FN], a1[FM], b1[FN];
     // fragments 2 f, 2 f + 1 of half kk
@@ -237,46 +246,53 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
             if (g < FN) tp_frag<T, BMN, true, FN>(bv, st + OPA, wn, kk, g);
         }
     };
+    // steps 0 .. SETS on their way, step 0 into LDS
 #pragma unroll
-    for (int f = 0; f < FN; ++f) load(f);
-    advance();
+    for (int s = 0; s < SETS; ++s) {
+#pragma unroll
+        for (int f = 0; f < FN; ++f) load(s, f);
+        advance();
+    }
 #pragma unroll
     for (int f = 0; f < FN; ++f) {
-        put(smem, f);
-        load(f);
+        put(smem, 0, f);
+        load(0, f);
     }
     advance();
     barrier();
 #pragma unroll
     for (int f = 0; f < FN; ++f) frags(a0, b0, smem, 0, f);
 
-    int cit = first, buf = 0;
+    int cit = first;
     TpItem ct = tile_of(cit);
     int crem = steps_of(ct.sp);
     while (true) {
-        char* const cur = smem + buf * STAGE;
-        char* const nxt = smem + (buf ^ 1) * STAGE;
-        // (sched_barrier: the scheduler interleaves inside a row of MFMAs but does not pull a whole step's loads together, which would not fit the registers)
 #pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            frags(a1, b1, cur, 1, f);
-            put(nxt, f);
-            load(f);
+        for (int p = 0; p < 2; ++p) {                         // steps of even and odd number: buffers and register sets by name
+            char* const cur = smem + p * STAGE;
+            char* const nxt = smem + (p ^ 1) * STAGE;
+            const int set = (p ^ 1) & (SETS - 1);
+            // (sched_barrier: the scheduler interleaves inside a row of MFMAs but does not pull a whole step's loads together, which would not fit the registers)
 #pragma unroll
-            for (int p = 0; p < FM; ++p) mma_b128<T>(acc[f][p], b0[f], a0[p]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int f = 0; f < FN; ++f) {
+                frags(a1, b1, cur, 1, f);
+                put(nxt, set, f);
+                load(set, f);
+#pragma unroll
+                for (int q = 0; q < FM; ++q) mma_b128<T>(acc[f][q], b0[f], a0[q]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance();
+            barrier();
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                frags(a0, b0, nxt, 0, f);
+#pragma unroll
+                for (int q = 0; q < FM; ++q) mma_b128<T>(acc[f][q], b1[f], a1[q]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        advance();
-        barrier();
-#pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            frags(a0, b0, nxt, 0, f);
-#pragma unroll
-            for (int p = 0; p < FM; ++p) mma_b128<T>(acc[f][p], b1[f], a1[p]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        buf ^= 1;
-        if (--crem > 0) continue;
+        if ((crem -= 2) > 0) continue;
 
         // ---- the tile is complete ----
         using Run = TpRun<T, BMN, FN>;
@@ -327,6 +343,7 @@ __global__ __launch_bounds__(256, tp_blocks(FM, FN)) void tok_product_kernel(con
             for (int p = 0; p < FM; ++p) acc[f][p] = f32x4{0.f, 0.f, 0.f, 0.f};
         ct = tile_of(cit);
         crem = steps_of(ct.sp);
+        __builtin_amdgcn_s_waitcnt(0xc07f);                   // (as above)
     }
 }
 
