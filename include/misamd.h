@@ -633,7 +633,7 @@ typedef struct MisLinearDesc {
     void* workspace; size_t workspace_bytes;
 } MisLinearDesc;
 size_t mis_linear_kept_bytes(const MisLinearDesc* d);
-/* of the forward pass: few rows of a long x are cut along x's width where a workspace is given (0 bytes: not cut anyhow, always so up to 64 rows); without one they are not */
+/* of the forward pass: few rows of a long x are cut along x's width where a workspace is given (0 bytes: not cut anyhow, always so up to 32 rows); without one they are not */
 size_t mis_linear_fwd_workspace_bytes(const MisLinearDesc* d);
 int mis_linear_fwd(const MisLinearDesc* d, void* stream);
 /* (of the descriptor as it will be passed: pointers and strides decide whether operands are copied to aligned rows) */

@@ -120,7 +120,7 @@ TgCut tg_cut_of(int dtype, bool aligned, int epi, bool slab, long long M, long l
     const TgCut parts = tg_cut(dtype, aligned, true, M, N, K, 1, epi == TG_GATED ? 2 : 1, false);
     return parts.splits > 1 && parts.us < 0.9 * whole.us ? parts : whole;
 }
-bool tg_few_rows(int epi, long long M) { return epi != TG_STORE && M <= 64 && mis_sw(SW_TOK_TILE) == 0; }
+bool tg_few_rows(int epi, long long M) { return epi != TG_STORE && M <= 32 && mis_sw(SW_TOK_TILE) == 0; }
 }   // namespace
 
 size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, int ranges, int batches) {

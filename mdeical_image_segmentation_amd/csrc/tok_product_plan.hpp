@@ -25,5 +25,5 @@ int tok_product_f32_128(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPl
 int tok_product_f32_128_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
 int tok_product_f32_64(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
 int tok_product_f32_64_any(int a_mn, int b_mn, int epi, const TgArgs& a, const TpPlan& pl, hipStream_t stream);
-// forward products of at most 64 rows (tok_skinny.hip)
+// forward products of at most 32 rows (tok_skinny.hip)
 int tok_product_skinny(int dtype, int epi, const TgArgs& a, bool aligned, hipStream_t stream);

@@ -1,16 +1,17 @@
-// Forward token products with few rows (serving: one token, or a handful of sequences' next tokens): y = act(x W^T + b) + res and h = act(g) u for M <= 64.
+// Forward token products with few rows (serving: one token, or a handful of sequences' next tokens): y = act(x W^T + b) + res and h = act(g) u for M <= 32.
 //
 // The weights are read once and are all there is to read, so the kernel is a stream of them: a block owns 16 columns (gated: the same 16 of gate and of up; 32 for more than 16 rows), its
 // waves take turns along k in units of 128 bytes per row, and a weight fragment goes from global memory straight into the MFMA's row side - no LDS, no barrier - against the rows of x,
 // which come out of the L2.  The waves' partial sums meet in LDS in wave order, then the epilogue runs on runs of 8 columns.  As many waves per block as bring ~2000 of them onto the
-// chip, at most 8 where a lane holds more than one tile of rows (16 leave it 128 registers, and the fragments of 64 rows spill: 8192 x 8192 bf16, 64 rows, 163 us instead of 53).
+// chip, at most 8 where a lane holds two tiles of rows (16 leave it 128 registers, and its fragments spill).
 //
-// Bound by the weights: one row of 8192 x 8192 bf16 (134 MB) 32.6 us, 4.1 TB/s; f32 57 us, 4.7 TB/s.  Up to which rows, against the 64 x 64 tiles (tok_product.hpp), us here / there:
-//      rows   bf16 2048 -> 8192   8192 -> 8192   gated 8192 -> 2 x 8192   f32 2048 -> 8192   8192 -> 8192
-//        1          7.8 / 17.8      32.6 / 60.4         39.3 / 91.5            15 / 54           57 / 206
-//       32         10.7 / 19.3      34.5 / 63.2         65.6 / 101             24 / 54           73 / 211
-//       64         15.8 / 19.3      53.1 / 64.6         92.1 / 99              40 / 55          141 / 213
-// Beyond 64 every further tile of rows would read the weights again.
+// Bound by the weights: one row of 8192 x 8192 bf16 (134 MB) 30 us, 4.5 TB/s; f32 57 us, 4.7 TB/s.  Up to which rows, against 64 x 64 tiles with k parts (tok_gemm.hip), us here / there:
+//      rows   bf16 2048 -> 8192   gated 2048 -> 2 x 8192   8192 -> 8192   f32 1024 -> 4096   2048 -> 8192   8192 -> 8192
+//        1          8.1 / 13.1          13.7 / 17.5          30 / 26         8.3 / 13.2        15 / 25        57 / 74
+//       16          9.9 / 13.1          15.2 / 17.1          35 / 27         8.2 / 13.2        18 / 25        70 / 75
+//       32         10.7 / 13.1          21.3 / 17.6          38 / 28        12.3 / 13.3        24 / 26        73 / 75
+//       48         14.2 / 13.1          23.3 / 17.8          43 / 28        18.7 / 13.3        38 / 27       134 / 77        (with four tiles of rows per lane)
+// - two launches and a sum where this is one, so the smallest calls are its own whatever the weights.
 #include "tok_epilogue.hpp"
 #include "tok_product_plan.hpp"
 
@@ -139,8 +140,7 @@ template <typename T, int NT, int MT, bool GATED, bool AL> int sk_go(const TgArg
 }
 template <typename T, bool GATED, bool AL> int sk_rows(const TgArgs& a, hipStream_t stream) {
     if (a.M <= 16) return sk_go<T, GATED ? 2 : 1, 1, GATED, AL>(a, stream);
-    if (a.M <= 32) return sk_go<T, 2, 2, GATED, AL>(a, stream);
-    return sk_go<T, 2, 4, GATED, AL>(a, stream);
+    return sk_go<T, 2, 2, GATED, AL>(a, stream);
 }
 template <typename T> int sk_type(int epi, const TgArgs& a, bool al, hipStream_t stream) {
     if (epi == TG_GATED) return al ? sk_rows<T, true, true>(a, stream) : sk_rows<T, true, false>(a, stream);

@@ -190,14 +190,14 @@ size_t most(size_t a, size_t b) { return a > b ? a : b; }
 // Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first.
 // dx and dW of an odd-sized linear, M x K x N, us with copies / without (dz and (dg | du) lie so from the start):
 //                                bf16              f32
-//      251 x 257 x 255          25 / 19           27 / 26
-//      640 x 637 x 651          32 / 32           43 / 42
-//      821 x 801 x 809          39 / 33           53 / 49
-//      1023 x 1021 x 1027       51 / 55           80 / 81
-//      1531 x 717 x 1209        54 / 57           89 / 94
-//      2047 x 2049 x 2051      117 / 202         413 / 454
-//      4099 x 1027 x 4097      140 / 478         766 / 878
-constexpr double TO_PACK = 1 << 30;          // multiply-adds of a product from which on a copy pays
+//      251 x 257 x 255          25 / 18           25 / 24
+//      640 x 637 x 651          26 / 37           41 / 38
+//      821 x 801 x 809          30 / 35           57 / 62
+//      1023 x 1021 x 1027       39 / 64           74 / 81
+//      1531 x 717 x 1209        43 / 81           92 / 107
+//      2047 x 2049 x 2051      102 / 180         409 / 444
+//      4099 x 1027 x 4097      139 / 431         767 / 863
+constexpr double TO_PACK = 1 << 29;          // multiply-adds of a product from which on a copy pays
 bool whole(const void* p, long long ld, long long n, size_t es) { return ((uintptr_t)p | (size_t)(ld * (long long)es)) % 16 == 0 && n % (16 / (long long)es) == 0; }
 struct LinWs {
     bool act, pack_dy, pack_w, pack_x;

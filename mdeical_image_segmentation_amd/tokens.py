@@ -20,7 +20,7 @@ from ._lib import MIS_BF16, MIS_F32, GatedDesc, LinearDesc, MisError, check, loa
 from .ops import token_act
 
 _F32, _BF16 = torch.float32, torch.bfloat16
-_FEW = 64          # rows up to which a forward product needs no workspace (misamd.h): single tokens save the question
+_FEW = 32          # rows up to which a forward product needs no workspace (misamd.h): single tokens save the question
 
 
 def _refuse(who, what):

@@ -340,7 +340,7 @@ def test_products_of_every_kind(M, K, N, tile, splits, switches):
         check_all(run_gated(x, w, v, b, None, "silu", dy), O.gated(x, w, v, b, None, "silu", dy), f"gated {M}x{K}x{N}")
 
 
-# few rows and a long k: the weights' kernel with one, two and four tiles of rows, several waves along k, rows and weights at any address
+# few rows and a long k: the weights' kernel with one and two tiles of rows, several waves along k, rows and weights at any address; the tiles behind it
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M, K, N", [(1, 4104, 24), (16, 1031, 40), (17, 2048, 72), (32, 1031, 33), (33, 520, 70), (48, 1031, 16), (64, 2048, 129), (65, 1031, 40)])
 def test_few_rows(M, K, N, dtype):

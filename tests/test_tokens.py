@@ -117,7 +117,7 @@ def test_null_descriptors_are_refused():
 def test_forward_workspaces():
     lib = _lib.load()
     assert lib.mis_linear_fwd_workspace_bytes(None) == 0 and lib.mis_gated_ffn_fwd_workspace_bytes(None) == 0
-    for M, some in ((1, False), (64, False), (100, True), (0, False)):          # few tiles and 128 steps: cut along the width, but not where the rows are few enough for the weights' kernel
+    for M, some in ((1, False), (32, False), (33, True), (100, True), (0, False)):          # few tiles and 128 steps: cut along the width, but not where the rows are few enough for the weights' kernel
         assert (lib.mis_linear_fwd_workspace_bytes(C.byref(_lin(M=M, N=256, K=8192))) > 0) == some
         assert (lib.mis_gated_ffn_fwd_workspace_bytes(C.byref(_gat(M=M, F=256, K=8192))) > 0) == some
     assert lib.mis_linear_fwd_workspace_bytes(C.byref(_lin(M=16384, N=8192, K=512))) == 0          # enough tiles
