@@ -109,6 +109,11 @@ def _wanted(*ts):
     return False
 
 
+def _new(t):
+    """a contiguous matrix of t's shape and type (empty_like is the cheapest of torch's allocations)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _once(backward):
     """differentiable once: the plain function, unless a graph of the backward pass itself is asked for (then torch's wrapper, whose outputs refuse a second differentiation)"""
     wrapped = once_differentiable(backward)
@@ -127,7 +132,7 @@ def _norm_fwd(x, weight, bias, eps, keep):
     x2, code = _tokens("layer_norm", x, D)
     M = x2.shape[0]
     pw, pb = _vec("layer_norm", weight, "weight", D, x2), _vec("layer_norm", bias, "bias", D, x2)
-    y = torch.empty((M, D), dtype=x2.dtype, device=x2.device)
+    y = _new(x2)
     st = torch.empty((2, M), dtype=_F32, device=x2.device) if keep else None
     ps = st.data_ptr() if keep else None
     _call("layer_norm", load().mis_layernorm_fwd, x2, code, x2.data_ptr(), _ld(x2), M, D, eps, pw, pb, y.data_ptr(), D, ps, ps + 4 * M if keep else None)
@@ -149,8 +154,8 @@ class _LayerNorm(torch.autograd.Function):
         code = MIS_BF16 if x.dtype is _BF16 else MIS_F32
         nx, nw, nb, _ = ctx.needs_input_grad
         dy = _rows("layer_norm (backward)", dy, D, "dy")
-        dx = torch.empty((M, D), dtype=x.dtype, device=x.device) if nx else None
-        dw = torch.empty((D,), dtype=_F32, device=x.device) if nw else None
+        dx = _new(x) if nx else None
+        dw = torch.empty_like(weight) if nw else None
         db = torch.empty((D,), dtype=_F32, device=x.device) if nb else None
         lib = load()
         n = lib.mis_layernorm_bwd_workspace_bytes(code, M, D) if nw or nb else 0
@@ -213,9 +218,9 @@ class _Linear(torch.autograd.Function):
         M, K = x.shape
         N = w.shape[0]
         d2 = _rows("linear (backward)", dy, N, "dy")
-        dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if nx else None
-        dw = torch.empty((N, K), dtype=x.dtype, device=x.device) if nw else None
-        db = torch.empty((N,), dtype=_F32, device=x.device) if nb else None
+        dx = _new(x) if nx else None
+        dw = _new(w) if nw else None
+        db = torch.empty_like(bias) if nb else None
         d = LinearDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, N, K, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ptr(bias), None, 0, None, 0, _ptr(kept),
                        d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dw), K, _ptr(db))
         lib = load()
@@ -274,10 +279,10 @@ class _GatedFFN(torch.autograd.Function):
         M, K = x.shape
         F = wg.shape[0]
         d2 = _rows("gated_ffn (backward)", dh, F, "dh")
-        dx = torch.empty((M, K), dtype=x.dtype, device=x.device) if nx else None
-        dwg, dwu = (torch.empty((F, K), dtype=x.dtype, device=x.device), torch.empty((F, K), dtype=x.dtype, device=x.device)) if ng or nu else (None, None)
-        dbg = torch.empty((F,), dtype=_F32, device=x.device) if nbg else None
-        dbu = torch.empty((F,), dtype=_F32, device=x.device) if nbu else None
+        dx = _new(x) if nx else None
+        dwg, dwu = (_new(wg), _new(wu)) if ng or nu else (None, None)
+        dbg = torch.empty_like(bg) if nbg else None
+        dbu = torch.empty_like(bu) if nbu else None
         d = GatedDesc(MIS_BF16 if x.dtype is _BF16 else MIS_F32, ctx.act, M, F, K, x.data_ptr(), _ld(x), wg.data_ptr(), wu.data_ptr(), _ld(wg), _ptr(bg), _ptr(bu), None, 0, _ptr(kept),
                       d2.data_ptr(), _ld(d2), _ptr(dx), K, _ptr(dwg), _ptr(dwu), K, _ptr(dbg), _ptr(dbu))
         lib = load()
