@@ -6,6 +6,13 @@
 // where batch bt is stored (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
 __device__ __forceinline__ char* tg_out(const TgArgs& a, int bt) { return (char*)a.y + (long long)bt * ((char*)a.y2 - (char*)a.y); }
 
+// a run's exponent is that of its values inside the matrix: behind it act'(0) or act(0) may be larger than all of them
+__device__ __forceinline__ void tg_inside(float (&v)[8], int nv) {
+    if (nv >= 8) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < nv ? v[j] : 0.f;
+}
+
 // y = act(v + bias) + res
 template <typename T, int ACT = -1> struct TgLinearRow {
     const TgArgs& a;
@@ -26,6 +33,7 @@ template <typename T, int ACT = -1> struct TgLinearRow {
         if (sizeof(T) == 2 && a.keep == TG_KEEP_RUNS) {
             float d[8];
             tok_act8<false, true>(ACT < 0 ? a.act : ACT, v, d);
+            tg_inside(d, nv);
             *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
         } else {
             tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
@@ -67,6 +75,8 @@ template <typename T, int ACT = -1> struct TgGatedRow {
             tok_act8<false, true>(ACT < 0 ? a.act : ACT, g, d);
 #pragma unroll
             for (int j = 0; j < 8; ++j) d[j] *= u[j];
+            tg_inside(d, nv);
+            tg_inside(g, nv);
             *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
             *reinterpret_cast<u32x4*>(a.kept2 + m * a.kept_ld + n * 2) = tok_run_pack(g);
         } else {

@@ -231,6 +231,18 @@ def test_what_is_kept_holds_any_scale_and_one_bad_value_spoils_only_its_own_grad
     assert not torch.isfinite(got2["dwg"][3]).any()
 
 
+# the last run of a width that is no multiple of 8: what lies behind the matrix (act'(0) or act(0), larger than every factor here) must not cost the factors their precision
+@pytest.mark.parametrize("N", [1, 3, 9, 12])
+@pytest.mark.parametrize("act, z", [("silu", -1.2784), ("gelu", -0.7518), ("sigmoid", -12.0)])
+def test_what_is_kept_of_a_ragged_run(act, z, N):
+    g = gen(N)
+    M, dt = 300, torch.bfloat16
+    x, w, dy = (z + 0.02 * randn(g, M, 1)).to(dt), torch.ones(N, 1, dtype=dt, device="cuda"), randn(g, M, N, dtype=dt)
+    check_all(run_linear(x, w, None, act, None, dy), O.linear(x, w, None, act, None, dy), f"linear {act} {N}")
+    v = randn(g, N, 1, dtype=dt)
+    check_all(run_gated(x, w, v, None, None, act, dy), O.gated(x, w, v, None, None, act, dy), f"gated {act} {N}")
+
+
 def test_gated_ffn_one_weight_twice():
     g = gen(9)
     x, w, dy = randn(g, 30, 48), randn(g, 40, 48), randn(g, 30, 40)
