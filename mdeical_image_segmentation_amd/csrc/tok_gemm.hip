@@ -4,10 +4,8 @@
 #include "tok_product_plan.hpp"
 
 // A product's k parts added in their order, then its epilogue: a rounded store (batch 1 goes to y2), bias + activation + residual, or act(batch 0) * batch 1
-template <typename T, int EPI> __global__ __launch_bounds__(256) void tg_slab_kernel(const TgArgs a, const float* __restrict__ slab, int splits) {
+template <typename T, int EPI> __device__ __forceinline__ void tg_slab_run(const TgArgs& a, const float* __restrict__ slab, int splits, long long id) {
     const long long per = (a.N + 7) >> 3;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.M * per * (EPI == TG_STORE ? a.batches : 1)) return;
     const long long row = id / per, n = (id - row * per) * 8;
     const int nv = a.N - n >= 8 ? 8 : (int)(a.N - n);
     const int bt = EPI == TG_STORE && row >= a.M ? 1 : 0;
@@ -36,22 +34,47 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void tg_slab_ke
         r(m, v, u);
     }
 }
+template <typename T, int EPI> __global__ __launch_bounds__(256) void tg_slab_kernel(const TgSum s) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (id < s.runs) tg_slab_run<T, EPI>(s.a, s.slab, s.splits, id);
+}
+// two products' sums: the first nb0 blocks add s, the others t
+template <typename T> __global__ __launch_bounds__(256) void tg_slab2_kernel(const TgSum s, const TgSum t, unsigned nb0) {
+    if (blockIdx.x < nb0) {
+        const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+        if (id < s.runs) tg_slab_run<T, TG_STORE>(s.a, s.slab, s.splits, id);
+    } else {
+        const long long id = (long long)(blockIdx.x - nb0) * 256 + threadIdx.x;
+        if (id < t.runs) tg_slab_run<T, TG_STORE>(t.a, t.slab, t.splits, id);
+    }
+}
 
 namespace {
-template <typename T> void tg_slab_go(int epi, unsigned blocks, const TgArgs& a, const float* slab, int splits, hipStream_t stream) {
-    if (epi == TG_STORE) hipLaunchKernelGGL((tg_slab_kernel<T, TG_STORE>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
-    else if (epi == TG_LINEAR) hipLaunchKernelGGL((tg_slab_kernel<T, TG_LINEAR>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
-    else hipLaunchKernelGGL((tg_slab_kernel<T, TG_GATED>), dim3(blocks), dim3(256), 0, stream, a, slab, splits);
+template <typename T> void tg_slab_go(int epi, unsigned blocks, const TgSum& s, hipStream_t stream) {
+    if (epi == TG_STORE) hipLaunchKernelGGL((tg_slab_kernel<T, TG_STORE>), dim3(blocks), dim3(256), 0, stream, s);
+    else if (epi == TG_LINEAR) hipLaunchKernelGGL((tg_slab_kernel<T, TG_LINEAR>), dim3(blocks), dim3(256), 0, stream, s);
+    else hipLaunchKernelGGL((tg_slab_kernel<T, TG_GATED>), dim3(blocks), dim3(256), 0, stream, s);
 }
-int tg_slab_sum(int dtype, int epi, const TgArgs& a, const float* slab, int splits, hipStream_t stream) {
-    const long long n = (a.M * ((a.N + 7) / 8) * (epi == TG_STORE ? a.batches : 1) + 255) / 256;
+int tg_slab_sum(int dtype, int epi, const TgSum& s, hipStream_t stream) {
+    const long long n = (s.runs + 255) / 256;
     MIS_REQUIRE(n < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
-    if (dtype == MIS_BF16) tg_slab_go<__bf16>(epi, (unsigned)n, a, slab, splits, stream);
-    else tg_slab_go<float>(epi, (unsigned)n, a, slab, splits, stream);
+    if (dtype == MIS_BF16) tg_slab_go<__bf16>(epi, (unsigned)n, s, stream);
+    else tg_slab_go<float>(epi, (unsigned)n, s, stream);
     MIS_LAUNCH_CHECK("token product (sum of k parts)");
     return MIS_OK;
 }
 }   // namespace
+
+int tg_sums(int dtype, const TgSum& s, const TgSum& t, hipStream_t stream) {
+    if (s.slab == nullptr && t.slab == nullptr) return MIS_OK;
+    if (s.slab == nullptr || t.slab == nullptr) return tg_slab_sum(dtype, TG_STORE, s.slab != nullptr ? s : t, stream);
+    const long long n0 = (s.runs + 255) / 256, n1 = (t.runs + 255) / 256;
+    MIS_REQUIRE(n0 + n1 < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
+    if (dtype == MIS_BF16) hipLaunchKernelGGL(tg_slab2_kernel<__bf16>, dim3((unsigned)(n0 + n1)), dim3(256), 0, stream, s, t, (unsigned)n0);
+    else hipLaunchKernelGGL(tg_slab2_kernel<float>, dim3((unsigned)(n0 + n1)), dim3(256), 0, stream, s, t, (unsigned)n0);
+    MIS_LAUNCH_CHECK("token product (sums of k parts)");
+    return MIS_OK;
+}
 
 namespace {
 // How a product is cut: the cheapest of the tiles and numbers of k parts by this model.  A 64-k step of the blocks that a CU holds takes (us; blocks per CU: 1 .. what fits)
@@ -134,7 +157,7 @@ size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, 
     return most;
 }
 
-int tg_launch(int dtype, int a_mn, int b_mn, int epi_, const TgArgs& args, float* slab, hipStream_t stream) {
+int tg_launch(int dtype, int a_mn, int b_mn, int epi_, const TgArgs& args, float* slab, hipStream_t stream, TgSum* later) {
     const bool al = tg_aligned(dtype, args, a_mn, b_mn);
     if (tg_few_rows(epi_, args.M)) return tok_product_skinny(dtype, epi_, args, al, stream);
     const TgCut c = tg_cut_of(dtype, al, epi_, slab != nullptr, args.M, args.N, args.K, args.ranges, args.batches);
@@ -157,5 +180,9 @@ int tg_launch(int dtype, int a_mn, int b_mn, int epi_, const TgArgs& args, float
         {{tok_product_f32_128, tok_product_f32_128_any}, {tok_product_f32_64, tok_product_f32_64_any}}};
     auto* const go = T == 256 ? tok_product_bf16_256 : kernels[dtype == MIS_F32][T == 64][!al];
     if (const int rc = go(a_mn, b_mn, epi, a, pl, stream)) return rc;
-    return epi == TG_SLAB ? tg_slab_sum(dtype, epi_, a, slab, pl.splits, stream) : MIS_OK;
+    if (epi != TG_SLAB) return MIS_OK;
+    const TgSum sum{a, slab, pl.splits, a.M * ((a.N + 7) / 8) * (epi_ == TG_STORE ? a.batches : 1)};
+    if (later == nullptr) return tg_slab_sum(dtype, epi_, sum, stream);
+    *later = sum;
+    return MIS_OK;
 }

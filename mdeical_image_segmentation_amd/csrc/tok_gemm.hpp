@@ -33,5 +33,13 @@ struct TgArgs {
 };
 // dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_LINEAR, TG_GATED or TG_STORE.  Enqueues on `stream`.  A product may be cut along
 // k: its parts go to `slab` (tg_slab_bytes; null: a forward product is not cut) and are added in their order.
-int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream);
+// later (TG_STORE): the sum of the parts, if there are any, is not enqueued but left there for tg_sums - a backward pass adds those of both its products in one launch.
+struct TgSum {
+    TgArgs a;
+    const float* slab;      // null: nothing to add
+    int splits;
+    long long runs;         // runs of 8 columns
+};
+int tg_launch(int dtype, int a_mn, int b_mn, int epi, const TgArgs& a, float* slab, hipStream_t stream, TgSum* later = nullptr);
+int tg_sums(int dtype, const TgSum& s, const TgSum& t, hipStream_t stream);
 size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, int ranges, int batches);

@@ -93,9 +93,16 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
     }
 }
 
-// rows of `cols` values, ld apart -> the same rows at a pitch of whole runs of 8, zeros behind them
-template <typename T> __global__ __launch_bounds__(256) void tok_pack_kernel(const T* __restrict__ src, long long ld, long long rows, long long cols, T* __restrict__ dst, long long pitch) {
-    const long long per = pitch >> 3;
+// Up to three matrices, `cols` values a row, rows ld apart -> the same rows at a pitch of whole runs of 8, zeros behind them
+struct ToPack {
+    struct { const void* src; long long ld, rows, cols; void* dst; } m[3];
+};
+template <typename T> __global__ __launch_bounds__(256) void tok_pack_kernel(const ToPack p) {
+    const T* const src = reinterpret_cast<const T*>(blockIdx.y == 0 ? p.m[0].src : blockIdx.y == 1 ? p.m[1].src : p.m[2].src);
+    T* const dst = reinterpret_cast<T*>(blockIdx.y == 0 ? p.m[0].dst : blockIdx.y == 1 ? p.m[1].dst : p.m[2].dst);
+    const long long ld = blockIdx.y == 0 ? p.m[0].ld : blockIdx.y == 1 ? p.m[1].ld : p.m[2].ld, rows = blockIdx.y == 0 ? p.m[0].rows : blockIdx.y == 1 ? p.m[1].rows : p.m[2].rows,
+                    cols = blockIdx.y == 0 ? p.m[0].cols : blockIdx.y == 1 ? p.m[1].cols : p.m[2].cols;
+    const long long per = (cols + 7) >> 3, pitch = per * 8;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (long long)gridDim.x * 256) {
         const long long r = i / per, c = (i - r * per) * 8;
         float v[8];
@@ -186,7 +193,6 @@ int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
 #define TO_LD(who, ld, n, what) MIS_REQUIRE((ld) >= (n) && (ld) < TO_MAX, MIS_EINVAL, "%s: the row stride of " what " (%lld) is below its width", who, (long long)(ld))
 #define TO_PTR(who, p, what) MIS_REQUIRE((p) != nullptr, MIS_EINVAL, "%s: " what " is null", who)
 
-size_t most(size_t a, size_t b) { return a > b ? a : b; }
 // Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first.
 // dx and dW of an odd-sized linear, M x K x N, us with copies / without (dz and (dg | du) lie so from the start):
 //                                bf16              f32
@@ -201,7 +207,7 @@ constexpr double TO_PACK = 1 << 29;          // multiply-adds of a product from 
 bool whole(const void* p, long long ld, long long n, size_t es) { return ((uintptr_t)p | (size_t)(ld * (long long)es)) % 16 == 0 && n % (16 / (long long)es) == 0; }
 struct LinWs {
     bool act, pack_dy, pack_w, pack_x;
-    size_t dz, w, x, part, slab, total;
+    size_t dz, w, x, part, slab_x, slab_w, total;
 };
 LinWs lin_ws(const MisLinearDesc* d) {
     LinWs w{};
@@ -220,14 +226,16 @@ LinWs lin_ws(const MisLinearDesc* d) {
     if (w.pack_x) at += tok_align((size_t)d->M * to_pitch(d->K) * es);
     w.part = at;
     if (d->dbias != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->N * 4);
-    w.slab = at;            // one product after the other
-    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->N, 1, 1) : 0, d->dw != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->N, d->K, d->M, 1, 1) : 0);
+    w.slab_x = at;
+    if (d->dx != nullptr) at += tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->N, 1, 1);
+    w.slab_w = at;
+    if (d->dw != nullptr) at += tg_slab_bytes(d->dtype, TG_STORE, d->N, d->K, d->M, 1, 1);
     w.total = at;
     return w;
 }
 struct GatWs {
     bool pack_w, pack_x;
-    size_t dz, w, x, pg, pu, slab, total;
+    size_t dz, w, x, pg, pu, slab_x, slab_w, total;
 };
 GatWs gat_ws(const MisGatedDesc* d) {
     GatWs w{};
@@ -246,19 +254,35 @@ GatWs gat_ws(const MisGatedDesc* d) {
     if (d->dbg != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
     w.pu = at;
     if (d->dbu != nullptr) at += tok_align((size_t)to_nblk(d->M) * d->F * 4);
-    w.slab = at;
-    at += most(d->dx != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->F, 2, 1) : 0, d->dwg != nullptr ? tg_slab_bytes(d->dtype, TG_STORE, d->F, d->K, d->M, 1, 2) : 0);
+    w.slab_x = at;
+    if (d->dx != nullptr) at += tg_slab_bytes(d->dtype, TG_STORE, d->M, d->K, d->F, 2, 1);
+    w.slab_w = at;
+    if (d->dwg != nullptr) at += tg_slab_bytes(d->dtype, TG_STORE, d->F, d->K, d->M, 1, 2);
     w.total = at;
     return w;
 }
-int to_pack(int dtype, const void* src, long long ld, long long rows, long long cols, void* dst, hipStream_t stream) {
-    const long long pitch = to_pitch(cols), n = (rows * (pitch / 8) + 255) / 256;
-    const dim3 grid((unsigned)(n < 8192 ? n : 8192));
-    if (dtype == MIS_BF16) hipLaunchKernelGGL(tok_pack_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)src, ld, rows, cols, (__bf16*)dst, pitch);
-    else hipLaunchKernelGGL(tok_pack_kernel<float>, grid, dim3(256), 0, stream, (const float*)src, ld, rows, cols, (float*)dst, pitch);
-    MIS_LAUNCH_CHECK("token rows");
-    return MIS_OK;
-}
+// the copies of a call, enqueued together
+struct ToCopies {
+    ToPack p{};
+    int n = 0;
+    long long runs = 0;          // of the largest
+    TgOperand add(const void* src, long long ld, long long rows, long long cols, void* dst) {
+        p.m[n].src = src; p.m[n].ld = ld; p.m[n].rows = rows; p.m[n].cols = cols; p.m[n].dst = dst;
+        ++n;
+        const long long r = rows * (to_pitch(cols) / 8);
+        runs = r > runs ? r : runs;
+        return TgOperand{dst, dst, to_pitch(cols), true};
+    }
+    int go(int dtype, hipStream_t stream) const {
+        if (n == 0) return MIS_OK;
+        const long long b = (runs + 255) / 256;
+        const dim3 grid((unsigned)(b < 8192 ? b : 8192), (unsigned)n);
+        if (dtype == MIS_BF16) hipLaunchKernelGGL(tok_pack_kernel<__bf16>, grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL(tok_pack_kernel<float>, grid, dim3(256), 0, stream, p);
+        MIS_LAUNCH_CHECK("token rows");
+        return MIS_OK;
+    }
+};
 // an empty batch has zero gradients
 __global__ void tok_zero_kernel(char* p, long long pitch, long long rows, long long bytes) {
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * bytes; i += (long long)gridDim.x * blockDim.x) p[(i / bytes) * pitch + i % bytes] = 0;
@@ -343,45 +367,40 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     char* const ws = (char*)d->workspace;
     TgOperand dz{d->dy, d->dy, d->lddy, false};
     float* const part = d->dbias != nullptr ? (float*)(ws + w.part) : nullptr;
+    ToCopies copies;
     if (w.act) {
         dz = TgOperand{ws + w.dz, ws + w.dz, to_pitch(d->N), true};
         if (prod || part != nullptr)
             TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->kept, k, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, dz.ld, part, nullptr, stream));
     } else {
         if (part != nullptr) TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, Keep{TG_KEEP_F32, 0, 0, 0}, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
-        if (w.pack_dy) {
-            TO_TRY(to_pack(d->dtype, d->dy, d->lddy, d->M, d->N, ws + w.dz, stream));
-            dz = TgOperand{ws + w.dz, ws + w.dz, to_pitch(d->N), true};
-        }
+        if (w.pack_dy) dz = copies.add(d->dy, d->lddy, d->M, d->N, ws + w.dz);
     }
     if (part != nullptr) TO_TRY(tok_column_sums(part, nullptr, to_nblk(d->M), d->N, d->dbias, nullptr, stream));
+    TgOperand W{d->w, d->w, d->ldw, false}, X{d->x, d->x, d->ldx, false};
+    if (w.pack_w) W = copies.add(d->w, d->ldw, d->N, d->K, ws + w.w);
+    if (w.pack_x) X = copies.add(d->x, d->ldx, d->M, d->K, ws + w.x);
+    TO_TRY(copies.go(d->dtype, stream));
+    TgSum sx{}, sw{};
     if (d->dx != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
         a.a = dz;
-        a.b = TgOperand{d->w, d->w, d->ldw, false};
-        if (w.pack_w) {
-            TO_TRY(to_pack(d->dtype, d->w, d->ldw, d->N, d->K, ws + w.w, stream));
-            a.b = TgOperand{ws + w.w, ws + w.w, to_pitch(d->K), true};
-        }
+        a.b = W;
         a.M = d->M; a.N = d->K; a.K = d->N;
         a.y = a.y2 = d->dx; a.ldy = d->lddx;
-        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab_x), stream, &sx));
     }
     if (d->dw != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
         a.a = dz;
-        a.b = TgOperand{d->x, d->x, d->ldx, false};
-        if (w.pack_x) {
-            TO_TRY(to_pack(d->dtype, d->x, d->ldx, d->M, d->K, ws + w.x, stream));
-            a.b = TgOperand{ws + w.x, ws + w.x, to_pitch(d->K), true};
-        }
+        a.b = X;
         a.M = d->N; a.N = d->K; a.K = d->M;
         a.y = a.y2 = d->dw; a.ldy = d->lddw;
-        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab_w), stream, &sw));
     }
-    return MIS_OK;
+    return tg_sums(d->dtype, sx, sw, stream);
 }
 
 extern "C" size_t mis_gated_ffn_kept_bytes(const MisGatedDesc* d) {
@@ -460,34 +479,33 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     void* const du = ws + w.dz + pitch * es;
     TO_TRY(to_dz<1>(d->dtype, d->dh, d->lddh, d->kept, k, d->act, d->M, F, dz, lddz, pg, pu, stream));
     if (pg != nullptr || pu != nullptr) TO_TRY(tok_column_sums(pg, pu, to_nblk(d->M), F, d->dbg, d->dbu, stream));
+    TgOperand W{d->wg, d->wu, d->ldw, false}, X{d->x, d->x, d->ldx, false};
+    ToCopies copies;
+    if (w.pack_w) {
+        W = copies.add(d->wg, d->ldw, F, d->K, ws + w.w);
+        W.p2 = copies.add(d->wu, d->ldw, F, d->K, ws + w.w + tok_align((size_t)F * to_pitch(d->K) * es)).p;
+    }
+    if (w.pack_x) X = copies.add(d->x, d->ldx, d->M, d->K, ws + w.x);
+    TO_TRY(copies.go(d->dtype, stream));
+    TgSum sx{}, sw{};
     if (d->dx != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
         a.a = TgOperand{dz, du, lddz, true};
-        a.b = TgOperand{d->wg, d->wu, d->ldw, false};
-        if (w.pack_w) {
-            char* const pu2 = ws + w.w + tok_align((size_t)F * to_pitch(d->K) * es);
-            TO_TRY(to_pack(d->dtype, d->wg, d->ldw, F, d->K, ws + w.w, stream));
-            TO_TRY(to_pack(d->dtype, d->wu, d->ldw, F, d->K, pu2, stream));
-            a.b = TgOperand{ws + w.w, pu2, to_pitch(d->K), true};
-        }
+        a.b = W;
         a.M = d->M; a.N = d->K; a.K = F;
         a.ranges = 2;
         a.y = a.y2 = d->dx; a.ldy = d->lddx;
-        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
+        TO_TRY(tg_launch(d->dtype, 0, 1, TG_STORE, a, (float*)(ws + w.slab_x), stream, &sx));
     }
     if (d->dwg != nullptr) {
         TgArgs a{};
         a.ranges = a.batches = 1;
         a.a = TgOperand{dz, du, lddz, true};
-        a.b = TgOperand{d->x, d->x, d->ldx, false};
-        if (w.pack_x) {
-            TO_TRY(to_pack(d->dtype, d->x, d->ldx, d->M, d->K, ws + w.x, stream));
-            a.b = TgOperand{ws + w.x, ws + w.x, to_pitch(d->K), true};
-        }
+        a.b = X;
         a.M = F; a.N = d->K; a.K = d->M;
         a.y = d->dwg; a.y2 = d->dwu; a.ldy = d->lddw; a.batches = 2;
-        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab), stream));
+        TO_TRY(tg_launch(d->dtype, 1, 1, TG_STORE, a, (float*)(ws + w.slab_w), stream, &sw));
     }
-    return MIS_OK;
+    return tg_sums(d->dtype, sx, sw, stream);
 }
