@@ -16,7 +16,7 @@
 //                              MFMA tiles (tile v then holds the indices 4 r + v)
 // Bound, f32: the MFMAs (16 x 16 x 4, 32 cycles): 8192 x 1024 x 4096 510 us, 135 of the 154 TFLOP/s that a large f32 product of the library reaches.  bf16: two blocks' LDS traffic (as many bytes
 // per MFMA and half as many again as the 256 x 256 tiles'): 2048^3 27 us, 0.63 PFLOP/s, where those tiles leave three quarters of the chip idle (45 us).  Operands at any address go by
-// element-aligned loads with a mask per chunk: 2047 x 2049 x 2051 dz W 87 us against 63 on aligned copies.
+// element-aligned loads with a mask per chunk: 2047 x 2049 x 2051 dz W 81 us against 50 with aligned copies.
 // Sums are f32 (MFMA accumulators); k order inside a step is the same for both operands, which is all the sum needs.
 #pragma once
 #include "tok_epilogue.hpp"

@@ -195,15 +195,15 @@ int check_dims(const char* who, int dtype, int act, long long M, int N, int K) {
 
 // Products want operands whose rows start on 16 bytes and end on whole chunks.  In a backward pass whose products are large enough to pay for a copy the others are copied to such rows first.
 // dx and dW of an odd-sized linear, M x K x N, us with copies / without (dz and (dg | du) lie so from the start):
-//                                bf16              f32
-//      251 x 257 x 255          25 / 18           25 / 24
-//      640 x 637 x 651          26 / 37           41 / 38
-//      821 x 801 x 809          30 / 35           57 / 62
-//      1023 x 1021 x 1027       39 / 64           74 / 81
-//      1531 x 717 x 1209        43 / 81           92 / 107
-//      2047 x 2049 x 2051      102 / 180         409 / 444
-//      4099 x 1027 x 4097      139 / 431         767 / 863
-constexpr double TO_PACK = 1 << 29;          // multiply-adds of a product from which on a copy pays
+//                                bf16              f32        (dx alone: bf16    f32)
+//      251 x 257 x 255          18 / 18           21 / 24            14 / 10   14 / 11
+//      411 x 405 x 403          19 / 28           31 / 36            14 / 12   17 / 18
+//      640 x 637 x 651          21 / 37           35 / 35            14 / 17   21 / 20
+//      1023 x 1021 x 1027       34 / 64           71 / 82            17 / 24   37 / 38
+//      1531 x 717 x 1209        38 / 81           88 / 108           22 / 30   49 / 51
+//      2047 x 2049 x 2051       95 / 181         404 / 443           50 / 81  209 / 223
+//      4099 x 1027 x 4097      134 / 434         757 / 860           74 / 205 387 / 429
+constexpr double TO_PACK = 1 << 26;          // multiply-adds of a product from which on a copy pays
 bool whole(const void* p, long long ld, long long n, size_t es) { return ((uintptr_t)p | (size_t)(ld * (long long)es)) % 16 == 0 && n % (16 / (long long)es) == 0; }
 struct LinWs {
     bool act, pack_dy, pack_w, pack_x;

@@ -385,7 +385,7 @@ def test_layer_norm_widths_of_every_kind(M, D, dtype):
     check_all(run_layer_norm(x, w, b, dy), O.layer_norm(x, w, b, 1e-5, dy), f"layer_norm {M}x{D}")
 
 
-# over 2^30 multiply-adds and odd: the backward products run on copies at aligned rows
+# large and odd: the backward products run on copies at aligned rows
 @pytest.mark.parametrize("dtype", TYPES)
 def test_large_odd_products(dtype):
     g = gen(31)
