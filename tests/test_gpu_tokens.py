@@ -467,6 +467,37 @@ def test_captured_training_step_replays():
         assert all(torch.equal(a, b) for a, b in zip(want, out if k % 2 else out2)), k
 
 
+def test_captured_products_in_parts_have_workspaces_of_their_own():
+    g = gen(17)
+    w, v = randn(g, 256, 4096, dtype=torch.bfloat16, scale=0.02), randn(g, 256, 4096, dtype=torch.bfloat16, scale=0.02)
+    xs = [randn(g, 100, 4096, dtype=torch.bfloat16) for _ in range(2)]
+
+    def call(x):
+        return tokens.linear(x, w, activation="gelu"), tokens.gated_ffn(x, w, v)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s), torch.no_grad():
+        call(xs[0])
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in xs], []
+    for graph, x in zip(graphs, xs):
+        with torch.cuda.graph(graph), torch.no_grad():
+            outs.append(call(x))
+    streams = [torch.cuda.Stream() for _ in xs]
+    for k in range(4):
+        for x in xs:
+            x.copy_(randn(gen(40 + k), 100, 4096, dtype=torch.bfloat16))
+        want = [call(x) for x in xs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):          # both at once
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(t, u) for t, u in zip(a, b)), k
+
+
 def test_rows_past_two_to_the_31_elements():
     # three tokens 2^30 + 8 elements apart: the last one starts past 2^31
     D, ld = 64, (1 << 30) + 8
