@@ -4,13 +4,13 @@
 // wave and step for 64 MFMAs) - the two waves of a SIMD are one barrier apart, so that one is always inside its 32 MFMAs (512 cycles) while the other fetches fragments:
 //
 //      slot        0            1            2            3               4
-//      group 0     R0 B(s+1)    M0           R1 A(s+2)    M1 wait         R0' ...      R = fragment reads, M = 32 MFMAs, every slot ends with a barrier of all 8 waves
-//      group 1     M1"          R0 B(s+1)    M0           R1 A(s+2) wait  M1 ...
+//      group 0     R0 B(s+1)    M0           R1 A(s+2) w  M1              R0' ...      R = fragment reads, M = 32 MFMAs, every slot ends with a barrier of all 8 waves
+//      group 1     M1"          R0 B(s+1)    M0           w R1 A(s+2)     M1 ...       w = wait for this wave's part of step s + 1
 //
 // Both operands arrive by LDS-DMA, 64 KiB a step, four instructions of 1 KiB per wave in each of its R segments: the CU's load path takes about 25 cycles for one, and a wave that
 // issues into the full path stalls (two of them inside an M segment made it 800 cycles long).  B is double-buffered and fetched one step ahead, A has three buffers and is fetched two
-// steps ahead (all 160 KiB of LDS); a buffer's last readers passed the barrier in front of the slot that refills it, and slot 3 retires step s + 1 by a counted wait that leaves the
-// four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
+// steps ahead (all 160 KiB of LDS); a buffer's last readers passed the barrier in front of the slot that refills it, and step s + 1 is waited for a segment before the barrier
+// in front of its first read, by a count that leaves group 0's four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
 // LDS images and swizzles are those of tok_product.hpp with 256 rows: [row][128 B] for a k-contiguous operand, [k][512 B] for the other kind, read with the transposing ds_read_b64_tr_b16.
 // Bound: per step 192 KiB of fragments leave and 64 KiB enter the LDS, 2048 cycles at its 128 B a cycle - as many as the MFMAs take, so every cycle of a segment that is neither shows.
 // 8192^3 759 us, 1.45 PFLOP/s (x W^T; dz W 767, dz^T x 818); 32768 x 1024 x 8192, 16 steps a tile: 492 us, 1.12, of which 4 to 5 steps' time a tile is the store of its 128 KiB.  A wave
@@ -406,6 +406,7 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
     if (va) pg_issue(pg_dma(la, na, lds0 + PG_OP + wave * 1024));          // A of step 1
     advance();                                                // nb: B of step 1, na: A of step 2
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_sleep(4);                              // 256 cycles between the first steps' arrival and the barrier behind which other waves read them (see retire)
     __syncthreads();
     if (grp == 1) __builtin_amdgcn_s_barrier();               // the stagger
     __builtin_amdgcn_sched_barrier(0);
@@ -449,7 +450,9 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    // step s + 1 is complete once at most the four A(s + 2) just issued are in flight
+    // Step s + 1 is complete in this wave's part once at most the four A(s + 2) just issued are in flight.  Both groups wait for it a whole segment before the barrier in front of its first
+    // read (slot 4), not right at that barrier: a read that starts within a few dozen cycles of another wave's vmcnt wait can still see the old contents of the last bytes of its LDS-DMA.
+    // Between the wait and that barrier lie group 0's 32 MFMAs (slot 3) and group 1's 12 fragment reads with their own wait (slot 3); scripts/codegen_guard.py pins both.
     auto retire = [&](int inflight) __attribute__((always_inline)) {
         if (inflight) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -458,7 +461,6 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
 #pragma unroll 1
     while (true) {
         // ---- segment 0 ----
-        if (grp == 0) __builtin_amdgcn_s_sleep(1);            // keep a distance between the barrier that published this step and its first read
         read(0, vb);
         barrier();
         __builtin_amdgcn_s_setprio(1);
@@ -466,9 +468,9 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         __builtin_amdgcn_s_setprio(0);
         barrier();
         // ---- segment 1 ----
-        const int inflight = va;
+        if (grp == 1) retire(0);                              // (its B(s + 1) is the youngest: A(s + 2) goes out with the reads below)
         read(1, va);
-        if (grp == 1) retire(inflight);
+        if (grp == 0) retire(va);
         barrier();
         __builtin_amdgcn_s_setprio(1);
         curA = curA == lds0 + 2 * PG_OP ? lds0 : curA + PG_OP;
@@ -479,7 +481,6 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         advance();
-        if (grp == 0) retire(inflight);
         barrier();
         if (--crem == 0) {
             // ---- the tile is complete: group 0 waits for group 1's last M, and both store at once (one after the other they would leave each SIMD to one wave's dependent VALU

@@ -102,6 +102,41 @@ def check_scratchless(obj):
     return len(kernels)
 
 
+# ... and the same kernel's distance between an LDS-DMA's arrival and another wave's first read of it: a wave that has waited for its DMA (a vmcnt wait of its own) has a whole segment
+# before the barrier behind which the others read - at least 12 fragment reads up to the next barrier, or 32 MFMAs between the next barrier and the one behind it; in the prologue a sleep.
+SEGMENT_KERNELS = {"tok_product_pp.o": "tg_pp_kernel"}
+
+
+def segment_waits(ins):
+    """kinds of the vmcnt waits up to the last MFMA: 'reads', 'mfmas', 'sleep', or None for a wait that stands right at its barrier"""
+    last = max(i for i, t in enumerate(ins) if t.startswith("v_mfma"))
+    kinds = []
+    for i, t in enumerate(ins[:last]):
+        if not re.match(r"s_waitcnt vmcnt\(\d+\)$", t):
+            continue
+        seen = [{"ds_read": 0, "v_mfma": 0, "s_sleep": 0}, {"ds_read": 0, "v_mfma": 0, "s_sleep": 0}]
+        part = 0
+        for u in ins[i + 1:]:
+            if u.startswith("s_barrier"):
+                part += 1
+                if part == 2:
+                    break
+            for k in seen[0]:
+                seen[min(part, 1)][k] += (int(u.split()[1], 0) if k == "s_sleep" else 1) if u.startswith(k) else 0
+        kinds.append("reads" if seen[0]["ds_read"] >= 12 else "mfmas" if seen[1]["v_mfma"] >= 32 else "sleep" if seen[0]["s_sleep"] >= 2 else None)
+    return kinds
+
+
+def check_segments(obj):
+    kernels = {k: v for k, v in disasm(obj).items() if SEGMENT_KERNELS[obj] in k}
+    assert kernels, f"no {SEGMENT_KERNELS[obj]} in {obj}"
+    for name, ins in kernels.items():
+        kinds = segment_waits(ins)
+        assert None not in kinds, f"{name}: a wave waits for its LDS-DMA right at the barrier behind which another one reads it"
+        assert {"reads", "mfmas", "sleep"} <= set(kinds), f"{name}: expected the prologue's wait and one of each group, found {kinds}"
+    return len(kernels)
+
+
 def main():
     if not os.path.exists(OBJDUMP):
         print(f"codegen guard: {OBJDUMP} is missing - the guard cannot run, and the build must not pass without it", file=sys.stderr)
@@ -135,6 +170,7 @@ def main():
             continue
         try:
             print(f"codegen guard: {obj}: {check_scratchless(obj)} kernels without scratch - ok")
+            print(f"codegen guard: {obj}: {check_segments(obj)} kernels with a segment between a DMA's arrival and its readers' barrier - ok")
         except AssertionError as e:
             print(f"codegen guard FAILED: {obj}: {e}", file=sys.stderr)
             rc = 1

@@ -31,5 +31,19 @@ def test_fp32_all_dma_kernels_keep_their_distance_between_a_barrier_and_the_next
     assert guard.check_margins(obj) >= 2
 
 
+@pytest.mark.parametrize("obj", sorted(guard.SEGMENT_KERNELS))
+def test_token_product_has_a_segment_between_a_dmas_arrival_and_its_readers_barrier(obj, built):
+    assert guard.check_segments(obj) >= 1
+
+
+def test_a_wait_right_at_the_barrier_is_found():
+    read, mma = ["ds_read_b128 v[0:3], v9"] * 12, ["v_mfma_f32_16x16x32_bf16 a[0:3], v[0:3], v[4:7], a[0:3]"] * 32
+    wait, bar = ["s_waitcnt vmcnt(4)"], ["s_barrier"]
+    assert guard.segment_waits(wait + read + bar + mma + bar + mma) == ["reads"]
+    assert guard.segment_waits(read + wait + bar + mma + bar + mma) == ["mfmas"]
+    assert guard.segment_waits(mma + wait + bar + read + bar + mma) == [None]
+    assert guard.segment_waits(wait + ["s_sleep 4"] + bar + read + bar + mma) == ["sleep"]
+
+
 def test_guard_script_exit_code(built):
     assert subprocess.run(["python3", os.path.join(ROOT, "scripts", "codegen_guard.py")], capture_output=True).returncode == 0

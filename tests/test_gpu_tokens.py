@@ -511,3 +511,29 @@ def test_rows_past_two_to_the_31_elements():
     check_all(run_layer_norm(x, b, b, v), O.layer_norm(v, b, b, 1e-5, v), "layer_norm far rows")
     ops.layernorm_fwd(v, x)                             # far rows written
     O.check(x, O.layer_norm(v, None, None, 1e-5)["y"], "layer_norm into far rows")
+
+
+# One, two and a short third step a tile, more tiles than CUs: each step is read as soon as it may be.  Whole numbers whose sums f32 holds exactly, so a fragment read too early (the tile
+# before still lies in the buffer) shows as a wrong value; all three operand layouts
+@pytest.mark.parametrize("k", [64, 128, 136])
+def test_short_tiles_of_the_large_product_are_exact(k, switches):
+    switches("MIS_TOK_TILE", 2)
+    switches("MIS_TOK_SPLITS", 1)
+    dt = torch.bfloat16
+
+    def whole(g, *shape):
+        return torch.randint(-8, 9, shape, generator=g, device="cuda").to(dt)
+
+    for seed in range(3):
+        g = gen(100 * k + seed)
+        a, b = whole(g, 8200, k), whole(g, 4104, k)
+        want = (a.float() @ b.float().t()).to(dt)           # (at most 136 products of at most 64: exact)
+        y = torch.empty(8200, 4104, dtype=dt, device="cuda")
+        ops.linear_fwd(a, b, y)
+        assert torch.equal(y, want), "x w^T"
+        dx = torch.empty(8200, 4104, dtype=dt, device="cuda")
+        ops.linear_bwd(a, y, b.t().contiguous(), dx=dx)     # (x is not read for dx)
+        assert torch.equal(dx, want), "dz w"
+        dw = torch.empty(8200, 4104, dtype=dt, device="cuda")
+        ops.linear_bwd(a.t().contiguous(), b.t().contiguous(), y, dw=dw)           # (nor w for dw)
+        assert torch.equal(dw, want), "dz^T x"
