@@ -109,62 +109,6 @@ template <bool PRECISE, bool D> __device__ __forceinline__ void tok_act8(int act
     }
 }
 
-// ---- 8 values in 16 bytes with one exponent: what a bf16 forward pass keeps for its backward pass when no f32 bias gradient has to come out of it.  Value i = q_i 2^(E - 140), q_i 15 bits
-// with sign, E the biased exponent of the largest of the run: off by at most 2^-14 of that one, against 2^-9 of itself by the rounding to bf16 that follows - half the bytes of f32 for an error
-// that does not show.  Dword d: q_2d | q_2d+1 << 15 | bits 2d, 2d+1 of E << 30.  A run with an infinity or a NaN in it (E = 255) holds each value's upper 15 bits of bf16 instead: the
-// others of the run keep 7 bits, and nothing spreads. ----
-__device__ __forceinline__ u32x4 tok_run_pack(const float (&v)[8]) {
-    uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-        top = a > top ? a : top;
-    }
-    const bool fine = top < 0x7f800000u;
-    // (+ 0x200: a largest value that would round up to 2^14 takes the next exponent; below 2^-114 the step stays 2^-127)
-    int E = fine ? (int)((top + 0x200u) >> 23) : 255;
-    E = E < 13 ? 13 : (fine && E > 254 ? 254 : E);
-    uint32_t q[8];
-    if (fine) {
-        // v 2^(140 - E) + 1.5 2^23: the sum's low bits are the rounded integer in two's complement
-        const float scale = __uint_as_float((uint32_t)(267 - E) << 23);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(fmaf(v[i], scale, 12582912.f));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t u = __float_as_uint(v[i]);
-            const bool nan = (u & 0x7fffffffu) > 0x7f800000u;
-            q[i] = nan ? 0x7fe0u : (u + 0xffffu + ((u >> 17) & 1u)) >> 17;          // (round to nearest even; a NaN's payload must not round into an infinity)
-        }
-    }
-    u32x4 w;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-        const uint32_t two = (q[2 * d] & 0x7fffu) | (~0x7fffu & (q[2 * d + 1] << 15));
-        w[d] = (two & 0x3fffffffu) | (0xc0000000u & ((uint32_t)E << (30 - 2 * d)));
-    }
-    return w;
-}
-__device__ __forceinline__ void tok_run_unpack(const u32x4& w, float (&v)[8]) {
-    const int E = (int)((w[0] >> 30) | ((w[1] >> 30) << 2) | ((w[2] >> 30) << 4) | ((w[3] >> 30) << 6));
-    if (E < 255) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int u = (int)w[d];
-            v[2 * d] = ldexpf((float)((u << 17) >> 17), E - 140);
-            v[2 * d + 1] = ldexpf((float)((u << 2) >> 17), E - 140);
-        }
-    } else {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const uint32_t u = w[d];
-            v[2 * d] = __uint_as_float(u << 17);
-            v[2 * d + 1] = __uint_as_float((u << 2) & 0xfffe0000u);
-        }
-    }
-}
-
 static inline size_t tok_align(size_t n) { return (n + 255) & ~(size_t)255; }
 static inline bool tok_act_ok(int act) { return act >= MIS_ACT_NONE && act <= MIS_ACT_SIGMOID; }
 // out0[n] = sum over the nrow rows of p0[row][n], out1 the same of p1 (either out may be null), in a fixed order; nrow = 0: zeros (token_ops.hip)

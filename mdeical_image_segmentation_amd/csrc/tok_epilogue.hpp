@@ -6,13 +6,6 @@
 // where batch bt is stored (p + s (p2 - p), not s ? p2 : p: hipcc turns that into an indexed load from a scratch copy of the arguments)
 __device__ __forceinline__ char* tg_out(const TgArgs& a, int bt) { return (char*)a.y + (long long)bt * ((char*)a.y2 - (char*)a.y); }
 
-// a run's exponent is that of its values inside the matrix: behind it act'(0) or act(0) may be larger than all of them
-__device__ __forceinline__ void tg_inside(float (&v)[8], int nv) {
-    if (nv >= 8) return;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < nv ? v[j] : 0.f;
-}
-
 // y = act(v + bias) + res
 template <typename T, int ACT = -1> struct TgLinearRow {
     const TgArgs& a;
@@ -29,15 +22,8 @@ template <typename T, int ACT = -1> struct TgLinearRow {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += bias[j];
         }
-        if (a.keep == TG_KEEP_F32) tok_stn<float>(reinterpret_cast<float*>(a.kept + m * a.kept_ld) + n, v, nv);
-        if (sizeof(T) == 2 && a.keep == TG_KEEP_RUNS) {
-            float d[8];
-            tok_act8<false, true>(ACT < 0 ? a.act : ACT, v, d);
-            tg_inside(d, nv);
-            *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
-        } else {
-            tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
-        }
+        if (a.kept != nullptr) tok_stn<float>(a.kept + m * a.N + n, v, nv);
+        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, v, nullptr);
         if (a.res != nullptr) {
             float r[8];
             tok_ldn<T>(reinterpret_cast<const T*>(a.res) + m * a.ldres + n, r, nv);
@@ -66,22 +52,11 @@ template <typename T, int ACT = -1> struct TgGatedRow {
 #pragma unroll
             for (int j = 0; j < 8; ++j) u[j] += bu[j];
         }
-        if (a.keep == TG_KEEP_F32) {
-            tok_stn<float>(reinterpret_cast<float*>(a.kept + m * a.kept_ld) + n, g, nv);
-            tok_stn<float>(reinterpret_cast<float*>(a.kept2 + m * a.kept_ld) + n, u, nv);
+        if (a.kept != nullptr) {
+            tok_stn<float>(a.kept + m * a.N + n, g, nv);
+            tok_stn<float>(a.kept2 + m * a.N + n, u, nv);
         }
-        if (sizeof(T) == 2 && a.keep == TG_KEEP_RUNS) {
-            float d[8];
-            tok_act8<false, true>(ACT < 0 ? a.act : ACT, g, d);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] *= u[j];
-            tg_inside(d, nv);
-            tg_inside(g, nv);
-            *reinterpret_cast<u32x4*>(a.kept + m * a.kept_ld + n * 2) = tok_run_pack(d);
-            *reinterpret_cast<u32x4*>(a.kept2 + m * a.kept_ld + n * 2) = tok_run_pack(g);
-        } else {
-            tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, g, nullptr);
-        }
+        tok_act8<sizeof(T) == 4, false>(ACT < 0 ? a.act : ACT, g, nullptr);
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] *= u[j];
         tok_stn<T>(reinterpret_cast<T*>(a.y) + m * a.ldy + n, g, nv);

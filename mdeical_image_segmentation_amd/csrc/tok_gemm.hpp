@@ -11,8 +11,6 @@ struct TgOperand {
     long long ld;
     bool padded;            // rows end on a whole 16-byte chunk whose surplus is readable, and zero where it lies along k
 };
-// f32: the pre-activations; runs (tok_common.hpp): act'(z), or u act'(g) and act(g), the two factors of the gradients
-enum { TG_KEEP_NONE = 0, TG_KEEP_F32 = 1, TG_KEEP_RUNS = 2 };
 enum { TG_LINEAR = 0, TG_GATED = 1, TG_STORE = 2, TG_SLAB = 3 };          // epilogues: forward products; a rounded store (gradients); an f32 slab of one part of k (internal)
 struct TgArgs {
     TgOperand a, b;
@@ -26,10 +24,8 @@ struct TgArgs {
     void* y;                // [M][N]
     void* y2;
     long long ldy;
-    int keep;               // what the backward pass will read: TG_KEEP_*
-    char* kept;             // [M] rows of kept_ld bytes (gated: gate rows; the others kept2 - kept bytes further)
-    char* kept2;
-    long long kept_ld;
+    float* kept;            // [M][N] pre-activations for the backward pass (gated: kept of gate, kept2 of up), or null
+    float* kept2;
 };
 // dtype MIS_F32 | MIS_BF16; a_mn / b_mn: 1 = the operand's own index is contiguous (else k); epi TG_LINEAR, TG_GATED or TG_STORE.  Enqueues on `stream`.  A product may be cut along
 // k: its parts go to `slab` (tg_slab_bytes; null: a forward product is not cut) and are added in their order.

@@ -3,9 +3,10 @@
 //   linear:  z = x W^T + b, y = act(z) + res          dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum_rows dz
 //   gated:   g = x Wg^T + bg, u = x Wu^T + bu,        dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, biases: row sums of dg, du
 //            h = act(g) u
-// What a forward pass keeps: with biases, and in f32, the pre-activations in f32 - the bias gradients are f32 sums of dz, and 2^-9 in every term would show in them; bf16 without biases the
-// factors of dz as runs of 16 bits (tok_common.hpp).  dz (dg | du) is rounded to the operand type once, for the matrix instructions; the bias sums are taken before that rounding, per
-// block of rows, and the blocks' partial rows are added in a fixed order.
+// What a forward pass keeps: the pre-activations in f32, whatever the type.  The bias gradients are f32 sums of dz, and 2^-9 in every term would show in them; and a form of fewer bits that
+// neighbouring columns share an exponent in (8 values in 16 bytes: 32768 x 1024 x 2 x 4096 training 1724 us instead of 1858) costs a column that is small beside its neighbours its
+// gradient.  dz (dg | du) is rounded to the operand type once, for the matrix instructions; the bias sums are taken before that rounding, per block of rows, and the blocks' partial rows are
+// added in a fixed order.
 #include "tok_gemm.hpp"
 
 namespace {
@@ -20,12 +21,10 @@ inline long long to_rows(long long M) {
 inline long long to_nblk(long long M) { return (M + to_rows(M) - 1) / to_rows(M); }
 }   // namespace
 
-// Bandwidth: per value 2 bytes of dy, 2 (runs) or 4 of z, 2 of dz; gated twice the last two.  32768 x 4096 gated bf16: 1.34 GB in 303 us, 4.4 TB/s; from f32 pre-activations 1.9 GB in 412.
-// dz = dy act'(z) (MODE 0: linear), (dg | du) (MODE 1: gated), nothing but the column sums of dy (MODE 2).  RUNS: the factors are kept instead of z.  A thread: 8 columns, every 16th row
-// of its block.
-template <typename T, int MODE, bool RUNS>
-__global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, long long lddy, const char* __restrict__ kept, const char* __restrict__ kept2, long long kept_ld, int act,
-                                                     long long M, long long N, T* __restrict__ dz, long long lddz, float* __restrict__ part, float* __restrict__ part2,
+// Bandwidth: per value 2 bytes of dy, 4 of z, 2 of dz; gated twice the last two.  32768 x 4096 gated bf16: 1.9 GB in 412 us, 4.6 TB/s.
+// dz = dy act'(z) (MODE 0: linear), (dg | du) (MODE 1: gated), nothing but the column sums of dy (MODE 2).  A thread: 8 columns, every 16th row of its block.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, long long lddy, const float* __restrict__ kept, const float* __restrict__ kept2, int act, long long M, long long N, T* __restrict__ dz, long long lddz, float* __restrict__ part, float* __restrict__ part2,
                                                      long long rows, int nrb) {
     constexpr bool PRECISE = sizeof(T) == 4;
     __shared__ float red[2][16][TO_COLS];
@@ -42,31 +41,20 @@ __global__ __launch_bounds__(256) void tok_dz_kernel(const T* __restrict__ dy, l
             tok_ldn<T>(dy + m * lddy + n, d, nv);
             if constexpr (MODE == 0) {
                 float v[8], e[8];
-                if constexpr (RUNS) {
-                    tok_run_unpack(*reinterpret_cast<const u32x4*>(kept + m * kept_ld + n * 2), e);
-                } else {
-                    tok_ldn<float>(reinterpret_cast<const float*>(kept + m * kept_ld) + n, v, nv);
-                    tok_act8<PRECISE, true>(act, v, e);
-                }
+                tok_ldn<float>(kept + m * N + n, v, nv);
+                tok_act8<PRECISE, true>(act, v, e);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] *= e[i];
                 if (dz != nullptr) tok_st8<T>(dz + m * lddz + n, d);          // (a row's pitch is whole runs of 8; behind column N: zeros)
             } else if constexpr (MODE == 1) {
                 float g[8], e[8], u[8], du[8];
-                if constexpr (RUNS) {
-                    tok_run_unpack(*reinterpret_cast<const u32x4*>(kept + m * kept_ld + n * 2), e);
-                    tok_run_unpack(*reinterpret_cast<const u32x4*>(kept2 + m * kept_ld + n * 2), g);
-                } else {
-                    tok_ldn<float>(reinterpret_cast<const float*>(kept + m * kept_ld) + n, g, nv);
-                    tok_ldn<float>(reinterpret_cast<const float*>(kept2 + m * kept_ld) + n, u, nv);
-                    tok_act8<PRECISE, true>(act, g, e);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] *= u[i];
-                }
+                tok_ldn<float>(kept + m * N + n, g, nv);
+                tok_ldn<float>(kept2 + m * N + n, u, nv);
+                tok_act8<PRECISE, true>(act, g, e);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     du[i] = d[i] * g[i];
-                    d[i] = d[i] * e[i];
+                    d[i] = d[i] * (e[i] * u[i]);
                     s2[i] += du[i];
                 }
                 tok_st8<T>(dz + m * lddz + n, d);
@@ -149,31 +137,19 @@ int tok_column_sums(const float* p0, const float* p1, long long nrow, long long 
 }
 
 namespace {
-// how and where a forward pass keeps what its backward pass reads
-struct Keep {
-    int how;
-    long long ld;           // bytes of a row
-    size_t one, total;      // bytes of one of the tensors, of both
-};
-Keep keep_of(int dtype, bool biases, long long M, long long N, int tensors) {
-    const bool runs = dtype == MIS_BF16 && !biases;
-    const long long ld = runs ? (N + 7) / 8 * 16 : N * 4;
-    const size_t one = tok_align((size_t)M * ld);
-    return Keep{runs ? TG_KEEP_RUNS : TG_KEEP_F32, ld, one, one * tensors};
-}
+// bytes of one [M][N] tensor that a forward pass keeps
+size_t kept_of(long long M, long long N) { return tok_align((size_t)M * N * 4); }
 template <int MODE>
-int to_dz(int dtype, const void* dy, long long lddy, const void* kept, const Keep& k, int act, long long M, long long N, void* dz, long long lddz, float* part, float* part2,
+int to_dz(int dtype, const void* dy, long long lddy, const void* kept, int act, long long M, long long N, void* dz, long long lddz, float* part, float* part2,
           hipStream_t stream) {
     const long long rows = to_rows(M), nrb = to_nblk(M), ncb = (N + TO_COLS - 1) / TO_COLS;
     MIS_REQUIRE(nrb * ncb < (1ll << 31), MIS_EUNSUPPORTED, "token gradient: the grid is too large");
     const dim3 grid((unsigned)(nrb * ncb));
-    const char *k0 = (const char*)kept, *k1 = k0 + k.one;
-    if (dtype == MIS_BF16 && k.how == TG_KEEP_RUNS)
-        hipLaunchKernelGGL((tok_dz_kernel<__bf16, MODE, true>), grid, dim3(256), 0, stream, (const __bf16*)dy, lddy, k0, k1, k.ld, act, M, N, (__bf16*)dz, lddz, part, part2, rows, (int)nrb);
-    else if (dtype == MIS_BF16)
-        hipLaunchKernelGGL((tok_dz_kernel<__bf16, MODE, false>), grid, dim3(256), 0, stream, (const __bf16*)dy, lddy, k0, k1, k.ld, act, M, N, (__bf16*)dz, lddz, part, part2, rows, (int)nrb);
+    const float *k0 = (const float*)kept, *k1 = MODE == 1 ? (const float*)((const char*)kept + kept_of(M, N)) : nullptr;
+    if (dtype == MIS_BF16)
+        hipLaunchKernelGGL((tok_dz_kernel<__bf16, MODE>), grid, dim3(256), 0, stream, (const __bf16*)dy, lddy, k0, k1, act, M, N, (__bf16*)dz, lddz, part, part2, rows, (int)nrb);
     else
-        hipLaunchKernelGGL((tok_dz_kernel<float, MODE, false>), grid, dim3(256), 0, stream, (const float*)dy, lddy, k0, k1, k.ld, act, M, N, (float*)dz, lddz, part, part2, rows, (int)nrb);
+        hipLaunchKernelGGL((tok_dz_kernel<float, MODE>), grid, dim3(256), 0, stream, (const float*)dy, lddy, k0, k1, act, M, N, (float*)dz, lddz, part, part2, rows, (int)nrb);
     MIS_LAUNCH_CHECK("token gradient");
     return MIS_OK;
 }
@@ -301,7 +277,7 @@ int to_zero(void* p, long long ld, long long rows, long long cols, size_t es, hi
 
 extern "C" size_t mis_linear_kept_bytes(const MisLinearDesc* d) {
     if (d == nullptr || check_dims("mis_linear", d->dtype, d->act, d->M, d->N, d->K) != MIS_OK || d->act == MIS_ACT_NONE) return 0;
-    return keep_of(d->dtype, d->bias != nullptr, d->M, d->N, 1).total;
+    return kept_of(d->M, d->N);
 }
 
 extern "C" size_t mis_linear_fwd_workspace_bytes(const MisLinearDesc* d) {
@@ -326,10 +302,7 @@ extern "C" int mis_linear_fwd(const MisLinearDesc* d, void* stream_) {
     a.M = d->M; a.N = d->N; a.K = d->K;
     a.act = d->act; a.bias = d->bias; a.res = d->res; a.ldres = d->ldres;
     a.y = a.y2 = d->y; a.ldy = d->ldy;
-    if (d->kept != nullptr && d->act != MIS_ACT_NONE) {
-        const Keep k = keep_of(d->dtype, d->bias != nullptr, d->M, d->N, 1);
-        a.keep = k.how; a.kept = (char*)d->kept; a.kept_ld = k.ld;
-    }
+    if (d->act != MIS_ACT_NONE) a.kept = (float*)d->kept;
     const size_t need = mis_linear_fwd_workspace_bytes(d);
     return tg_launch(d->dtype, 0, 0, TG_LINEAR, a, need > 0 && d->workspace != nullptr && d->workspace_bytes >= need ? (float*)d->workspace : nullptr, stream);
 }
@@ -354,11 +327,10 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     const bool act = d->act != MIS_ACT_NONE, prod = d->dx != nullptr || d->dw != nullptr;
     TO_PTR(who, d->dy, "dy");
     TO_LD(who, d->lddy, d->N, "dy");
-    const Keep k = keep_of(d->dtype, d->bias != nullptr, d->M, d->N, 1);
     if (act) {
         TO_PTR(who, d->kept, "what the forward pass keeps");
         MIS_REQUIRE((uintptr_t)d->kept % 16 == 0, MIS_EINVAL, "%s: kept must be 16-byte aligned", who);
-        MIS_REQUIRE(d->dbias == nullptr || k.how == TG_KEEP_F32, MIS_EINVAL, "%s: dbias without bias", who);
+        MIS_REQUIRE(d->dbias == nullptr || d->bias != nullptr || d->dtype == MIS_F32, MIS_EINVAL, "%s: dbias without bias", who);          // (f32 calls may have it alone)
     }
     if (d->dx != nullptr) { TO_PTR(who, d->w, "w"); TO_LD(who, d->ldw, d->K, "w"); TO_LD(who, d->lddx, d->K, "dx"); }
     if (d->dw != nullptr) { TO_PTR(who, d->x, "x"); TO_LD(who, d->ldx, d->K, "x"); }
@@ -371,9 +343,9 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
     if (w.act) {
         dz = TgOperand{ws + w.dz, ws + w.dz, to_pitch(d->N), true};
         if (prod || part != nullptr)
-            TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->kept, k, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, dz.ld, part, nullptr, stream));
+            TO_TRY(to_dz<0>(d->dtype, d->dy, d->lddy, d->kept, d->act, d->M, d->N, prod ? ws + w.dz : nullptr, dz.ld, part, nullptr, stream));
     } else {
-        if (part != nullptr) TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, Keep{TG_KEEP_F32, 0, 0, 0}, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
+        if (part != nullptr) TO_TRY(to_dz<2>(d->dtype, d->dy, d->lddy, nullptr, 0, d->M, d->N, nullptr, 0, part, nullptr, stream));
         if (w.pack_dy) dz = copies.add(d->dy, d->lddy, d->M, d->N, ws + w.dz);
     }
     if (part != nullptr) TO_TRY(tok_column_sums(part, nullptr, to_nblk(d->M), d->N, d->dbias, nullptr, stream));
@@ -405,7 +377,7 @@ extern "C" int mis_linear_bwd(const MisLinearDesc* d, void* stream_) {
 
 extern "C" size_t mis_gated_ffn_kept_bytes(const MisGatedDesc* d) {
     if (d == nullptr || check_dims("mis_gated_ffn", d->dtype, d->act, d->M, d->F, d->K) != MIS_OK) return 0;
-    return keep_of(d->dtype, d->bg != nullptr || d->bu != nullptr, d->M, d->F, 2).total;
+    return 2 * kept_of(d->M, d->F);
 }
 
 extern "C" size_t mis_gated_ffn_fwd_workspace_bytes(const MisGatedDesc* d) {
@@ -430,8 +402,8 @@ extern "C" int mis_gated_ffn_fwd(const MisGatedDesc* d, void* stream_) {
     a.act = d->act; a.bias = d->bg; a.bias2 = d->bu;
     a.y = a.y2 = d->h; a.ldy = d->ldh;
     if (d->kept != nullptr) {
-        const Keep k = keep_of(d->dtype, d->bg != nullptr || d->bu != nullptr, d->M, d->F, 2);
-        a.keep = k.how; a.kept = (char*)d->kept; a.kept2 = a.kept + k.one; a.kept_ld = k.ld;
+        a.kept = (float*)d->kept;
+        a.kept2 = (float*)((char*)d->kept + kept_of(d->M, d->F));
     }
     const size_t need = mis_gated_ffn_fwd_workspace_bytes(d);
     return tg_launch(d->dtype, 0, 0, TG_GATED, a, need > 0 && d->workspace != nullptr && d->workspace_bytes >= need ? (float*)d->workspace : nullptr, stream);
@@ -461,9 +433,8 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     }
     TO_PTR(who, d->dh, "dh"); TO_PTR(who, d->kept, "what the forward pass keeps");
     TO_LD(who, d->lddh, d->F, "dh");
-    const Keep k = keep_of(d->dtype, d->bg != nullptr || d->bu != nullptr, d->M, d->F, 2);
     MIS_REQUIRE((uintptr_t)d->kept % 16 == 0, MIS_EINVAL, "%s: kept must be 16-byte aligned", who);
-    MIS_REQUIRE((d->dbg == nullptr && d->dbu == nullptr) || k.how == TG_KEEP_F32, MIS_EINVAL, "%s: dbg / dbu without bg / bu", who);
+    MIS_REQUIRE((d->dbg == nullptr && d->dbu == nullptr) || d->bg != nullptr || d->bu != nullptr || d->dtype == MIS_F32, MIS_EINVAL, "%s: dbg / dbu without bg / bu", who);
     if (d->dx != nullptr) {
         TO_PTR(who, d->wg, "wg"); TO_PTR(who, d->wu, "wu");
         TO_LD(who, d->ldw, d->K, "wg / wu"); TO_LD(who, d->lddx, d->K, "dx");
@@ -477,7 +448,7 @@ extern "C" int mis_gated_ffn_bwd(const MisGatedDesc* d, void* stream_) {
     float* const pu = d->dbu != nullptr ? (float*)(ws + w.pu) : nullptr;
     void* const dz = ws + w.dz;          // [M][dg (F, padded to pitch) | du]
     void* const du = ws + w.dz + pitch * es;
-    TO_TRY(to_dz<1>(d->dtype, d->dh, d->lddh, d->kept, k, d->act, d->M, F, dz, lddz, pg, pu, stream));
+    TO_TRY(to_dz<1>(d->dtype, d->dh, d->lddh, d->kept, d->act, d->M, F, dz, lddz, pg, pu, stream));
     if (pg != nullptr || pu != nullptr) TO_TRY(tok_column_sums(pg, pu, to_nblk(d->M), F, d->dbg, d->dbu, stream));
     TgOperand W{d->wg, d->wu, d->ldw, false}, X{d->x, d->x, d->ldx, false};
     ToCopies copies;

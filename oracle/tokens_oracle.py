@@ -87,15 +87,6 @@ def _activated(name, z, ez):
     return f, 1.13 * ez + e * 0.25, fp, efp
 
 
-def _kept(f, dy, kept):
-    """what a factor f of dz = dy f loses where the forward pass keeps it in 16 bytes for 8 values: half a step of 15 bits with sign under the largest of the 8"""
-    if not kept:
-        return 0.0
-    n = (-f.shape[1]) % 8
-    top = torch.nn.functional.pad(f.abs(), (0, n)).view(f.shape[0], -1, 8).amax(2)
-    return dy.abs() * 2.0 ** -14 * top.repeat_interleave(8, 1)[:, :f.shape[1]]
-
-
 def _back(dz, edz, h, w, x, rounded):
     """(dx, dw, db) with their bounds from dz and its bound before the rounding to the operand type"""
     e = edz + h * (dz.abs() + edz) if rounded else edz
@@ -108,7 +99,6 @@ def _back(dz, edz, h, w, x, rounded):
 
 def linear(x, w, b, name, res, dy=None):
     h = half(x.dtype)
-    runs = x.dtype == torch.bfloat16 and b is None and name not in (None, "none")
     x, w, b, res, dy = _d(x), _d(w), _d(b), _d(res), _d(dy)
     z, ez = _product(x, w, b)
     f, ef, fp, efp = _activated(name, z, ez)
@@ -117,14 +107,13 @@ def linear(x, w, b, name, res, dy=None):
     if dy is not None:
         rounded = name not in (None, "none")
         dz = dy * fp
-        out["dx"], out["dw"], out["db"] = _back(dz, dy.abs() * efp + 2 * U * dz.abs() * rounded + _kept(fp, dy, runs), h, w, x, rounded)
+        out["dx"], out["dw"], out["db"] = _back(dz, dy.abs() * efp + 2 * U * dz.abs() * rounded, h, w, x, rounded)
         out["dres"] = (dy, torch.zeros_like(dy))
     return out
 
 
 def gated(x, wg, wu, bg, bu, name, dy=None):
     h = half(x.dtype)
-    runs = x.dtype == torch.bfloat16 and bg is None and bu is None
     x, wg, wu, bg, bu, dy = _d(x), _d(wg), _d(wu), _d(bg), _d(bu), _d(dy)
     (g, eg), (u, eu) = _product(x, wg, bg), _product(x, wu, bu)
     f, ef, fp, efp = _activated(name, g, eg)
@@ -132,8 +121,8 @@ def gated(x, wg, wu, bg, bu, name, dy=None):
     out = {"y": (y, (ef * u.abs() + eu * f.abs() + ef * eu + U * y.abs()) * (1 + h) + h * y.abs())}
     if dy is not None:
         dg, du = dy * u * fp, dy * f
-        edg = dy.abs() * (u.abs() * efp + eu * fp.abs() + eu * efp) + 3 * U * dg.abs() + _kept(u * fp, dy, runs)
-        edu = dy.abs() * ef + 2 * U * du.abs() + _kept(f, dy, runs)
+        edg = dy.abs() * (u.abs() * efp + eu * fp.abs() + eu * efp) + 3 * U * dg.abs()
+        edu = dy.abs() * ef + 2 * U * du.abs()
         (dxg, exg), out["dwg"], out["dbg"] = _back(dg, edg, h, wg, x, True)
         (dxu, exu), out["dwu"], out["dbu"] = _back(du, edu, h, wu, x, True)
         # one sum over 2 F terms instead of two over F, rounded once: twice the longer bounds cover it

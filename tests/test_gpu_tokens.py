@@ -537,3 +537,55 @@ def test_short_tiles_of_the_large_product_are_exact(k, switches):
         dw = torch.empty(8200, 4104, dtype=dt, device="cuda")
         ops.linear_bwd(a.t().contiguous(), b.t().contiguous(), y, dw=dw)           # (nor w for dw)
         assert torch.equal(dw, want), "dz^T x"
+
+
+# A column's gradients against the column's own size, whatever its neighbours are: e = dz (1 + d) with |d| <= r per value gives || dw's error || <= s r || dz || + h || dw ||, s the largest
+# singular value of x, r = h + 2^-14: one rounding to the type and what f32 sums and the bf16 activations (exp2, reciprocal: a few 2^-20, at |z| <= 14) are off by
+def check_columns(got, want, dz, x, what):
+    h = O.half(x.dtype)
+    off, size = (got.double() - want).norm(dim=1), torch.linalg.matrix_norm(x.double(), 2) * (h + 2.0 ** -14) * dz.norm(dim=0) + h * want.norm(dim=1)
+    bad = ~(off <= size)
+    assert not bad.any(), f"{what}: columns {bad.nonzero().flatten().tolist()[:8]}, errors {(off / want.norm(dim=1))[bad].tolist()[:8]} of their own size"
+
+
+@pytest.mark.parametrize("bits", [4, 8, 10, 12, 14, 17, 20])
+@pytest.mark.parametrize("loud", [False, True])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", None])
+def test_gradients_of_a_quiet_column_beside_loud_ones(bits, loud, act):
+    # one column of the up projection 2^-bits of its neighbours, or 2^bits of them
+    g = gen(bits)
+    dt = torch.bfloat16
+    x, wg, wu, dy = randn(g, 512, 64, dtype=dt), randn(g, 19, 64, dtype=dt, scale=0.125), randn(g, 19, 64, dtype=dt, scale=0.125), randn(g, 512, 19, dtype=dt)
+    for i in (5, 17):
+        wu[i] *= 2.0 ** (bits if loud else -bits)
+    got = run_gated(x, wg, wu, None, None, act, dy)
+    z, u, d = x.double() @ wg.double().t(), x.double() @ wu.double().t(), dy.double()
+    f, fp = O.act(act, z)
+    dg, du = d * u * fp, d * f
+    check_columns(got["dwg"], dg.t() @ x.double(), dg, x, "dwg")
+    check_columns(got["dwu"], du.t() @ x.double(), du, x, "dwu")
+    check_all(got, O.gated(x, wg, wu, None, None, act, dy), "gated")
+
+
+@pytest.mark.parametrize("z", [-7.0, -9.0, -12.0])
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_gradients_of_a_saturated_unit_beside_ordinary_ones(act, z):
+    g = gen(41)
+    dt = torch.bfloat16
+    x, w, dy = randn(g, 512, 64, dtype=dt), randn(g, 19, 64, dtype=dt, scale=0.02), randn(g, 512, 19, dtype=dt)
+    x[:, 0] = 1.0
+    for i in (2, 18):
+        w[i, 0] = z
+    got = run_linear(x, w, None, act, None, dy)
+    dz = dy.double() * O.act(act, x.double() @ w.double().t())[1]
+    check_columns(got["dw"], dz.t() @ x.double(), dz, x, "dw")
+    check_all(got, O.linear(x, w, None, act, None, dy), "linear")
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_the_largest_values_keep_their_sign(sign):
+    # u = (2^128 - 2^120) + (2^120 - 2^112), the largest sum of two bf16 values; dh = 2^-20, so that no gradient overflows (h does)
+    dt = torch.bfloat16
+    x, wg, dy = torch.ones(4, 2, dtype=dt, device="cuda"), torch.ones(9, 2, dtype=dt, device="cuda"), torch.full((4, 9), 2.0 ** -20, dtype=dt, device="cuda")
+    wu = (sign * torch.tensor([2.0 ** 128 - 2.0 ** 120, 2.0 ** 120 - 2.0 ** 112], dtype=torch.float64, device="cuda")).to(dt).expand(9, 2).contiguous()
+    check_all({k: v for k, v in run_gated(x, wg, wu, None, None, None, dy).items() if k != "y"}, O.gated(x, wg, wu, None, None, None, dy), "gated")
