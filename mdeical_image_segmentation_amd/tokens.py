@@ -5,7 +5,7 @@
     y = linear(h, w_down, residual=x)               # h w_down^T + x, one kernel
 
 x is (..., width) with any number of leading dimensions, float32 or bfloat16; weights are (out, width) as in nn.Linear, in x's type; biases and norm parameters are float32.  Each
-function is differentiable once (forward and backward are HIP kernels of libmisamd; torch is the allocator and the tape) and keeps what its backward pass needs only when a gradient is
+function is differentiable once, in reverse mode (forward and backward are HIP kernels of libmisamd; torch is the allocator and the tape) and keeps what its backward pass needs only when a gradient is
 wanted.  Work is enqueued on torch's current stream of x's device; workspaces come from the caching allocator call by call, so streams and captured graphs share none.  Under stream
 capture take gradients with torch.autograd.grad, or call the ops.*_bwd functions.  There is no CPU path: a tensor that is not on the GPU raises.
 
@@ -14,6 +14,7 @@ host: the functions here fill the C descriptors directly, with the checks inline
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad as _fw
 from torch.autograd.function import once_differentiable
 
 from ._lib import MIS_BF16, MIS_F32, GatedDesc, LinearDesc, MisError, check, load
@@ -100,8 +101,12 @@ def _scratch(nbytes, x):
     return torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
 
 
-def _wanted(*ts):
-    """whether a gradient is (what is not a tensor is refused by the forward pass's checks)"""
+def _wanted(who, *ts):
+    """whether a gradient is (what is not a tensor is refused by the forward pass's checks); a forward-mode tangent, which the kernels would drop, is refused"""
+    if _fw._current_level >= 0:
+        for t in ts:
+            if isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None:
+                _refuse(who, f"differentiable in reverse mode only, got a tensor with a forward-mode tangent: {_say(t)}")
     if torch.is_grad_enabled():
         for t in ts:
             if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -167,7 +172,7 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension; weight, bias (width,) float32 or None"""
-    if _wanted(x, weight, bias):
+    if _wanted("layer_norm", x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _norm_fwd(x, weight, bias, float(eps), False)[1]
 
@@ -234,7 +239,7 @@ class _Linear(torch.autograd.Function):
 def linear(x, weight, bias=None, activation=None, residual=None):
     """activation(x weight^T + bias) + residual; activation None | 'relu' | 'gelu' | 'gelu_tanh' | 'silu' | 'sigmoid', residual with the result's shape"""
     act = token_act(activation)
-    if _wanted(x, weight, bias, residual):
+    if _wanted("linear", x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, act, residual)
     return _linear_fwd(x, weight, bias, act, residual, False)[2]
 
@@ -296,6 +301,6 @@ class _GatedFFN(torch.autograd.Function):
 def gated_ffn(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """activation(x w_gate^T + b_gate) * (x w_up^T + b_up); w_gate, w_up (features, width), activation 'silu' | 'gelu' | 'gelu_tanh' | 'relu' | 'sigmoid' | None"""
     act = token_act(activation)
-    if _wanted(x, w_gate, w_up, b_gate, b_up):
+    if _wanted("gated_ffn", x, w_gate, w_up, b_gate, b_up):
         return _GatedFFN.apply(x, w_gate, w_up, b_gate, b_up, act)
     return _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, False)[3]

@@ -151,3 +151,25 @@ def test_oracle_gradients_are_torchs(name):
     o = O.layer_norm(r, gam, bet, 1e-5, dz)
     for got, want in zip((y, *torch.autograd.grad(y, (r, gam, bet), dz)), (o["y"], o["dx"], o["dw"], o["db"])):
         torch.testing.assert_close(want[0], got.detach(), rtol=1e-12, atol=1e-12)
+
+
+# a tangent would vanish behind the data pointers: refused, with gradients on or off, for every argument that may carry one
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call", [
+    lambda x, w, b, d: tokens.layer_norm(d(x)), lambda x, w, b, d: tokens.layer_norm(x, d(x[0])), lambda x, w, b, d: tokens.layer_norm(x, None, d(x[0])), lambda x, w, b, d: tokens.linear(d(x), w),
+    lambda x, w, b, d: tokens.linear(x, d(w)), lambda x, w, b, d: tokens.linear(x, w, d(b)), lambda x, w, b, d: tokens.linear(x, w, residual=d(x @ w.t())), lambda x, w, b, d: tokens.gated_ffn(d(x), w, w),
+    lambda x, w, b, d: tokens.gated_ffn(x, d(w), w), lambda x, w, b, d: tokens.gated_ffn(x, w, d(w)), lambda x, w, b, d: tokens.gated_ffn(x, w, w, d(b)), lambda x, w, b, d: tokens.gated_ffn(x, w, w, None, d(b))])
+def test_forward_mode_tangents_are_refused(call, grad):
+    import torch.autograd.forward_ad as fw
+    x, w, b = torch.randn(4, 8), torch.randn(6, 8), torch.randn(6)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        with pytest.raises(MisError, match="tangent"):
+            call(x, w, b, lambda t: fw.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(MisError, match="MI355X"):           # without one: the ordinary checks
+            call(x, w, b, lambda t: t)
+
+
+def test_jvp_of_a_token_operator_is_refused():
+    x, w = torch.randn(4, 8), torch.randn(6, 8)
+    with pytest.raises(MisError, match="tangent"):
+        torch.func.jvp(lambda t: tokens.linear(t, w), (x,), (torch.ones_like(x),))
