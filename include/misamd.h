@@ -599,7 +599,8 @@ int mis_comm_finalize(void);
  * Rows: from 0 (a forward call then does nothing, a backward call writes zero parameter gradients) to below 2^31.  Outputs must not overlap inputs.
  * Workspaces belong to the call until the stream has passed it.  Sums have a fixed order: equal calls give equal bits. */
 
-/* y = (x - mean) * rstd * gamma + beta over each row's D values, rstd = 1 / sqrt(var + eps); gamma / beta NULL: 1 / 0; mean / rstd ([M] f32) NULL: not kept */
+/* (layer norm: D up to 2^22)
+ * y = (x - mean) * rstd * gamma + beta over each row's D values, rstd = 1 / sqrt(var + eps); gamma / beta NULL: 1 / 0; mean / rstd ([M] f32) NULL: not kept */
 int mis_layernorm_fwd(int dtype, const void* x, long long ldx, long long M, int D, float eps, const float* gamma, const float* beta, void* y, long long ldy, float* mean, float* rstd,
                       void* stream);
 size_t mis_layernorm_bwd_workspace_bytes(int dtype, long long M, int D);

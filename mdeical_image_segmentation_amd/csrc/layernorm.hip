@@ -303,9 +303,11 @@ __global__ __launch_bounds__(LN_THREADS) void ln_bwd_param_kernel(const T* __res
 }
 
 namespace {
-inline long long ln_rows(long long M) {
+// a grid holds fewer than 2^32 work-items: kernels that give every row its lanes are launched again behind this many
+constexpr long long LN_ITEMS = 1ll << 31;
+inline long long ln_rows(long long M, int D) {
     long long r = 64;
-    while ((M + r - 1) / r > 512) r *= 2;
+    while ((M + r - 1) / r > 512 || (M + r - 1) / r * ((D + 63) / 64) * LN_THREADS > LN_ITEMS) r *= 2;
     return r;
 }
 // lanes per row and runs per lane that a width takes; 0: the kernels for any width
@@ -317,7 +319,7 @@ inline int ln_runs(int D) { return (D + 8 * ln_lanes(D) - 1) / (8 * ln_lanes(D))
 constexpr int LN_PART = 512, LN_PART_LIGHT = 1024;
 inline long long ln_parts(int dtype, long long M, int D) {
     const int n = ln_lanes(D);
-    if (n == 0) return (M + ln_rows(M) - 1) / ln_rows(M);
+    if (n == 0) return (M + ln_rows(M, D) - 1) / ln_rows(M, D);
     const long long blocks = (M * n + 255) / 256, most = D <= 256 || (dtype == MIS_BF16 && ln_runs(D) <= 2) ? LN_PART_LIGHT : LN_PART;
     return blocks < most ? blocks : most;
 }
@@ -330,41 +332,65 @@ template <typename T, typename F> int ln_by_width(int D, F&& f) {
     if (w == 64) return n == 1 ? f(ln_int<64>{}, ln_int<1>{}) : n == 2 ? f(ln_int<64>{}, ln_int<2>{}) : n == 3 ? f(ln_int<64>{}, ln_int<3>{}) : f(ln_int<64>{}, ln_int<4>{});
     return n == 2 ? f(ln_int<256>{}, ln_int<2>{}) : n == 3 ? f(ln_int<256>{}, ln_int<3>{}) : f(ln_int<256>{}, ln_int<4>{});          // (one run of a block: up to 2048, which a wave takes)
 }
+// f(first row, rows) for as many rows at a time as one grid of L lanes a row holds
+template <int L, typename F> int ln_by_rows(long long M, F&& f) {
+    for (long long r = 0; r < M; r += LN_ITEMS / L)
+        if (const int rc = f(r, M - r < LN_ITEMS / L ? M - r : LN_ITEMS / L)) return rc;
+    return MIS_OK;
+}
 template <typename T>
-int ln_fwd(const void* x, long long ldx, long long M, int D, float eps, const float* gamma, const float* beta, void* y, long long ldy, float* mean, float* rstd, hipStream_t stream) {
-    if (ln_lanes(D) == 0) {
-        hipLaunchKernelGGL((ln_fwd_kernel<T>), dim3((unsigned)M), dim3(LN_THREADS), 0, stream, (const T*)x, ldx, D, eps, gamma, beta, (T*)y, ldy, mean, rstd);
-        return MIS_OK;
-    }
+int ln_fwd(const void* x_, long long ldx, long long M, int D, float eps, const float* gamma, const float* beta, void* y_, long long ldy, float* mean, float* rstd, hipStream_t stream) {
+    const T* const x = (const T*)x_;
+    T* const y = (T*)y_;
+    auto at = [](float* p, long long r) { return p != nullptr ? p + r : nullptr; };
+    if (ln_lanes(D) == 0)
+        return ln_by_rows<LN_THREADS>(M, [&](long long r, long long rows) {
+            hipLaunchKernelGGL((ln_fwd_kernel<T>), dim3((unsigned)rows), dim3(LN_THREADS), 0, stream, x + r * ldx, ldx, D, eps, gamma, beta, y + r * ldy, ldy, at(mean, r), at(rstd, r));
+            MIS_LAUNCH_CHECK("mis_layernorm_fwd");
+            return (int)MIS_OK;
+        });
     return ln_by_width<T>(D, [&](auto w, auto n) {
         constexpr int L = decltype(w)::value, NV = decltype(n)::value;
-        hipLaunchKernelGGL((ln_fwd_row_kernel<T, L, NV>), dim3((unsigned)((M * L + 255) / 256)), dim3(LN_THREADS), 0, stream, (const T*)x, ldx, M, D, eps, gamma, beta, (T*)y, ldy,
-                           mean, rstd);
-        return MIS_OK;
+        return ln_by_rows<L>(M, [&](long long r, long long rows) {
+            hipLaunchKernelGGL((ln_fwd_row_kernel<T, L, NV>), dim3((unsigned)((rows * L + 255) / 256)), dim3(LN_THREADS), 0, stream, x + r * ldx, ldx, rows, D, eps, gamma, beta, y + r * ldy, ldy,
+                               at(mean, r), at(rstd, r));
+            MIS_LAUNCH_CHECK("mis_layernorm_fwd");
+            return (int)MIS_OK;
+        });
     });
 }
 template <typename T>
-int ln_bwd(const void* dy, long long lddy, const void* x, long long ldx, long long M, int D, const float* gamma, const float* mean, const float* rstd, void* dx, long long lddx, float* pg,
+int ln_bwd(const void* dy_, long long lddy, const void* x_, long long ldx, long long M, int D, const float* gamma, const float* mean, const float* rstd, void* dx_, long long lddx, float* pg,
            float* pb, hipStream_t stream) {
+    const T *const dy = (const T*)dy_, *const x = (const T*)x_;
+    T* const dx = (T*)dx_;
     const long long parts = ln_parts(sizeof(T) == 2 ? MIS_BF16 : MIS_F32, M, D);
     if (ln_lanes(D) == 0) {
         if (dx != nullptr)
-            hipLaunchKernelGGL((ln_bwd_dx_kernel<T>), dim3((unsigned)M), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, D, gamma, mean, rstd, (T*)dx, lddx);
+            if (const int rc = ln_by_rows<LN_THREADS>(M, [&](long long r, long long rows) {
+                    hipLaunchKernelGGL((ln_bwd_dx_kernel<T>), dim3((unsigned)rows), dim3(LN_THREADS), 0, stream, dy + r * lddy, lddy, x + r * ldx, ldx, D, gamma, mean + r, rstd + r,
+                                       dx + r * lddx, lddx);
+                    MIS_LAUNCH_CHECK("mis_layernorm_bwd");
+                    return (int)MIS_OK;
+                }))
+                return rc;
         if (pg != nullptr || pb != nullptr)
-            hipLaunchKernelGGL((ln_bwd_param_kernel<T>), dim3((unsigned)(parts * ((D + 63) / 64))), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, M, D, mean, rstd, pg, pb,
-                               ln_rows(M), (int)parts);
+            hipLaunchKernelGGL((ln_bwd_param_kernel<T>), dim3((unsigned)(parts * ((D + 63) / 64))), dim3(LN_THREADS), 0, stream, dy, lddy, x, ldx, M, D, mean, rstd, pg, pb, ln_rows(M, D),
+                               (int)parts);
+        MIS_LAUNCH_CHECK("mis_layernorm_bwd");
         return MIS_OK;
     }
     return ln_by_width<T>(D, [&](auto w, auto n) {
         constexpr int L = decltype(w)::value, NV = decltype(n)::value;
-        hipLaunchKernelGGL((ln_bwd_row_kernel<T, L, NV>), dim3((unsigned)parts), dim3(LN_THREADS), 0, stream, (const T*)dy, lddy, (const T*)x, ldx, M, D, gamma, mean, rstd, (T*)dx, lddx, pg, pb);
-        return MIS_OK;
+        hipLaunchKernelGGL((ln_bwd_row_kernel<T, L, NV>), dim3((unsigned)parts), dim3(LN_THREADS), 0, stream, dy, lddy, x, ldx, M, D, gamma, mean, rstd, dx, lddx, pg, pb);
+        MIS_LAUNCH_CHECK("mis_layernorm_bwd");
+        return (int)MIS_OK;
     });
 }
 int ln_check(const char* who, int dtype, long long M, int D) {
     MIS_REQUIRE(dtype == MIS_F32 || dtype == MIS_BF16, MIS_EINVAL, "%s: dtype must be MIS_F32 or MIS_BF16", who);
     MIS_REQUIRE(M >= 0 && D >= 1, MIS_EINVAL, "%s: needs rows >= 0 and a width >= 1 (got %lld, %d)", who, M, D);
-    MIS_REQUIRE(M < (1ll << 31), MIS_EUNSUPPORTED, "%s: %lld rows are more than a grid holds", who, M);
+    MIS_REQUIRE(M < (1ll << 31), MIS_EUNSUPPORTED, "%s: %lld rows are more than its grids hold", who, M);
     MIS_REQUIRE(D <= (1 << 22), MIS_EUNSUPPORTED, "%s: width %d is over 2^22", who, D);
     return MIS_OK;
 }
@@ -377,10 +403,7 @@ extern "C" int mis_layernorm_fwd(int dtype, const void* x, long long ldx, long l
     MIS_REQUIRE(x != nullptr && y != nullptr, MIS_EINVAL, "mis_layernorm_fwd: null pointer");
     MIS_REQUIRE(ldx >= D && ldy >= D, MIS_EINVAL, "mis_layernorm_fwd: a row stride is below the width");
     const hipStream_t s = (hipStream_t)stream;
-    if (dtype == MIS_BF16) ln_fwd<__bf16>(x, ldx, M, D, eps, gamma, beta, y, ldy, mean, rstd, s);
-    else ln_fwd<float>(x, ldx, M, D, eps, gamma, beta, y, ldy, mean, rstd, s);
-    MIS_LAUNCH_CHECK("mis_layernorm_fwd");
-    return MIS_OK;
+    return dtype == MIS_BF16 ? ln_fwd<__bf16>(x, ldx, M, D, eps, gamma, beta, y, ldy, mean, rstd, s) : ln_fwd<float>(x, ldx, M, D, eps, gamma, beta, y, ldy, mean, rstd, s);
 }
 
 extern "C" size_t mis_layernorm_bwd_workspace_bytes(int dtype, long long M, int D) {
@@ -402,9 +425,9 @@ extern "C" int mis_layernorm_bwd(int dtype, const void* dy, long long lddy, cons
     float* const pg = dgamma != nullptr ? (float*)workspace : nullptr;
     float* const pb = dbeta != nullptr ? (float*)((char*)workspace + half) : nullptr;
     if (M > 0 && (params || dx != nullptr)) {
-        if (dtype == MIS_BF16) ln_bwd<__bf16>(dy, lddy, x, ldx, M, D, gamma, mean, rstd, dx, lddx, pg, pb, stream);
-        else ln_bwd<float>(dy, lddy, x, ldx, M, D, gamma, mean, rstd, dx, lddx, pg, pb, stream);
-        MIS_LAUNCH_CHECK("mis_layernorm_bwd");
+        const int rc = dtype == MIS_BF16 ? ln_bwd<__bf16>(dy, lddy, x, ldx, M, D, gamma, mean, rstd, dx, lddx, pg, pb, stream)
+                                         : ln_bwd<float>(dy, lddy, x, ldx, M, D, gamma, mean, rstd, dx, lddx, pg, pb, stream);
+        if (rc != MIS_OK) return rc;
     }
     // (no rows: the sums are over nothing and the gradients zero)
     if (params) return tok_column_sums(pg, pb, parts, D, dgamma, dbeta, stream);

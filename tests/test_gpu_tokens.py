@@ -589,3 +589,27 @@ def test_the_largest_values_keep_their_sign(sign):
     x, wg, dy = torch.ones(4, 2, dtype=dt, device="cuda"), torch.ones(9, 2, dtype=dt, device="cuda"), torch.full((4, 9), 2.0 ** -20, dtype=dt, device="cuda")
     wu = (sign * torch.tensor([2.0 ** 128 - 2.0 ** 120, 2.0 ** 120 - 2.0 ** 112], dtype=torch.float64, device="cuda")).to(dt).expand(9, 2).contiguous()
     check_all({k: v for k, v in run_gated(x, wg, wu, None, None, None, dy).items() if k != "y"}, O.gated(x, wg, wu, None, None, None, dy), "gated")
+
+
+def far_rows(g, M, D, rows, dtype):
+    """(M, D) of zeros but for the given rows"""
+    t = torch.zeros(M, D, dtype=dtype, device="cuda")
+    t[rows] = randn(g, len(rows), D, dtype=dtype)
+    return t
+
+
+# more lanes than one grid holds: 2^32 work-items lie at 2^29 rows of up to 64 values and at 2^26 rows of 257 to 2048.  Rows of zeros but for some at the start, around the borders and at the end
+@pytest.mark.parametrize("M, D, borders", [((1 << 29) + 5, 2, (1 << 28, 1 << 29)), ((1 << 26) + 3, 257, (1 << 25, 1 << 26))])
+def test_layer_norm_of_more_rows_than_a_grid_holds(M, D, borders):
+    g = gen(51)
+    rows = torch.tensor([0, 1, 70] + [b + i for b in borders for i in (-33, -1, 0, 1)] + [M - 2, M - 1], device="cuda")
+    x, w, b = far_rows(g, M, D, rows, torch.bfloat16), randn(g, D) + 2, randn(g, D)
+    dy = far_rows(g, M, D, rows, torch.bfloat16)
+    rows = rows.unique()                                        # (one of them is named twice: its row counts once)
+    got = run_layer_norm(x, w, b, dy)
+    want = O.layer_norm(x[rows], w, b, 1e-5, dy[rows])          # (a row of zeros has no part in the sums)
+    check_all({"y": got["y"][rows], "dx": got["dx"][rows], "dw": got["dw"], "db": got["db"]}, want, "layer_norm of many rows")
+    others = torch.tensor([5, borders[0] + 99, borders[1] - 99], device="cuda")
+    assert torch.equal(got["y"][others], b.bfloat16().expand(3, D)) and (got["dx"][others] == 0).all()
+    del x, dy, got
+    torch.cuda.empty_cache()
