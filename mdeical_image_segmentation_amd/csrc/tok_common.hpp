@@ -109,6 +109,7 @@ template <bool PRECISE, bool D> __device__ __forceinline__ void tok_act8(int act
     }
 }
 
+constexpr long long TOK_BLOCKS = 1ll << 24;          // blocks of 256 threads: a grid holds fewer than 2^32 work-items, and HIP cuts a larger one without an error
 static inline size_t tok_align(size_t n) { return (n + 255) & ~(size_t)255; }
 static inline bool tok_act_ok(int act) { return act >= MIS_ACT_NONE && act <= MIS_ACT_SIGMOID; }
 // out0[n] = sum over the nrow rows of p0[row][n], out1 the same of p1 (either out may be null), in a fixed order; nrow = 0: zeros (token_ops.hip)

@@ -57,7 +57,7 @@ template <typename T> void tg_slab_go(int epi, unsigned blocks, const TgSum& s, 
 }
 int tg_slab_sum(int dtype, int epi, const TgSum& s, hipStream_t stream) {
     const long long n = (s.runs + 255) / 256;
-    MIS_REQUIRE(n < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
+    MIS_REQUIRE(n < TOK_BLOCKS, MIS_EUNSUPPORTED, "token product: the grid is too large");
     if (dtype == MIS_BF16) tg_slab_go<__bf16>(epi, (unsigned)n, s, stream);
     else tg_slab_go<float>(epi, (unsigned)n, s, stream);
     MIS_LAUNCH_CHECK("token product (sum of k parts)");
@@ -69,7 +69,7 @@ int tg_sums(int dtype, const TgSum& s, const TgSum& t, hipStream_t stream) {
     if (s.slab == nullptr && t.slab == nullptr) return MIS_OK;
     if (s.slab == nullptr || t.slab == nullptr) return tg_slab_sum(dtype, TG_STORE, s.slab != nullptr ? s : t, stream);
     const long long n0 = (s.runs + 255) / 256, n1 = (t.runs + 255) / 256;
-    MIS_REQUIRE(n0 + n1 < (1ll << 31), MIS_EUNSUPPORTED, "token product: the grid is too large");
+    MIS_REQUIRE(n0 + n1 < TOK_BLOCKS, MIS_EUNSUPPORTED, "token product: the grid is too large");
     if (dtype == MIS_BF16) hipLaunchKernelGGL(tg_slab2_kernel<__bf16>, dim3((unsigned)(n0 + n1)), dim3(256), 0, stream, s, t, (unsigned)n0);
     else hipLaunchKernelGGL(tg_slab2_kernel<float>, dim3((unsigned)(n0 + n1)), dim3(256), 0, stream, s, t, (unsigned)n0);
     MIS_LAUNCH_CHECK("token product (sums of k parts)");
@@ -143,11 +143,12 @@ TgCut tg_cut_of(int dtype, bool aligned, int epi, bool slab, long long M, long l
     const TgCut parts = tg_cut(dtype, aligned, true, M, N, K, 1, epi == TG_GATED ? 2 : 1, false);
     return parts.splits > 1 && parts.us < 0.9 * whole.us ? parts : whole;
 }
-bool tg_few_rows(int epi, long long M) { return epi != TG_STORE && M <= 32 && mis_sw(SW_TOK_TILE) == 0; }
+// (the weights' kernel gives every 16 or 32 columns a block: up to 2^29 columns its grid holds them)
+bool tg_few_rows(int epi, long long M, long long N) { return epi != TG_STORE && M <= 32 && N <= (1ll << 29) && mis_sw(SW_TOK_TILE) == 0; }
 }   // namespace
 
 size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, int ranges, int batches) {
-    if (M == 0 || tg_few_rows(epi, M)) return 0;
+    if (M == 0 || tg_few_rows(epi, M, N)) return 0;
     size_t most = 0;
     for (int al = 0; al < 2; ++al) {
         const TgCut c = tg_cut_of(dtype, al == 1, epi, true, M, N, K, ranges, batches);
@@ -159,14 +160,14 @@ size_t tg_slab_bytes(int dtype, int epi, long long M, long long N, long long K, 
 
 int tg_launch(int dtype, int a_mn, int b_mn, int epi_, const TgArgs& args, float* slab, hipStream_t stream, TgSum* later) {
     const bool al = tg_aligned(dtype, args, a_mn, b_mn);
-    if (tg_few_rows(epi_, args.M)) return tok_product_skinny(dtype, epi_, args, al, stream);
+    if (tg_few_rows(epi_, args.M, args.N)) return tok_product_skinny(dtype, epi_, args, al, stream);
     const TgCut c = tg_cut_of(dtype, al, epi_, slab != nullptr, args.M, args.N, args.K, args.ranges, args.batches);
     TgArgs a = args;
     if (epi_ == TG_GATED && c.splits > 1) a.batches = 2;
     const int epi = c.splits > 1 ? TG_SLAB : epi_;
     const long long T = c.tile, BN = epi == TG_GATED ? (T == 256 ? 128 : 64) : T, ck = dtype == MIS_BF16 ? 64 : 32;
     const long long tm = (a.M + T - 1) / T, tn = (a.N + BN - 1) / BN, spr = (a.K + ck - 1) / ck;
-    MIS_REQUIRE(tm < (1ll << 24) && tn < (1ll << 24) && spr < (1ll << 28) && tm * tn * a.batches * c.splits < (1ll << 30), MIS_EUNSUPPORTED,
+    MIS_REQUIRE(tm < (1ll << 26) && tn < (1ll << 26) && spr < (1ll << 28) && tm * tn * a.batches * c.splits < (1ll << 30), MIS_EUNSUPPORTED,
                 "token product: %lld x %lld tiles of %lld steps are too many", tm, tn, spr);
     TpPlan pl;
     pl.tm = (int)tm; pl.tn = (int)tn;

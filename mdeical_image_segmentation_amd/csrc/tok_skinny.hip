@@ -131,8 +131,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void tok_skinny_kernel(const 
 namespace {
 template <typename T, int NT, int MT, bool GATED, bool AL> int sk_go(const TgArgs& a, hipStream_t stream) {
     const long long cols = GATED ? 16 : 16 * NT, blocks = (a.N + cols - 1) / cols, units = (a.K + 8 * Tr<T>::EPC - 1) / (8 * Tr<T>::EPC);
-    MIS_REQUIRE(blocks < (1ll << 31), MIS_EUNSUPPORTED, "token product: %lld columns are more than a grid holds", a.N);
-    int W = 1;
+    int W = 1;          // (at most 2^25 blocks: tg_few_rows)
     while (W < (MT == 1 ? 16 : 8) && blocks * W < 2048 && 2 * W <= units) W *= 2;
     hipLaunchKernelGGL((tok_skinny_kernel<T, NT, MT, GATED, AL>), dim3((unsigned)blocks), dim3(64 * W), (size_t)W * NT * MT * 1024, stream, a);
     MIS_LAUNCH_CHECK("token product (few rows)");

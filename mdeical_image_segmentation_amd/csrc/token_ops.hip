@@ -101,14 +101,14 @@ template <typename T> __global__ __launch_bounds__(256) void tok_pack_kernel(con
 
 // Column sums of up to a few hundred partial rows: 16 row groups a block, so that a thread adds some 32 values with 8 loads in flight (four groups of 256 threads took 39 us for
 // 512 x 1024 partial rows, this one 5)
-__global__ __launch_bounds__(1024) void tok_colsum_kernel(const float* __restrict__ p0, const float* __restrict__ p1, long long nrow, long long N, float* __restrict__ out0,
-                                                          float* __restrict__ out1) {
+__global__ __launch_bounds__(1024) void tok_colsum_kernel(const float* __restrict__ p0, const float* __restrict__ p1, long long nrow, long long N, long long col0,
+                                                          float* __restrict__ out0, float* __restrict__ out1) {
     __shared__ float red[16][64];
     const float* const part = blockIdx.y == 0 ? p0 : p1;
     float* const out = blockIdx.y == 0 ? out0 : out1;
     if (out == nullptr) return;                              // (block-uniform)
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const long long n = (long long)blockIdx.x * 64 + c;
+    const long long n = (col0 + blockIdx.x) * 64 + c;
     float s = 0.f;
     if (n < N) {
         long long r = g;
@@ -131,8 +131,11 @@ __global__ __launch_bounds__(1024) void tok_colsum_kernel(const float* __restric
 }
 
 int tok_column_sums(const float* p0, const float* p1, long long nrow, long long N, float* out0, float* out1, hipStream_t stream) {
-    hipLaunchKernelGGL(tok_colsum_kernel, dim3((unsigned)((N + 63) / 64), out1 != nullptr ? 2 : 1), dim3(1024), 0, stream, p0, p1, nrow, N, out0, out1);
-    MIS_LAUNCH_CHECK("token column sums");
+    constexpr long long most = TOK_BLOCKS / 8;          // (2 x 1024 threads for 64 columns: 2^27 columns at a time)
+    for (long long col0 = 0, all = (N + 63) / 64; col0 < all; col0 += most) {
+        hipLaunchKernelGGL(tok_colsum_kernel, dim3((unsigned)(all - col0 < most ? all - col0 : most), out1 != nullptr ? 2 : 1), dim3(1024), 0, stream, p0, p1, nrow, N, col0, out0, out1);
+        MIS_LAUNCH_CHECK("token column sums");
+    }
     return MIS_OK;
 }
 
@@ -143,7 +146,7 @@ template <int MODE>
 int to_dz(int dtype, const void* dy, long long lddy, const void* kept, int act, long long M, long long N, void* dz, long long lddz, float* part, float* part2,
           hipStream_t stream) {
     const long long rows = to_rows(M), nrb = to_nblk(M), ncb = (N + TO_COLS - 1) / TO_COLS;
-    MIS_REQUIRE(nrb * ncb < (1ll << 31), MIS_EUNSUPPORTED, "token gradient: the grid is too large");
+    MIS_REQUIRE(nrb * ncb < TOK_BLOCKS, MIS_EUNSUPPORTED, "token gradient: the grid is too large");
     const dim3 grid((unsigned)(nrb * ncb));
     const float *k0 = (const float*)kept, *k1 = MODE == 1 ? (const float*)((const char*)kept + kept_of(M, N)) : nullptr;
     if (dtype == MIS_BF16)

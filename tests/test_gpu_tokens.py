@@ -613,3 +613,38 @@ def test_layer_norm_of_more_rows_than_a_grid_holds(M, D, borders):
     assert torch.equal(got["y"][others], b.bfloat16().expand(3, D)) and (got["dx"][others] == 0).all()
     del x, dy, got
     torch.cuda.empty_cache()
+
+
+def test_products_of_more_than_two_to_the_30_rows():
+    g = gen(52)
+    M, dt = (1 << 30) + 70, torch.bfloat16
+    rows = torch.tensor([0, 65, (1 << 29) - 1, 1 << 29, (1 << 30) - 1, 1 << 30, (1 << 30) + 63, M - 6, M - 1], device="cuda")
+    x, w, v, b = far_rows(g, M, 2, rows, dt), randn(g, 1, 2, dtype=dt), randn(g, 1, 2, dtype=dt), randn(g, 1)
+    dy = far_rows(g, M, 1, rows, dt)
+    got = run_linear(x, w, b, None, None, dy)
+    check_all({"y": got["y"][rows], "dx": got["dx"][rows], "dw": got["dw"], "db": got["db"]}, O.linear(x[rows], w, b, None, None, dy[rows]), "linear of many rows")
+    others = torch.tensor([7, (1 << 30) + 9, M - 2], device="cuda")
+    assert (got["y"][others] == b.bfloat16()).all() and (got["dx"][others] == 0).all()
+    del got
+    with torch.no_grad():
+        h = tokens.gated_ffn(x, w, v, b, None)
+    O.check(h[rows], O.gated(x[rows], w, v, b, None, "silu")["y"], "gated of many rows")
+    del x, dy, h
+    torch.cuda.empty_cache()
+
+
+def test_products_of_more_than_two_to_the_30_columns():
+    g = gen(53)
+    N, dt = (1 << 30) + 16, torch.bfloat16
+    cols = torch.tensor([0, 8, (1 << 27) - 1, 1 << 27, (1 << 28) + 3, (1 << 29) - 1, 1 << 29, (1 << 30) - 1, 1 << 30, N - 1], device="cuda")
+    x, w, b = randn(g, 2, 1, dtype=dt), far_rows(g, N, 1, cols, dt), far_rows(g, N, 1, cols, torch.float32)[:, 0]
+    dy = torch.zeros(2, N, dtype=dt, device="cuda")
+    dy[:, cols] = randn(g, 2, len(cols), dtype=dt)
+    got = run_linear(x, w, b, None, None, dy)
+    check_all({"y": got["y"][:, cols], "dx": got["dx"], "dw": got["dw"][cols], "db": got["db"][cols]}, O.linear(x, w[cols], b[cols], None, None, dy[:, cols]), "linear of many columns")
+    others = torch.tensor([9, (1 << 28) + 100, (1 << 30) + 9], device="cuda")
+    assert (got["y"][:, others] == 0).all() and (got["dw"][others] == 0).all() and (got["db"][others] == 0).all()
+    with torch.no_grad():
+        O.check(tokens.linear(x, w, b)[:, cols], O.linear(x, w[cols], b[cols], None, None)["y"], "linear of many columns, inference")
+    del w, b, dy, got
+    torch.cuda.empty_cache()
