@@ -1050,6 +1050,7 @@ class _TokenCall:
 
     def mat(self, t, name, rows, cols, dtype=None):
         """(pointer, row stride) of a [rows][cols] matrix"""
+        self.width(cols, name)
         dtype = self.dtype if dtype is None else dtype
         if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
             raise MisError(f"{self.who}: {name} must be a ({rows}, {cols}) {dtype} tensor on {self.device}, got {self.say(t)}")
@@ -1057,6 +1058,11 @@ class _TokenCall:
         if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
             raise MisError(f"{self.who}: {name} must have unit stride inside its rows and rows that do not overlap, got strides {(s0, s1)}")
         return t.data_ptr(), (s0 if rows > 1 else cols)
+
+    def width(self, n, name):
+        """widths are C ints (ctypes would cut a longer one to its low bits)"""
+        if n >= 1 << 31:
+            raise MisError(f"{self.who}: {name} has a width of 2^31 or more: {n}")
 
     def vec(self, t, name, n):
         """pointer of a contiguous f32 vector, None for None"""
@@ -1105,6 +1111,7 @@ def layernorm_bwd(dy, x, mean, rstd, gamma=None, dx=None, dgamma=None, dbeta=Non
 def _linear_desc(c, x, w, act):
     if x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 2:
         raise MisError(f"{c.who}: x and w must be matrices, got {c.say(x)} and {c.say(w)}")
+    c.width(x.shape[1], "x"), c.width(w.shape[0], "w")
     d = _lib.LinearDesc()
     d.dtype, d.act = c.code, token_act(act)
     d.M, d.K, d.N = x.shape[0], x.shape[1], w.shape[0]
@@ -1170,6 +1177,7 @@ def linear_bwd(dy, x, w, bias=None, act=None, kept=None, dx=None, dw=None, dbias
 def _gated_desc(c, x, wg, wu, act):
     if x.dim() != 2 or not isinstance(wg, torch.Tensor) or wg.dim() != 2:
         raise MisError(f"{c.who}: x, wg and wu must be matrices, got {c.say(x)}, {c.say(wg)}, {c.say(wu)}")
+    c.width(x.shape[1], "x"), c.width(wg.shape[0], "wg")
     d = _lib.GatedDesc()
     d.dtype, d.act = c.code, token_act(act)
     d.M, d.K, d.F = x.shape[0], x.shape[1], wg.shape[0]

@@ -21,6 +21,7 @@ from ._lib import MIS_BF16, MIS_F32, GatedDesc, LinearDesc, MisError, check, loa
 from .ops import token_act
 
 _F32, _BF16 = torch.float32, torch.bfloat16
+_WIDEST = (1 << 31) - 1          # widths are C ints (ctypes would cut a longer one to its low bits)
 _FEW = 32          # rows up to which a forward product needs no workspace (misamd.h): single tokens save the question
 
 
@@ -134,6 +135,8 @@ def _norm_fwd(x, weight, bias, eps, keep):
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         _refuse("layer_norm", f"x must be a (..., width) tensor, got {_say(x)}")
     D = x.shape[-1]
+    if D > _WIDEST:
+        _refuse("layer_norm", f"x has a width of 2^31 or more: {_say(x)}")
     x2, code = _tokens("layer_norm", x, D)
     M = x2.shape[0]
     pw, pb = _vec("layer_norm", weight, "weight", D, x2), _vec("layer_norm", bias, "bias", D, x2)
@@ -181,6 +184,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def _linear_fwd(x, weight, bias, act, residual, keep):
     w = _weight("linear", weight, "weight")
     N, K = w.shape
+    if (N | K) > _WIDEST:
+        _refuse("linear", f"weight has a width of 2^31 or more: {_say(w)}")
     x2, code = _tokens("linear", x, K)
     _like("linear", w, "weight", x2)
     M = x2.shape[0]
@@ -248,6 +253,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, keep):
     wg, wu = _weight("gated_ffn", w_gate, "w_gate"), _weight("gated_ffn", w_up, "w_up")
     F, K = wg.shape
+    if (F | K) > _WIDEST:
+        _refuse("gated_ffn", f"w_gate has a width of 2^31 or more: {_say(w_gate)}")
     if wu.shape != wg.shape:
         _refuse("gated_ffn", f"w_gate and w_up must have one shape, got {_say(w_gate)} and {_say(w_up)}")
     if F > 1 and wg.stride(0) != wu.stride(0):

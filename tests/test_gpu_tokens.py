@@ -648,3 +648,15 @@ def test_products_of_more_than_two_to_the_30_columns():
         O.check(tokens.linear(x, w, b)[:, cols], O.linear(x, w[cols], b[cols], None, None)["y"], "linear of many columns, inference")
     del w, b, dy, got
     torch.cuda.empty_cache()
+
+
+def test_widths_that_an_int_does_not_hold_are_refused_for_buffers():
+    wide, x = torch.empty(1, 1 << 32 | 64, dtype=torch.bfloat16, device="cuda"), torch.empty(1, 1, dtype=torch.bfloat16, device="cuda")
+    kept = torch.empty(64, dtype=torch.uint8, device="cuda")
+    for call in (lambda: ops.layernorm_fwd(wide, wide), lambda: ops.layernorm_bwd(wide, wide, x[0].float(), x[0].float()), lambda: ops.linear_fwd(wide, wide, x), lambda: ops.linear_fwd(x, wide.view(-1, 1), wide),
+                 lambda: ops.linear_kept_bytes(x, wide.view(-1, 1), None, "gelu"), lambda: ops.linear_bwd(wide, x, wide.view(-1, 1)), lambda: ops.gated_ffn_fwd(x, wide.view(-1, 1), wide.view(-1, 1), wide),
+                 lambda: ops.gated_ffn_bwd(x, wide, wide, wide, kept)):
+        with pytest.raises(MisError, match="2\\^31"):
+            call()
+    del wide
+    torch.cuda.empty_cache()

@@ -173,3 +173,12 @@ def test_jvp_of_a_token_operator_is_refused():
     x, w = torch.randn(4, 8), torch.randn(6, 8)
     with pytest.raises(MisError, match="tangent"):
         torch.func.jvp(lambda t: tokens.linear(t, w), (x,), (torch.ones_like(x),))
+
+
+# the C descriptors hold widths in 32 bits, and ctypes would cut a longer one to its low bits
+@pytest.mark.parametrize("call", [
+    lambda t: tokens.layer_norm(t(2, 1 << 32 | 64)), lambda t: tokens.linear(t(2, 1 << 32 | 64), t(4, 1 << 32 | 64)), lambda t: tokens.linear(t(2, 8), t(1 << 32 | 4, 8)),
+    lambda t: tokens.gated_ffn(t(2, 1 << 31), t(4, 1 << 31), t(4, 1 << 31)), lambda t: tokens.gated_ffn(t(2, 8), t(1 << 32 | 4, 8), t(1 << 32 | 4, 8))])
+def test_widths_that_an_int_does_not_hold_are_refused(call):
+    with pytest.raises(MisError, match="2\\^31"):
+        call(lambda *shape: torch.empty(*shape, device="meta"))
