@@ -120,6 +120,16 @@ def _new(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _saved(t):
+    """a saved matrix as the kernels read it: saved-tensor hooks may hand it back in another layout"""
+    return t if t.is_contiguous() else _unit(t)
+
+
+def _whole(t):
+    """... and what is no matrix of rows"""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _once(backward):
     """differentiable once: the plain function, unless a graph of the backward pass itself is asked for (then torch's wrapper, whose outputs refuse a second differentiation)"""
     wrapped = once_differentiable(backward)
@@ -158,6 +168,7 @@ class _LayerNorm(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         x, weight, st = ctx.saved_tensors
+        x, weight, st = _saved(x), _whole(weight), _whole(st)
         M, D = x.shape
         code = MIS_BF16 if x.dtype is _BF16 else MIS_F32
         nx, nw, nb, _ = ctx.needs_input_grad
@@ -225,6 +236,7 @@ class _Linear(torch.autograd.Function):
         if not (nx or nw or nb):
             return None, None, None, None, dres
         x, w, bias, kept = ctx.saved_tensors
+        x, w, kept = _saved(x), _saved(w), _whole(kept)
         M, K = x.shape
         N = w.shape[0]
         d2 = _rows("linear (backward)", dy, N, "dy")
@@ -287,6 +299,9 @@ class _GatedFFN(torch.autograd.Function):
     @_once
     def backward(ctx, dh):
         x, wg, wu, bg, bu, kept = ctx.saved_tensors
+        x, wg, wu, kept = _saved(x), _saved(wg), _saved(wu), _whole(kept)
+        if _ld(wg) != _ld(wu):
+            wg, wu = wg.contiguous(), wu.contiguous()
         nx, ng, nu, nbg, nbu, _ = ctx.needs_input_grad
         M, K = x.shape
         F = wg.shape[0]

@@ -660,3 +660,30 @@ def test_widths_that_an_int_does_not_hold_are_refused_for_buffers():
             call()
     del wide
     torch.cuda.empty_cache()
+
+
+# saved-tensor hooks may hand a tensor back in another layout than it was saved in (an offload that leaves parameters alone, say): rows closer together than those of its partner, columns first
+@pytest.mark.parametrize("change", [
+    lambda t: t.contiguous(), lambda t: t.t().contiguous().t() if t.dim() == 2 else t, lambda t: torch.nn.functional.pad(t, (0, 3))[:, :t.shape[1]] if t.dim() == 2 else t])
+@pytest.mark.parametrize("nth", [0, 1, 2, 3, None])
+def test_saved_tensors_that_come_back_in_another_layout(nth, change):
+    g = gen(61)
+    x, w, v, dy, gam = odd(randn(g, 40, 24)), randn(g, 30, 48)[:, :24], randn(g, 30, 48)[:, 24:], randn(g, 40, 30), randn(g, 24)
+    xd, dx = randn(g, 40, 24), randn(g, 40, 24)
+    seen = []
+
+    def pack(t):
+        seen.append(len(seen))
+        return t, seen[-1]
+
+    def unpack(p):
+        return change(p[0]) if nth is None or p[1] == nth else p[0]
+
+    def run(f, *a):
+        seen.clear()
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            return f(*a)
+
+    check_all(run(run_gated, x, w, v, None, None, "silu", dy), O.gated(x, w, v, None, None, "silu", dy), "gated")
+    check_all(run(run_linear, x, w, None, "gelu", None, dy), O.linear(x, w, None, "gelu", None, dy), "linear")
+    check_all(run(run_layer_norm, xd, gam, gam, dx), O.layer_norm(xd, gam, gam, 1e-5, dx), "layer_norm")
