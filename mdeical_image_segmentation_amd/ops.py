@@ -1055,8 +1055,8 @@ class _TokenCall:
         if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != dtype or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
             raise MisError(f"{self.who}: {name} must be a ({rows}, {cols}) {dtype} tensor on {self.device}, got {self.say(t)}")
         s0, s1 = t.stride()
-        if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
-            raise MisError(f"{self.who}: {name} must have unit stride inside its rows and rows that do not overlap, got strides {(s0, s1)}")
+        if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1) or t.is_neg():
+            raise MisError(f"{self.who}: {name} must have unit stride inside its rows, rows that do not overlap and no negation pending, got strides {(s0, s1)}")
         return t.data_ptr(), (s0 if rows > 1 else cols)
 
     def width(self, n, name):
@@ -1068,7 +1068,7 @@ class _TokenCall:
         """pointer of a contiguous f32 vector, None for None"""
         if t is None:
             return None
-        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.is_neg():
             raise MisError(f"{self.who}: {name} must be a contiguous ({n},) float32 tensor on {self.device}, got {self.say(t)}")
         return t.data_ptr()
 

@@ -34,7 +34,9 @@ def _say(t):
 
 
 def _unit(t):
-    """a matrix with unit stride inside its rows and rows that do not overlap: itself, or a copy"""
+    """a matrix with unit stride inside its rows, rows that do not overlap and no negation pending: itself, or a copy"""
+    if t.is_neg():
+        return t.resolve_neg().contiguous()
     s0, s1 = t.stride()
     return t if (s1 == 1 or t.shape[1] == 1) and (s0 >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
@@ -45,7 +47,7 @@ def _rows(who, t, width, name="x"):
         _refuse(who, f"{name} must be a (..., {width}) tensor, got {_say(t)}")
     if t.dim() != 2:
         t = t.reshape(t.numel() // width, width)
-    return t if t.is_contiguous() else _unit(t)
+    return t if width > 1 and t.is_contiguous() else _unit(t)          # (a pending negation, from the imaginary part of a conjugate, leaves only one column contiguous)
 
 
 def _tokens(who, x, width):
@@ -62,7 +64,7 @@ def _tokens(who, x, width):
 def _weight(who, w, name):
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         _refuse(who, f"{name} must be an (out, in) matrix, got {_say(w)}")
-    return w if w.is_contiguous() else _unit(w)
+    return w if w.is_contiguous() and w.shape[1] > 1 else _unit(w)
 
 
 def _like(who, t, name, x):
@@ -74,7 +76,7 @@ def _vec(who, v, name, n, x):
     """pointer of a float32 vector of n, None for None"""
     if v is None:
         return None
-    if not isinstance(v, torch.Tensor) or v.dtype is not _F32 or v.dim() != 1 or v.shape[0] != n or v.device != x.device or not v.is_contiguous():
+    if not isinstance(v, torch.Tensor) or v.dtype is not _F32 or v.dim() != 1 or v.shape[0] != n or v.device != x.device or not v.is_contiguous() or (n == 1 and v.is_neg()):
         _refuse(who, f"{name} must be a contiguous ({n},) float32 tensor on {x.device}, got {_say(v)}")
     return v.data_ptr()
 

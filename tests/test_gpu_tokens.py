@@ -687,3 +687,17 @@ def test_saved_tensors_that_come_back_in_another_layout(nth, change):
     check_all(run(run_gated, x, w, v, None, None, "silu", dy), O.gated(x, w, v, None, None, "silu", dy), "gated")
     check_all(run(run_linear, x, w, None, "gelu", None, dy), O.linear(x, w, None, "gelu", None, dy), "linear")
     check_all(run(run_layer_norm, xd, gam, gam, dx), O.layer_norm(xd, gam, gam, 1e-5, dx), "layer_norm")
+
+
+def test_pending_negations():
+    g = gen(71)
+    z = torch.complex(randn(g, 5, 1), randn(g, 5, 1)).conj().imag
+    x, w, dy = z.clone(), randn(g, 6, 1), randn(g, 5, 6)
+    assert z.is_neg() and not x.is_neg()
+    check_all(run_linear(z, w, None, "gelu", None, dy), O.linear(x, w, None, "gelu", None, dy), "x")
+    check_all(run_linear(w, z, None, "gelu", None, dy.t().contiguous()), O.linear(w, x, None, "gelu", None, dy.t().contiguous()), "weight")
+    r = randn(g, 1, 1)
+    check_all(run_linear(x, r, None, None, z, x), O.linear(x, r, None, None, x, x), "residual")
+    for call in (lambda: ops.linear_fwd(z, w, dy), lambda: ops.linear_fwd(x, r, x.clone(), z[0]), lambda: tokens.linear(x, r, z[0])):
+        with pytest.raises(MisError):
+            call()

@@ -182,3 +182,16 @@ def test_jvp_of_a_token_operator_is_refused():
 def test_widths_that_an_int_does_not_hold_are_refused(call):
     with pytest.raises(MisError, match="2\\^31"):
         call(lambda *shape: torch.empty(*shape, device="meta"))
+
+
+def test_rows_with_a_pending_negation_are_resolved():
+    # the imaginary part of a conjugate is a view whose sign torch flips when it reads it; one column of it has rows that look like the kernels' own
+    z = torch.complex(torch.randn(5, 1), torch.randn(5, 1)).conj().imag
+    assert z.is_neg()
+    for t in (z, z[:1]):
+        r = tokens._rows("test", t, 1)
+        assert not r.is_neg() and torch.equal(r, t)
+        w = tokens._weight("test", t, "weight")
+        assert not w.is_neg() and torch.equal(w, t)
+    with pytest.raises(MisError, match="bias"):
+        tokens._vec("test", z[0], "bias", 1, z)
