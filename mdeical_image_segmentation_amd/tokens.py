@@ -33,6 +33,12 @@ def _say(t):
     return f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
 
 
+def _no_width(who, t, name, n):
+    if type(n) is not int:          # (torch.jit.trace makes tensors of sizes; it would record the outputs' allocation and lose the kernels)
+        _refuse(who, f"cannot be traced: the sizes of {name} are no integers")
+    _refuse(who, f"{name} has a width of 2^31 or more: {_say(t)}")
+
+
 def _unit(t):
     """a matrix with unit stride inside its rows, rows that do not overlap and no negation pending: itself, or a copy"""
     if t.is_neg():
@@ -147,8 +153,8 @@ def _norm_fwd(x, weight, bias, eps, keep):
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         _refuse("layer_norm", f"x must be a (..., width) tensor, got {_say(x)}")
     D = x.shape[-1]
-    if D > _WIDEST:
-        _refuse("layer_norm", f"x has a width of 2^31 or more: {_say(x)}")
+    if type(D) is not int or D > _WIDEST:
+        _no_width("layer_norm", x, "x", D)
     x2, code = _tokens("layer_norm", x, D)
     M = x2.shape[0]
     pw, pb = _vec("layer_norm", weight, "weight", D, x2), _vec("layer_norm", bias, "bias", D, x2)
@@ -197,8 +203,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 def _linear_fwd(x, weight, bias, act, residual, keep):
     w = _weight("linear", weight, "weight")
     N, K = w.shape
-    if (N | K) > _WIDEST:
-        _refuse("linear", f"weight has a width of 2^31 or more: {_say(w)}")
+    if type(K) is not int or (N | K) > _WIDEST:
+        _no_width("linear", weight, "weight", K)
     x2, code = _tokens("linear", x, K)
     _like("linear", w, "weight", x2)
     M = x2.shape[0]
@@ -267,8 +273,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, keep):
     wg, wu = _weight("gated_ffn", w_gate, "w_gate"), _weight("gated_ffn", w_up, "w_up")
     F, K = wg.shape
-    if (F | K) > _WIDEST:
-        _refuse("gated_ffn", f"w_gate has a width of 2^31 or more: {_say(w_gate)}")
+    if type(K) is not int or (F | K) > _WIDEST:
+        _no_width("gated_ffn", w_gate, "w_gate", K)
     if wu.shape != wg.shape:
         _refuse("gated_ffn", f"w_gate and w_up must have one shape, got {_say(w_gate)} and {_say(w_up)}")
     if F > 1 and wg.stride(0) != wu.stride(0):

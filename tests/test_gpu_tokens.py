@@ -701,3 +701,23 @@ def test_pending_negations():
     for call in (lambda: ops.linear_fwd(z, w, dy), lambda: ops.linear_fwd(x, r, x.clone(), z[0]), lambda: tokens.linear(x, r, z[0])):
         with pytest.raises(MisError):
             call()
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_transforms_are_refused_and_hooks_are_called():
+    # what looks behind a tensor's data cannot see the kernels: function transforms and tracing raise instead of losing the call; hooks see the gradients as of any function
+    g = gen(81)
+    x, w, dy = randn(g, 5, 8), randn(g, 6, 8), randn(g, 5, 6)
+    for f in (lambda t: tokens.linear(t, w), lambda t: tokens.gated_ffn(t, w, w), lambda t: tokens.layer_norm(t)):
+        for call in (lambda: torch.func.vmap(f)(x[None]), lambda: torch.func.grad(lambda t: f(t).sum())(x), lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.jit.trace(f, (x,), check_trace=False)):
+            with pytest.raises(Exception):
+                call()
+    xl, seen = leaf(x), []
+    y = tokens.linear(xl, w, None, "silu")
+    y.register_hook(lambda d: 2 * d)
+    xl.register_hook(seen.append)
+    y.backward(dy)
+    O.check(xl.grad, O.linear(x, w, None, "silu", None, 2 * dy)["dx"], "dx behind a hook")
+    assert len(seen) == 1 and torch.equal(seen[0], xl.grad)
+    with torch.autograd.forward_ad.dual_level():        # no tangent: an ordinary call
+        O.check(tokens.linear(x, w), O.linear(x, w, None, None, None)["y"], "in a dual level")

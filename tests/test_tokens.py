@@ -195,3 +195,12 @@ def test_rows_with_a_pending_negation_are_resolved():
         assert not w.is_neg() and torch.equal(w, t)
     with pytest.raises(MisError, match="bias"):
         tokens._vec("test", z[0], "bias", 1, z)
+
+
+# a trace would record the outputs' allocation and lose the kernels
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_is_refused():
+    x, w = torch.randn(4, 8), torch.randn(6, 8)
+    for f in (lambda t: tokens.layer_norm(t), lambda t: tokens.linear(t, w), lambda t: tokens.gated_ffn(t, w, w)):
+        with pytest.raises(MisError, match="traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
