@@ -13,6 +13,7 @@
 //      16384 x 2048     26.4 / 45.0   5.1, 4.5                  44.2 / 85.4   6.1, 4.7           (four waves a row: 29.2 / 57.8, 40.3 / 77.7)
 //      8192 x 4096      23.7 / 44.5   5.7, 4.5                  43.4 / 82.2   6.2, 4.9           (read again: 28.6 / 72.1, 59.6 / 141)
 //      2048 x 16384     39.7 / 80.4   3.4, 2.5                  75.9 / 141    3.5, 2.9
+//      8192 x 2056      19.2 / 34.3   3.5, 2.9                  24.0 / 41.7   5.6, 4.9           (just past a power of two: half of the lanes have nothing)
 #include <type_traits>
 
 #include "tok_common.hpp"

@@ -85,9 +85,9 @@ namespace {
 //                                       256      128       64                                          256      128       64
 //      512 x 512 x 512       x W^T       17       11     *8.6      2048 x 2048 x 2048       dz W       40      *27       33
 //      1024 x 4096 x 1024    x W^T       32      *24       25      4096 x 4096 x 1024       dz W      *33       42       63
-//      2048 x 2048 x 2048    x W^T       45      *27       31      8192 x 1024 x 4096       dz^T x    *76       88      118
-//      8192 x 1024 x 4096    x W^T      *61       82      119      8192 x 1024 x 4096       gated    *110      148      175
-//      8192 x 2048 x 8192    x W^T     *211      294      440      f32 8192 x 1024 x 4096   x W^T       -     *510      527
+//      2048 x 2048 x 2048    x W^T       44      *27       31      8192 x 1024 x 4096       dz^T x    *76       88      118
+//      8192 x 1024 x 4096    x W^T      *65       82      119      8192 x 1024 x 4096       gated    *112      148      175
+//      8192 x 2048 x 8192    x W^T     *214      294      440      f32 8192 x 1024 x 4096   x W^T       -     *510      527
 // A forward product in parts (its epilogue then runs where they are added), us against one piece: 128 x 4096 x 1024 bf16 14 / 29, 128 x 8192 x 8192 38 / 64, f32 512 x 4096 x 1024 47 / 105.
 struct TgCut {
     int tile;               // 256, 128 or 64 rows

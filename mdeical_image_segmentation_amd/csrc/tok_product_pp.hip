@@ -13,7 +13,7 @@
 // in front of its first read, by a count that leaves group 0's four A(s+2) in flight.  The step sequence is flat over a block's tiles (grid = number of CUs), so a tile's first steps are in flight while the tile before is finished and stored.
 // LDS images and swizzles are those of tok_product.hpp with 256 rows: [row][128 B] for a k-contiguous operand, [k][512 B] for the other kind, read with the transposing ds_read_b64_tr_b16.
 // Bound: per step 192 KiB of fragments leave and 64 KiB enter the LDS, 2048 cycles at its 128 B a cycle - as many as the MFMAs take, so every cycle of a segment that is neither shows.
-// 8192^3 759 us, 1.45 PFLOP/s (x W^T; dz W 767, dz^T x 818); 32768 x 1024 x 8192, 16 steps a tile: 492 us, 1.12, of which 4 to 5 steps' time a tile is the store of its 128 KiB.  A wave
+// 8192^3 770 us, 1.43 PFLOP/s (x W^T; dz W 783, dz^T x 837); 32768 x 1024 x 8192, 16 steps a tile: 493 us, 1.11, of which 4 to 5 steps' time a tile is the store of its 128 KiB.  A wave
 // tile of 128 x 128 would need a third less from the LDS, but 256 accumulators and 64 fragment registers a lane do not fit beside the addresses.
 // The fragment reads and their wait are one asm statement: hipcc would put a vmcnt(0), i.e. a wait for the prefetch, in front of a plain LDS read while an LDS-DMA is in flight.
 
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(512, 2) void tg_pp_kernel(const TgArgs a, const TpP
         barrier();
         if (--crem == 0) {
             // ---- the tile is complete: group 0 waits for group 1's last M, and both store at once (one after the other they would leave each SIMD to one wave's dependent VALU
-            // instructions: 32768 x 1024 x 2 x 4096 with SiLU 600 -> 536 us) ----
+            // instructions: 32768 x 1024 x 2 x 4096 with SiLU and half the bytes kept 600 -> 536 us; with all of them 616, with none 454) ----
             if (grp == 0) barrier();
             if constexpr (EPI == TG_GATED) {
                 const TgGatedRow<T, ACT> row(a, ct.n0 + wn * 32 + 8 * lg);
