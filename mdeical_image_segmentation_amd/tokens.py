@@ -110,12 +110,17 @@ def _scratch(nbytes, x):
     return torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
 
 
+def _no_tangents(who, *ts):
+    """a forward-mode tangent, which the kernels would drop, is refused"""
+    for t in ts:
+        if isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None:
+            _refuse(who, f"differentiable in reverse mode only, got a tensor with a forward-mode tangent: {_say(t)}")
+
+
 def _wanted(who, *ts):
-    """whether a gradient is (what is not a tensor is refused by the forward pass's checks); a forward-mode tangent, which the kernels would drop, is refused"""
+    """whether a gradient is (what is not a tensor is refused by the forward pass's checks)"""
     if _fw._current_level >= 0:
-        for t in ts:
-            if isinstance(t, torch.Tensor) and _fw.unpack_dual(t).tangent is not None:
-                _refuse(who, f"differentiable in reverse mode only, got a tensor with a forward-mode tangent: {_say(t)}")
+        _no_tangents(who, *ts)
     if torch.is_grad_enabled():
         for t in ts:
             if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -143,6 +148,8 @@ def _once(backward):
     wrapped = once_differentiable(backward)
 
     def run(ctx, dy):
+        if _fw._current_level >= 0:
+            _no_tangents("token operator (backward)", dy)
         return wrapped(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
 
     return staticmethod(run)

@@ -721,3 +721,29 @@ def test_transforms_are_refused_and_hooks_are_called():
     assert len(seen) == 1 and torch.equal(seen[0], xl.grad)
     with torch.autograd.forward_ad.dual_level():        # no tangent: an ordinary call
         O.check(tokens.linear(x, w), O.linear(x, w, None, None, None)["y"], "in a dual level")
+
+
+def test_a_tangent_of_the_arriving_gradient_is_refused():
+    import torch.autograd.forward_ad as fw
+    g = gen(91)
+    x, w, dy, d2 = leaf(randn(g, 5, 8)), leaf(randn(g, 6, 8)), randn(g, 5, 6), randn(g, 5, 8)
+    for y, d in ((tokens.linear(x, w, None, "silu"), dy), (tokens.linear(x, w), dy), (tokens.gated_ffn(x, w, w), dy), (tokens.layer_norm(x), d2)):
+        with fw.dual_level(), pytest.raises(MisError, match="tangent"):
+            torch.autograd.grad(y, x, fw.make_dual(d, torch.ones_like(d)), retain_graph=True)
+        assert torch.isfinite(torch.autograd.grad(y, x, d)[0]).all()
+
+
+def test_compiled_callers_get_the_eager_results():
+    # torch.compile cannot look into the kernels: it runs the call between the graphs on its two sides
+    g = gen(92)
+    x, w, dy = randn(g, 40, 24), randn(g, 30, 24), randn(g, 40, 30)
+
+    def f(x, w):
+        return tokens.linear(torch.nn.functional.relu(x), w, None, "silu") * 2
+
+    xl, wl = leaf(x), leaf(w)
+    c = torch.compile(f, backend="eager")
+    with torch.no_grad():
+        assert torch.equal(c(x, w), f(x, w))
+    for a, b in zip(torch.autograd.grad(c(xl, wl), (xl, wl), dy), torch.autograd.grad(f(xl, wl), (xl, wl), dy)):
+        assert torch.equal(a, b)
